@@ -32,6 +32,26 @@ pub struct FkMatvecLaunch {
     pub n_blocks_per_row: c_int,
 }
 
+/// `fk_pages`: a paged KV cache; all device memory is the caller's.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct FkPages {
+    pub data_dev: *mut c_void,
+    pub table_dev: *mut c_int,
+    pub lens_dev: *mut c_int,
+    pub refs_dev: *mut c_int,
+    pub ws_dev: *mut c_void,
+    pub ws_bytes: usize,
+    pub kind: c_int,
+    pub n_layers: c_int,
+    pub n_pages: c_int,
+    pub page: c_int,
+    pub n_kv: c_int,
+    pub head_dim: c_int,
+    pub n_seqs: c_int,
+    pub max_pages: c_int,
+}
+
 /// `fk_status`.
 pub const FK_OK: c_int = 0;
 pub const FK_DRIVER_INIT: c_int = 1;
@@ -627,6 +647,97 @@ extern "C" {
         out_dev: *mut c_int,
     ) -> c_int;
     pub fn fk_add_int(ctx: *mut FkCtx, stream: *mut c_void, p_dev: *mut c_int, v: c_int) -> c_int;
+    pub fn fk_pages_workspace(ctx: *mut FkCtx, n_pages: c_int) -> usize;
+    pub fn fk_pages_grow(
+        ctx: *mut FkCtx,
+        stream: *mut c_void,
+        pages: *const FkPages,
+        n_new_dev: *const c_int,
+        n_new: c_int,
+    ) -> c_int;
+    pub fn fk_pages_advance(
+        ctx: *mut FkCtx,
+        stream: *mut c_void,
+        pages: *const FkPages,
+        n_new_dev: *const c_int,
+        n_new: c_int,
+    ) -> c_int;
+    pub fn fk_pages_fork(
+        ctx: *mut FkCtx,
+        stream: *mut c_void,
+        pages: *const FkPages,
+        src_host: *const c_int,
+        dst_host: *const c_int,
+        n_host: *const c_int,
+        m: c_int,
+    ) -> c_int;
+    pub fn fk_pages_free(
+        ctx: *mut FkCtx,
+        stream: *mut c_void,
+        pages: *const FkPages,
+        seqs_host: *const c_int,
+        m: c_int,
+    ) -> c_int;
+    pub fn fk_pages_compact(
+        ctx: *mut FkCtx,
+        stream: *mut c_void,
+        pages: *const FkPages,
+        used_dev: *mut c_int,
+    ) -> c_int;
+    pub fn fk_rope_kv_paged(
+        ctx: *mut FkCtx,
+        stream: *mut c_void,
+        pages: *const FkPages,
+        layer: c_int,
+        q_dev: *const f32,
+        k_dev: *const f32,
+        v_dev: *const f32,
+        q_ld: c_int,
+        k_ld: c_int,
+        v_ld: c_int,
+        rows: c_int,
+        n_new_dev: *const c_int,
+        n_heads: c_int,
+        theta: f32,
+        neox: c_int,
+        q_norm_dev: *const f32,
+        k_norm_dev: *const f32,
+        norm_eps: f32,
+        q_out_dev: *mut f32,
+    ) -> c_int;
+    pub fn fk_attention_paged(
+        ctx: *mut FkCtx,
+        stream: *mut c_void,
+        pages: *const FkPages,
+        layer: c_int,
+        q_dev: *const f32,
+        q_ld: c_int,
+        rows: c_int,
+        n_new_dev: *const c_int,
+        n_heads: c_int,
+        scale: f32,
+        window: c_int,
+        first: c_int,
+        sinks_dev: *const f32,
+        out_dev: *mut f32,
+    ) -> c_int;
+    pub fn fk_logit_rules(
+        ctx: *mut FkCtx,
+        stream: *mut c_void,
+        logits_dev: *const f32,
+        ld: usize,
+        n_rows: c_int,
+        vocab: c_int,
+        history_dev: *const c_int,
+        history: c_int,
+        penalties_dev: *const f32,
+        bias_dev: *const f32,
+        bias_ld: usize,
+        mask_dev: *const c_int,
+        mask_ld: usize,
+        out_dev: *mut f32,
+        tokens_dev: *mut c_int,
+    ) -> c_int;
     pub fn fk_comm_create(
         ctx: *mut FkCtx,
         arena_bytes: usize,

@@ -8,7 +8,7 @@ import re
 
 ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 TYPES = {"int": "c_int", "float": "f32", "size_t": "usize", "uint64_t": "u64", "int32_t": "i32", "uint8_t": "u8", "char": "c_char", "void": "c_void",
-         "fk_ctx": "FkCtx", "fk_comm": "FkComm", "fk_matvec_launch": "FkMatvecLaunch"}
+         "fk_ctx": "FkCtx", "fk_comm": "FkComm", "fk_matvec_launch": "FkMatvecLaunch", "fk_pages": "FkPages"}
 
 HEAD = '''//! Raw declarations of `libfrink_b200.so`'s C ABI, one per entry point of `include/frink_b200.h`, in the
 //! header's order and with the header's argument names (written by `bindings/rust/gen_sys.py`).  Semantics,
@@ -42,6 +42,26 @@ pub struct FkMatvecLaunch {
     pub rows: c_int,
     pub row_bytes: c_int,
     pub n_blocks_per_row: c_int,
+}
+
+/// `fk_pages`: a paged KV cache; all device memory is the caller's.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct FkPages {
+    pub data_dev: *mut c_void,
+    pub table_dev: *mut c_int,
+    pub lens_dev: *mut c_int,
+    pub refs_dev: *mut c_int,
+    pub ws_dev: *mut c_void,
+    pub ws_bytes: usize,
+    pub kind: c_int,
+    pub n_layers: c_int,
+    pub n_pages: c_int,
+    pub page: c_int,
+    pub n_kv: c_int,
+    pub head_dim: c_int,
+    pub n_seqs: c_int,
+    pub max_pages: c_int,
 }
 
 /// `fk_status`.
@@ -79,7 +99,7 @@ def rust_type(t):
 def main():
     h = open(os.path.join(ROOT, "include", "frink_b200.h")).read()
     h = re.sub(r"/\*.*?\*/", "", h, flags=re.S)
-    h = re.sub(r"typedef struct fk_matvec_launch \{.*?\} fk_matvec_launch;", "", h, flags=re.S)
+    h = re.sub(r"typedef struct (fk_matvec_launch|fk_pages) \{.*?\} \1;", "", h, flags=re.S)
     decls = re.findall(r"\n((?:int|void|size_t|const char\*)\s+fk_\w+\s*\([^;]*\));", h)
     out = []
     for d in decls:

@@ -1,0 +1,680 @@
+// Attention over a paged KV cache: causal, grouped-query, with an optional window, first tokens that stay visible and a sink
+// logit per head.  One new row a sequence (decode) or a few.
+//
+//   o = sum_j w_j v_j / (sum_j w_j + exp(sink)),  w_j = exp(scale q.k_j)  over the visible keys j
+//
+// kept as a running maximum m, a denominator l and unnormalised sums, so every key and value is read once; partial results of
+// a split are joined by m.  All exponentials are powers of two (scale and log2 e go into q).
+//
+// Matrix products.  A warp takes 16 tokens of one KV head and 8 or 16 columns; a column is one (row, query head) pair of the
+// group, so that all query heads of a KV head share one read of its keys.  Scores are K (16 tokens x 16 dims) times q
+// (16 dims x 8 columns), outputs are V^T (16 dims x 16 tokens) times w (16 tokens x 8 columns), both mma.m16n8k16 with f32
+// sums.  K and V go from global memory straight into operand registers, 16 bytes a lane: which dims a lane's piece holds is
+// free as long as both operands agree, so the order of dims is permuted instead of the data.  The scores' fragment becomes the
+// weights' operand by a transposition of 8 x 8 blocks inside the warp (movmatrix).
+//
+// Precision.  The cache's 16-bit values are exact operands.  q and w are f32 and are split into parts of the cache's type:
+// three bf16 parts hold all 24 bits; two f16 parts hold 22, their range kept by a power of two per column of q and by a
+// factor 2^14 on w.  f32 pages are split like q into three bf16 parts and the six products above 2^-24 are kept.  The tensor
+// cores' own running sums are cut off rather than rounded, which over thousands of tiles adds up to a bias, so a product of
+// a few steps starts from zero and joins the running sum in an ordinary, rounded addition.
+//
+// Work.  The keys of every (sequence, block of columns, KV head) are cut into units of 64 tokens (16 a warp) and all units,
+// one after another, are dealt out in equal runs to the CTAs of one grid, so that ragged lengths keep every SM busy and the
+// grid does not depend on lengths that only the device knows.  A run's first and last item may be shared with other CTAs: their
+// partial sums go to a record of the CTA, and the CTA that arrives last joins them.
+#include "fk_paged.cuh"
+
+#include <type_traits>
+
+using namespace fk_paged;
+
+namespace {
+
+constexpr int WARPS = 4;
+constexpr int MAX_ENTRIES = 2048;          // (sequence, block of columns) pairs that are dealt out in runs
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct AttnArgs {
+    const void* data;                      // the layer's pages
+    const int *table, *lens, *n_new;
+    const float *q, *sinks;
+    float* out;
+    unsigned* cnt;
+    float* rec;
+    int* err;
+    float scale;
+    int q_ld, rows, n_seqs, n_heads, n_kv, group, head_dim, page, n_pages, max_pages, window, first, n_cb, whole;
+};
+
+// ---- operand types
+template <int KIND> struct Kind;
+template <> struct Kind<KIND_F16> { static constexpr int Q = 2; };
+template <> struct Kind<FK_BF16> { static constexpr int Q = 3; };
+template <> struct Kind<KIND_F32> { static constexpr int Q = 3; };
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// (lo, hi) as parts: parts[0] the nearest pair of the type, parts[1] the nearest to what is left, ...
+template <int KIND> __device__ __forceinline__ void split_pair(float lo, float hi, uint32_t* parts) {
+    if (KIND == KIND_F16) {
+        parts[0] = pack_f16(lo, hi);
+        const __half2 h = *(const __half2*)&parts[0];
+        parts[1] = pack_f16(lo - __low2float(h), hi - __high2float(h));
+    } else {
+        parts[0] = pack_bf16(lo, hi);
+        lo -= __uint_as_float(parts[0] << 16);
+        hi -= __uint_as_float(parts[0] & 0xffff0000u);
+        parts[1] = pack_bf16(lo, hi);
+        lo -= __uint_as_float(parts[1] << 16);
+        hi -= __uint_as_float(parts[1] & 0xffff0000u);
+        parts[2] = pack_bf16(lo, hi);
+    }
+}
+template <int KIND> __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if (KIND == KIND_F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ float pow2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint4 ld16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// ---- which keys an item sees: those below `hi`, in tiles of 16: [0, na) and then [b0, ...)
+struct Span {
+    int n;          // rows of the sequence
+    int base;       // its length before them
+    int lo;         // the oldest key of the window of the block's first row (0: no window)
+    int hi;         // keys below this
+    int na, b0, tiles;
+};
+template <int COLS> __device__ __forceinline__ Span span_of(const AttnArgs& a, int s, int cb, bool raise) {
+    Span r;
+    r.n = a.n_new ? min(max(a.n_new[s], 0), a.rows) : a.rows;
+    r.base = a.lens[s];
+    if (r.base < 0 || (long long)r.base + r.n > (long long)a.max_pages * a.page) {
+        if (raise && r.n > 0) fk_raise(a.err, 95);
+        r.n = 0;
+    }
+    const int row0 = cb * COLS / a.group, row1 = min((cb * COLS + COLS - 1) / a.group, r.n - 1);
+    r.lo = r.hi = r.na = r.b0 = r.tiles = 0;
+    if (row1 < row0) return r;                         // no real row in the block
+    r.hi = r.base + row1 + 1;
+    r.lo = a.window > 0 ? max(0, r.base + row0 + 1 - a.window) : 0;
+    r.b0 = r.lo >> 4;
+    r.na = (min(a.first, r.lo) + 15) >> 4;
+    if (r.na >= r.b0) r.na = r.b0 = 0;
+    r.tiles = r.na + ((r.hi + 15) >> 4) - r.b0;
+    return r;
+}
+
+template <int KIND, int HDP, int NT> struct Smem {
+    uint4 q[NT][HDP / 32][Kind<KIND>::Q][32];          // q's operand registers, part by part
+    float qscale[NT * 8];                              // 2^-e of a column whose q was scaled by 2^e (f16)
+    float o[WARPS][NT * 8][HDP];
+    float m[WARPS][NT * 8], l[WARPS][NT * 8];
+    int start[MAX_ENTRIES + 1];                        // first unit of every (sequence, block of columns)
+    int part[33];
+    int last;
+};
+
+template <int KIND, int HDP, int NT>
+__global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a) {
+    pdl_sync();
+    constexpr int COLS = 8 * NT, KB = HDP / 32, VB = HDP / 64, QP = Kind<KIND>::Q;
+    constexpr float SHIFT = KIND == KIND_F16 ? 14.0f : 0.0f;       // weights are 2^SHIFT times exp(score - m)
+    using T = typename std::conditional<KIND == KIND_F32, float, uint16_t>::type;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    Smem<KIND, HDP, NT>& sm = *reinterpret_cast<Smem<KIND, HDP, NT>*>(smem_raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int hd = a.head_dim, n_e = a.n_seqs * a.n_cb;
+
+    // ---- this CTA's run of units [u, u_end); sm.start[e]: units before entry e (per KV head), times n_kv in the global order
+    int u, u_end, chunk;
+    if (a.whole) {                                                 // one item a CTA: blockIdx.x = entry * n_kv + kv head
+        u = 0;
+        u_end = 1;
+        chunk = 1;
+    } else {
+        int total = 0;
+        for (int e0 = 0; e0 < n_e; e0 += WARPS * 32) {
+            const int e = e0 + tid;
+            const int units = e < n_e ? (span_of<COLS>(a, e / a.n_cb, e % a.n_cb, blockIdx.x == 0).tiles + WARPS - 1) / WARPS : 0;
+            int sum;
+            const int at = block_prefix(units, sm.part, &sum);
+            if (e < n_e) sm.start[e] = total + at;
+            total += sum;
+            __syncthreads();
+        }
+        if (tid == 0) sm.start[n_e] = total;
+        __syncthreads();
+        const long long all = (long long)total * a.n_kv;
+        if (all > 0x3fffffffLL) {                                  // no cache holds that many; table rows that share pages could claim it
+            if (blockIdx.x == 0 && tid == 0) fk_raise(a.err, 95);
+            return;
+        }
+        chunk = (int)((all + gridDim.x - 1) / gridDim.x);
+        const long long b = (long long)blockIdx.x * chunk;
+        u = (int)(b < all ? b : all);
+        u_end = (int)(b + chunk < all ? b + chunk : all);
+    }
+    const int u_begin = u;
+
+    while (u < u_end) {
+        int e, kvh, i0, i1, item0 = 0, units;                      // units [i0, i1) of the item, the item's first unit
+        if (a.whole) {
+            e = blockIdx.x / a.n_kv;
+            kvh = blockIdx.x % a.n_kv;
+        } else {
+            int lo = 0, hi = n_e - 1;                              // the last entry that starts at or before u
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if ((long long)sm.start[mid] * a.n_kv <= u) lo = mid; else hi = mid - 1;
+            }
+            e = lo;
+        }
+        const int s = e / a.n_cb, cb = e % a.n_cb;
+        const Span sp = span_of<COLS>(a, s, cb, a.whole && tid == 0);
+        units = (sp.tiles + WARPS - 1) / WARPS;
+        if (a.whole) {
+            if (units == 0) return;
+            i0 = 0;
+            i1 = units;
+            u = 1;
+        } else {
+            kvh = (u - sm.start[e] * a.n_kv) / units;
+            item0 = sm.start[e] * a.n_kv + kvh * units;
+            i0 = u - item0;
+            i1 = min(units, u_end - item0);
+            u = item0 + i1;
+        }
+
+        // ---- q of the item's columns into operand registers' order, scaled, split into parts
+        __syncthreads();                                           // the previous item's shared memory is read
+        if (warp < NT) {
+            const int c = cb * COLS + warp * 8 + g, row = c / a.group, h = kvh * a.group + c % a.group;
+            const bool on = row < sp.n;
+            const float* qr = a.q + ((size_t)s * a.rows + row) * a.q_ld + (size_t)h * hd;
+            float v[KB][8], top = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+                const int d = 32 * kb + 8 * t;
+                float4 x = make_float4(0, 0, 0, 0), y = x;
+                if (on && d < hd) {
+                    x = *(const float4*)(qr + d);
+                    y = *(const float4*)(qr + d + 4);
+                }
+                const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    v[kb][j] = w[j] * (a.scale * LOG2E);
+                    top = fmaxf(top, fabsf(v[kb][j]));
+                }
+            }
+            if (KIND == KIND_F16) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // 2^e with top * 2^e in [2^13, 2^14): no part leaves f16's range, and the low part keeps its bits
+                int ex = top > 0.0f && top < INFINITY ? 13 - (int)((__float_as_uint(top) >> 23) & 255) + 127 : 0;
+                ex = max(-100, min(100, ex));
+                const float f = __uint_as_float((uint32_t)(127 + ex) << 23);
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[kb][j] *= f;
+                if (t == 0) sm.qscale[warp * 8 + g] = __uint_as_float((uint32_t)(127 - ex) << 23);
+            }
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+                uint32_t p[4][3];
+#pragma unroll
+                for (int j = 0; j < 4; j++) split_pair<KIND>(v[kb][2 * j], v[kb][2 * j + 1], p[j]);
+#pragma unroll
+                for (int k = 0; k < QP; k++) sm.q[warp][kb][k][lane] = make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
+            }
+        }
+        __syncthreads();
+
+        // ---- this lane's columns: 2t and 2t + 1 of every block of 8
+        int p_c[NT][2];                                            // position of the column's row; -1: no such column
+        float cs[NT][2];
+        int p_min = 0x7fffffff, p_max = -1;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int row = (cb * COLS + n * 8 + 2 * t + k) / a.group;
+                p_c[n][k] = row < sp.n ? sp.base + row : -1;
+                cs[n][k] = KIND == KIND_F16 ? sm.qscale[n * 8 + 2 * t + k] : 1.0f;
+            }
+        {
+            const int row0 = cb * COLS / a.group, row1 = min((cb * COLS + COLS - 1) / a.group, sp.n - 1);
+            p_min = sp.base + row0;
+            p_max = sp.base + row1;
+        }
+        float m[NT][2], l[NT][2], o[NT][VB * 4][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VB * 4; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+        }
+
+        // ---- the warp's tiles: unit i, tile 4 i + warp of the item's list
+        const int* tab = a.table + (size_t)s * a.max_pages;
+        const size_t head_elems = (size_t)a.page * hd;
+        auto tile_key = [&](int i) {                               // first key of the warp's tile of unit i
+            const int x = i * WARPS + warp;
+            return (x < sp.na ? x : x - sp.na + sp.b0) << 4;
+        };
+        auto page_of = [&](int i) {                                // its page
+            if (i * WARPS + warp >= sp.tiles) return 0;
+            const int pg = tab[tile_key(i) / a.page];
+            if (pg >= 0 && pg < a.n_pages) return pg;
+            if (lane == 0) fk_raise(a.err, 97);
+            return 0;
+        };
+        constexpr int KR = KIND == KIND_F32 ? 2 : 1;               // 16-byte pieces of 8 values
+        uint4 kr[KB][2][KR], vr[VB][4][KR];
+        auto request_k = [&](int i, int pg) {
+            const T* base = (const T*)a.data + (2 * (size_t)pg * a.n_kv + kvh) * head_elems + (size_t)(tile_key(i) & (a.page - 1)) * hd;
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                for (int r = 0; r < 2; r++)
+#pragma unroll
+                    for (int k = 0; k < KR; k++) {
+                        const int d = 32 * kb + 8 * t;
+                        kr[kb][r][k] = make_uint4(0, 0, 0, 0);
+                        if (HDP == 64 && hd == 64 || d < hd) kr[kb][r][k] = ld16(base + (size_t)(g + 8 * r) * hd + d + 4 * k);
+                    }
+        };
+        auto request_v = [&](int i, int pg) {
+            const T* base = (const T*)a.data + ((2 * (size_t)pg + 1) * a.n_kv + kvh) * head_elems + (size_t)(tile_key(i) & (a.page - 1)) * hd;
+#pragma unroll
+            for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int k = 0; k < KR; k++) {
+                        const int d = 64 * vb + 8 * g;
+                        vr[vb][r][k] = make_uint4(0, 0, 0, 0);
+                        if (d < hd) vr[vb][r][k] = ld16(base + (size_t)(2 * t + (r & 1) + 8 * (r >> 1)) * hd + d + 4 * k);
+                    }
+        };
+        int pg = i0 < i1 ? page_of(i0) : 0;
+        if (i0 < i1 && i0 * WARPS + warp < sp.tiles) request_k(i0, pg);
+        for (int i = i0; i < i1; i++) {
+            if (i * WARPS + warp >= sp.tiles) break;               // the last unit may be short of tiles
+            const int key0 = tile_key(i);
+            request_v(i, pg);
+            const int pg_next = i + 1 < i1 ? page_of(i + 1) : 0;
+            // scores
+            float sc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+                // two steps of 16 dims: registers 0, 1 and 2, 3 of both rows' pieces
+                uint32_t ka[KIND == KIND_F32 ? 3 : 1][2][4];
+                if (KIND == KIND_F32) {
+#pragma unroll
+                    for (int r = 0; r < 2; r++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const uint4 x = kr[kb][r][KR - 1 == 0 ? 0 : j >> 1];
+                            uint32_t p[3];
+                            split_pair<FK_BF16>(__uint_as_float(j & 1 ? x.z : x.x), __uint_as_float(j & 1 ? x.w : x.y), p);
+#pragma unroll
+                            for (int k = 0; k < 3; k++) ka[KIND == KIND_F32 ? k : 0][j >> 1][r + 2 * (j & 1)] = p[k];
+                        }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        ka[0][h][0] = h ? kr[kb][0][0].z : kr[kb][0][0].x;
+                        ka[0][h][1] = h ? kr[kb][1][0].z : kr[kb][1][0].x;
+                        ka[0][h][2] = h ? kr[kb][0][0].w : kr[kb][0][0].y;
+                        ka[0][h][3] = h ? kr[kb][1][0].w : kr[kb][1][0].y;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int k = QP - 1; k >= 0; k--) {            // the small parts first
+                        const uint4 qv = sm.q[n][kb][k][lane];
+#pragma unroll
+                        for (int kk = (KIND == KIND_F32 ? 2 - k : 0); kk >= 0; kk--) {
+                            mma<KIND>(x, ka[kk][0], qv.x, qv.y);
+                            mma<KIND>(x, ka[kk][1], qv.z, qv.w);
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++) sc[n][k] += x[k];
+                }
+            }
+            if (KIND != KIND_F32 && (i + 1) * WARPS + warp < sp.tiles && i + 1 < i1) request_k(i + 1, pg_next);
+            // masks: only where a tile reaches over an edge
+            const bool edge = key0 + 15 > p_min || (a.window > 0 && key0 <= p_max - a.window && key0 + 15 >= a.first);
+            if (edge) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int j = key0 + g + 8 * (k >> 1), p = p_c[n][k & 1];
+                        const bool vis = j <= p && (a.window <= 0 || j > p - a.window || j < a.first);
+                        sc[n][k] = vis ? sc[n][k] * cs[n][k & 1] : -INFINITY;
+                    }
+            } else if (KIND == KIND_F16) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) sc[n][k] *= cs[n][k & 1];
+            }
+            // a new maximum anywhere in the warp: find it and rescale (rare once a sequence is under way)
+            bool up = false;
+#pragma unroll
+            for (int n = 0; n < NT; n++) up = up || fmaxf(sc[n][0], sc[n][2]) > m[n][0] || fmaxf(sc[n][1], sc[n][3]) > m[n][1];
+            if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        float x = fmaxf(fmaxf(sc[n][k], sc[n][2 + k]), m[n][k]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        const float corr = m[n][k] == -INFINITY ? 0.0f : pow2(m[n][k] - x);
+                        m[n][k] = x;
+                        l[n][k] *= corr;
+#pragma unroll
+                        for (int d = 0; d < VB * 4; d++) {
+                            o[n][d][k] *= corr;
+                            o[n][d][2 + k] *= corr;
+                        }
+                    }
+            }
+            // weights, as parts in the layout of the second product's operand
+            uint32_t wp[NT][QP][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0] - SHIFT, m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1] - SHIFT;
+                const float w0 = pow2(sc[n][0] - m0), w1 = pow2(sc[n][1] - m1), w2 = pow2(sc[n][2] - m0), w3 = pow2(sc[n][3] - m1);
+                l[n][0] += w0 + w2;
+                l[n][1] += w1 + w3;
+                uint32_t a0[3], a1[3];
+                split_pair<KIND>(w0, w1, a0);
+                split_pair<KIND>(w2, w3, a1);
+#pragma unroll
+                for (int k = 0; k < QP; k++) {
+                    wp[n][k][0] = transposed(a0[k]);
+                    wp[n][k][1] = transposed(a1[k]);
+                }
+            }
+            // A value whose key no column of the item sees may be anything, NaN among it: it must not meet a weight of 0.
+            // Values that some columns see and others do not are finite in any sane model; where one is not, the columns'
+            // rows are taken one by one, each with the values it does not see as zeros.
+            int passes = 1;
+            if (edge) {
+                bool odd = false;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int j = key0 + 2 * t + (r & 1) + 8 * (r >> 1);
+                    const bool some = j <= p_max && (a.window <= 0 || j > p_min - a.window || j < a.first);
+                    const bool every = j <= p_min && (a.window <= 0 || j > p_max - a.window || j < a.first);
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                        for (int k = 0; k < KR; k++) {
+                            uint4& x = vr[vb][r][k];
+                            if (!some) x = make_uint4(0, 0, 0, 0);
+                            else if (!every) {
+                                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                for (int q = 0; q < 4; q++) {
+                                    if (KIND == KIND_F32) odd = odd || (w[q] & 0x7f800000u) == 0x7f800000u;
+                                    else if (KIND == KIND_F16) odd = odd || (w[q] & 0x7c00u) == 0x7c00u || (w[q] & 0x7c000000u) == 0x7c000000u;
+                                    else odd = odd || (w[q] & 0x7f80u) == 0x7f80u || (w[q] & 0x7f800000u) == 0x7f800000u;
+                                }
+                            }
+                        }
+                }
+                if (__any_sync(0xffffffffu, odd)) passes = p_max - p_min + 1;
+            }
+            for (int ps = 0; ps < passes; ps++) {
+                const int p_row = p_min + ps;
+#pragma unroll
+                for (int vb = 0; vb < VB; vb++) {
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {                  // dims 64 vb + 8 g + 2 d and + 1
+                        uint32_t va[KIND == KIND_F32 ? 3 : 1][4];
+                        if (KIND == KIND_F32) {
+                            float x[4][2];
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const uint4 y = vr[vb][r][KR - 1 == 0 ? 0 : d >> 1];
+                                x[r][0] = __uint_as_float(d & 1 ? y.z : y.x);
+                                x[r][1] = __uint_as_float(d & 1 ? y.w : y.y);
+                            }
+#pragma unroll
+                            for (int h = 0; h < 2; h++)
+#pragma unroll
+                                for (int k = 0; k < 2; k++) {
+                                    uint32_t p[3];
+                                    split_pair<FK_BF16>(x[2 * h][k], x[2 * h + 1][k], p);
+#pragma unroll
+                                    for (int q = 0; q < 3; q++) va[KIND == KIND_F32 ? q : 0][2 * h + k] = p[q];
+                                }
+                        } else {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int r = 0; r < 4; r++) w[r] = d == 0 ? vr[vb][r][0].x : d == 1 ? vr[vb][r][0].y : d == 2 ? vr[vb][r][0].z : vr[vb][r][0].w;
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                va[0][2 * h] = __byte_perm(w[2 * h], w[2 * h + 1], 0x5410);
+                                va[0][2 * h + 1] = __byte_perm(w[2 * h], w[2 * h + 1], 0x7632);
+                            }
+                        }
+                        if (passes > 1) {
+                            // tokens of this lane's operand that the row does not see
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const int j = key0 + 2 * t + (r & 1) + 8 * (r >> 1);
+                                if (j <= p_row && (a.window <= 0 || j > p_row - a.window || j < a.first)) continue;
+                                const uint32_t keep = r & 1 ? 0x0000ffffu : 0xffff0000u;
+#pragma unroll
+                                for (int q = 0; q < (KIND == KIND_F32 ? 3 : 1); q++) {
+                                    va[q][2 * (r >> 1)] &= keep;
+                                    va[q][2 * (r >> 1) + 1] &= keep;
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            // of the operand's column g only the row of this pass
+                            const bool mine = passes == 1 || sp.base + (cb * COLS + n * 8 + g) / a.group == p_row;
+                            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for (int k = QP - 1; k >= 0; k--) {
+                                const uint32_t b0 = mine ? wp[n][k][0] : 0u, b1 = mine ? wp[n][k][1] : 0u;
+#pragma unroll
+                                for (int kk = (KIND == KIND_F32 ? 2 - k : 0); kk >= 0; kk--) mma<KIND>(x, va[kk], b0, b1);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4; k++) o[n][vb * 4 + d][k] += x[k];
+                        }
+                    }
+                }
+            }
+            pg = pg_next;
+            if (KIND == KIND_F32 && (i + 1) * WARPS + warp < sp.tiles && i + 1 < i1) request_k(i + 1, pg);
+        }
+
+        // ---- join the warps
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                float x = l[n][k];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (g == 0) {
+                    sm.m[warp][n * 8 + 2 * t + k] = m[n][k];
+                    sm.l[warp][n * 8 + 2 * t + k] = x;
+                }
+#pragma unroll
+                for (int d = 0; d < VB * 4; d++) {
+                    float* dst = sm.o[warp][n * 8 + 2 * t + k] + 64 * (d >> 2) + 8 * g + 2 * (d & 3);
+                    *(float2*)dst = make_float2(o[n][d][k], o[n][d][2 + k]);
+                }
+            }
+        __syncthreads();
+        const bool direct = a.whole || (i0 == 0 && i1 == units);
+        // a CTA's record 1 is the item that begins in its run and goes on behind it, record 0 the one that began before
+        float* rec = a.rec + ((size_t)2 * blockIdx.x + (item0 >= u_begin ? 1 : 0)) * ATTN_RECORD;
+        for (int x = tid; x < COLS * (HDP / 4); x += WARPS * 32) {
+            const int c = x / (HDP / 4), d = 4 * (x % (HDP / 4));
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) M = fmaxf(M, sm.m[w][c]);
+            float L = 0.0f;
+            float4 O = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) {
+                const float f = sm.m[w][c] == -INFINITY ? (sm.l[w][c] != sm.l[w][c] ? sm.l[w][c] : 0.0f) : pow2(sm.m[w][c] - M);
+                const float4 v = *(const float4*)(sm.o[w][c] + d);
+                L += sm.l[w][c] * f;
+                O.x += v.x * f; O.y += v.y * f; O.z += v.z * f; O.w += v.w * f;
+            }
+            if (direct) {
+                const int cc = cb * COLS + c, row = cc / a.group, h = kvh * a.group + cc % a.group;
+                if (row < sp.n && d < hd) {
+                    if (a.sinks) {
+                        const float z = a.sinks[h] * LOG2E;
+                        // against a maximum far below the sink the sum overflows to infinity and the output is 0, as it should be
+                        L += M == -INFINITY ? 1.0f : pow2(z - M + SHIFT);
+                    }
+                    const float inv = 1.0f / L;
+                    *(float4*)(a.out + ((size_t)s * a.rows + row) * a.n_heads * hd + (size_t)h * hd + d) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+                }
+            } else {
+                *(float4*)(rec + c * 128 + d) = O;
+                if (d == 0) {
+                    rec[16 * 128 + c] = M;
+                    rec[16 * 129 + c] = L;
+                }
+            }
+        }
+        if (direct) continue;
+
+        // ---- the last CTA of the item joins the records of CTAs [c0, c1]
+        const int c0 = item0 / chunk, c1 = (item0 + units - 1) / chunk;
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) sm.last = atomicAdd(&a.cnt[c0], 1u) == (unsigned)(c1 - c0);
+        __syncthreads();
+        if (!sm.last) continue;
+        __threadfence();
+        for (int x = tid; x < COLS * (HDP / 4); x += WARPS * 32) {
+            const int c = x / (HDP / 4), d = 4 * (x % (HDP / 4));
+            const int cc = cb * COLS + c, row = cc / a.group, h = kvh * a.group + cc % a.group;
+            if (row >= sp.n || d >= hd) continue;
+            float M = -INFINITY;
+            for (int k = c0; k <= c1; k++) {
+                const float* r = a.rec + ((size_t)2 * k + (k == c0 && item0 >= k * chunk ? 1 : 0)) * ATTN_RECORD;
+                M = fmaxf(M, __ldcg(r + 16 * 128 + c));
+            }
+            float L = 0.0f;
+            float4 O = make_float4(0, 0, 0, 0);
+            for (int k = c0; k <= c1; k++) {
+                const float* r = a.rec + ((size_t)2 * k + (k == c0 && item0 >= k * chunk ? 1 : 0)) * ATTN_RECORD;
+                const float mk = __ldcg(r + 16 * 128 + c), lk = __ldcg(r + 16 * 129 + c);
+                const float4 v = __ldcg((const float4*)(r + c * 128 + d));
+                const float f = mk == -INFINITY ? (lk != lk ? lk : 0.0f) : pow2(mk - M);
+                L += lk * f;
+                O.x += v.x * f; O.y += v.y * f; O.z += v.z * f; O.w += v.w * f;
+            }
+            if (a.sinks) L += M == -INFINITY ? 1.0f : pow2(a.sinks[h] * LOG2E - M + SHIFT);
+            const float inv = 1.0f / L;
+            *(float4*)(a.out + ((size_t)s * a.rows + row) * a.n_heads * hd + (size_t)h * hd + d) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+        }
+        if (tid == 0) a.cnt[c0] = 0;
+    }
+}
+
+template <int KIND, int HDP, int NT> int launch_attn(fk_ctx* ctx, cudaStream_t st, AttnArgs a) {
+    auto kern = attn_paged_kernel<KIND, HDP, NT>;
+    const size_t smem = sizeof(Smem<KIND, HDP, NT>);
+    static thread_local int resident[64] = {};                     // CTAs an SM holds, by device
+    int& per_sm = resident[ctx->device & 63];
+    if (per_sm == 0) {
+        FK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), FK_KERNEL);
+        FK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared), FK_KERNEL);
+        int n = 0;
+        FK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, WARPS * 32, smem), FK_KERNEL);
+        per_sm = n < 1 ? 1 : n > ATTN_CTAS_PER_SM ? ATTN_CTAS_PER_SM : n;
+    }
+    a.n_cb = (int)(((long long)a.rows * a.group + 8 * NT - 1) / (8 * NT));
+    const long long entries = (long long)a.n_cb * a.n_seqs;
+    if (entries * a.n_kv > 0x7fffffffLL) return fk_fail(FK_UNSUPPORTED, "attention_paged: %d rows of %d sequences", a.rows, a.n_seqs);
+    a.whole = entries > MAX_ENTRIES;
+    const unsigned grid = a.whole ? (unsigned)(entries * a.n_kv) : (unsigned)(per_sm * ctx->sm_count);
+    FK_CUDA(launch(kern, dim3(grid), dim3(WARPS * 32), smem, st, a), FK_LAUNCH);
+    return FK_OK;
+}
+
+template <int KIND> int launch_kind(fk_ctx* ctx, cudaStream_t st, const AttnArgs& a) {
+    const bool wide = (long long)a.rows * a.group > 8;
+    if (a.head_dim <= 64) return wide ? launch_attn<KIND, 64, 2>(ctx, st, a) : launch_attn<KIND, 64, 1>(ctx, st, a);
+    return wide ? launch_attn<KIND, 128, 2>(ctx, st, a) : launch_attn<KIND, 128, 1>(ctx, st, a);
+}
+
+}  // namespace
+
+FK_EXPORT int fk_attention_paged(fk_ctx* ctx, void* stream, const fk_pages* p, int layer, const float* q_dev, int q_ld, int rows, const int* n_new_dev,
+                                 int n_heads, float scale, int window, int first, const float* sinks_dev, float* out_dev) {
+    int rc = check("attention_paged", ctx, p, layer);
+    if (rc != FK_OK) return rc;
+    if (!q_dev || !out_dev) return fk_fail(FK_INVALID, "attention_paged: null argument");
+    if (window < 0 || first < 0) return fk_fail(FK_INVALID, "attention_paged: window %d, first %d", window, first);
+    if (rows < 1 || n_heads < 1 || n_heads % p->n_kv || (long long)rows * p->n_seqs > 0x7fffffffLL || (long long)n_heads * p->head_dim > 0x7fffffffLL)
+        return fk_fail(FK_UNSUPPORTED, "attention_paged: %d rows, %d/%d heads of %d", rows, n_heads, p->n_kv, p->head_dim);
+    if (q_ld == 0) q_ld = n_heads * p->head_dim;
+    if (q_ld < n_heads * p->head_dim || (q_ld & 3) || (((uintptr_t)q_dev | (uintptr_t)out_dev) & 15))
+        return fk_fail(FK_INVALID, "attention_paged: rows must be 16-byte aligned, %d floats apart", q_ld);
+    FkDeviceGuard g(ctx->device);
+    AttnArgs a{(const char*)p->data_dev + (size_t)layer * page_bytes(p) * p->n_pages, p->table_dev, p->lens_dev, n_new_dev, q_dev, sinks_dev, out_dev,
+               (unsigned*)p->ws_dev, (float*)((char*)p->ws_dev + WS_COUNTERS), ctx->err_flag, scale, q_ld, rows, p->n_seqs, n_heads, p->n_kv,
+               n_heads / p->n_kv, p->head_dim, p->page, p->n_pages, p->max_pages, window, first, 0, 0};
+    cudaStream_t st = (cudaStream_t)stream;
+    rc = p->kind == KIND_F32 ? launch_kind<KIND_F32>(ctx, st, a) : p->kind == KIND_F16 ? launch_kind<KIND_F16>(ctx, st, a) : launch_kind<FK_BF16>(ctx, st, a);
+    if (rc != FK_OK) return rc;
+    FK_CUDA(cudaGetLastError(), FK_LAUNCH);
+    ctx->launches++;
+    return FK_OK;
+}

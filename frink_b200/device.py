@@ -28,8 +28,8 @@ def context(device=None):
         return _contexts[idx]
 
 
-def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+def _stream(device=None):
+    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
 def _ptr(t):
@@ -547,3 +547,208 @@ def argmax(x, out=None):
 
 def add_int_(p, v):
     check(lib().fk_add_int(context(p.device), _stream(), _ptr(_i32(p)), int(v)))
+
+
+# ---- paged KV cache -----------------------------------------------------------
+_PAGE_KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+
+
+class _CPages(C.Structure):
+    """`fk_pages` of the C ABI."""
+    _fields_ = [("data_dev", C.c_void_p), ("table_dev", C.c_void_p), ("lens_dev", C.c_void_p), ("refs_dev", C.c_void_p), ("ws_dev", C.c_void_p),
+                ("ws_bytes", C.c_size_t), ("kind", C.c_int), ("n_layers", C.c_int), ("n_pages", C.c_int), ("page", C.c_int), ("n_kv", C.c_int),
+                ("head_dim", C.c_int), ("n_seqs", C.c_int), ("max_pages", C.c_int)]
+
+
+class Pages:
+    """A KV cache of pages shared by many sequences: data [n_layers, n_pages, 2, n_kv, page, head_dim] (float32, float16 or
+    bfloat16; page 16, 32, 64 or 128), table [n_seqs, max_pages] int32 (-1: no page), lens [n_seqs] int32, refs [n_pages]
+    int32.  The tensors stay the caller's; the workspace is this object's, and calls on it belong on one stream at a time."""
+
+    def __init__(self, data, table, lens, refs, _ws=None):
+        if data.dim() != 6 or data.shape[2] != 2 or data.dtype not in _PAGE_KINDS:
+            raise _lib.Invalid("pages: data is [n_layers, n_pages, 2, n_kv, page, head_dim] of float32, float16 or bfloat16")
+        for t in (data, table, lens, refs):
+            if not (t.is_cuda and t.device == data.device and t.is_contiguous()):
+                raise _lib.Invalid("pages: data, table, lens and refs are contiguous CUDA tensors of one device")
+        for t in (table, lens, refs):
+            if t.dtype != torch.int32:
+                raise _lib.Invalid("pages: table, lens and refs are int32")
+        n_layers, n_pages, _, n_kv, page, hd = data.shape
+        if table.dim() != 2 or lens.shape != (table.shape[0],) or refs.shape != (n_pages,):
+            raise _lib.Invalid("pages: table [n_seqs, max_pages], lens [n_seqs], refs [n_pages]")
+        self.data, self.table, self.lens, self.refs = data, table, lens, refs
+        self.n_layers, self.n_pages, self.page, self.n_kv, self.head_dim = n_layers, n_pages, page, n_kv, hd
+        self.n_seqs, self.max_pages = table.shape
+        self._ctx = context(data.device)
+        if _ws is None:
+            need = lib().fk_pages_workspace(self._ctx, n_pages)
+            _ws = torch.empty(need + 256, dtype=torch.uint8, device=data.device)
+            _ws[:8192 + 256].zero_()                      # the arrival counters; what lies behind them is scratch
+            torch.cuda.current_stream(data.device).synchronize()    # whatever stream the first call comes on
+        self._ws = _ws
+        base = (_ws.data_ptr() + 255) & ~255
+        self._c = _CPages(data.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), base, _ws.numel() - (base - _ws.data_ptr()),
+                          _PAGE_KINDS[data.dtype], n_layers, n_pages, page, n_kv, hd, self.n_seqs, self.max_pages)
+        self._p = C.byref(self._c)
+
+    @classmethod
+    def alloc(cls, n_layers, n_pages, page, n_kv, head_dim, n_seqs, max_pages, dtype=torch.bfloat16, device="cuda"):
+        """An empty cache."""
+        i32 = dict(dtype=torch.int32, device=device)
+        return cls(torch.zeros((n_layers, n_pages, 2, n_kv, page, head_dim), dtype=dtype, device=device), torch.full((n_seqs, max_pages), -1, **i32),
+                   torch.zeros(n_seqs, **i32), torch.zeros(n_pages, **i32))
+
+    def seq(self, s):
+        """Sequence s alone, on the same pages (a prompt's rows)."""
+        if not 0 <= s < self.n_seqs:
+            raise _lib.Invalid(f"pages: sequence {s} of {self.n_seqs}")
+        return Pages(self.data, self.table[s:s + 1], self.lens[s:s + 1], self.refs, _ws=self._ws)
+
+
+def _n_new(pg, n_new):
+    """(device pointer or None, count) of the rows every sequence gets."""
+    if isinstance(n_new, torch.Tensor):
+        if not (n_new.dtype == torch.int32 and n_new.device == pg.data.device and n_new.shape == (pg.n_seqs,) and n_new.is_contiguous()):
+            raise _lib.Invalid(f"pages: n_new is an int32 tensor of {pg.n_seqs} counts on the pages' device")
+        return n_new.data_ptr(), 0
+    return None, int(n_new)
+
+
+def _list(ids):
+    return (C.c_int * len(ids))(*ids)
+
+
+def pages_grow(pg, n_new):
+    """Every sequence gets the pages for n_new (an int, or int32 [n_seqs] on the device) tokens more than it holds."""
+    check(lib().fk_pages_grow(pg._ctx, _stream(pg.data.device), pg._p, *_n_new(pg, n_new)))
+
+
+def pages_advance(pg, n_new):
+    """lens += n_new: the step's tokens are in."""
+    check(lib().fk_pages_advance(pg._ctx, _stream(pg.data.device), pg._p, *_n_new(pg, n_new)))
+
+
+def pages_fork(pg, src, dst, n=None):
+    """Sequence dst[i] (empty) becomes the first n[i] tokens of src[i] (None, or a negative count: all): whole pages are
+    shared, the last part of one is copied in every layer.  Lists of at most 64."""
+    src, dst = list(src), list(dst)
+    if len(src) != len(dst) or (n is not None and len(n) != len(src)):
+        raise _lib.Invalid("pages_fork: lists of one length")
+    check(lib().fk_pages_fork(pg._ctx, _stream(pg.data.device), pg._p, _list(src), _list(dst), _list(list(n)) if n is not None else None, len(src)))
+
+
+def pages_free(pg, seqs):
+    """The listed sequences give their pages back and hold nothing (at most 64 a call)."""
+    seqs = list(seqs)
+    check(lib().fk_pages_free(pg._ctx, _stream(pg.data.device), pg._p, _list(seqs), len(seqs)))
+
+
+def pages_compact(pg):
+    """Moves the pages in use to the front of the pool -> their number (int32 [1] on the device)."""
+    used = torch.empty(1, dtype=torch.int32, device=pg.data.device)
+    check(lib().fk_pages_compact(pg._ctx, _stream(pg.data.device), pg._p, used.data_ptr()))
+    return used
+
+
+def _rows_of(pg, q, width, what):
+    """q [n_seqs * rows, width], any row stride -> (rows, row stride)."""
+    if not (q.is_cuda and q.device == pg.data.device and q.dtype == torch.float32 and q.dim() == 2 and q.shape[1] == width and q.stride(1) == 1):
+        raise _lib.Invalid(f"{what}: float32 rows of {width} on the pages' device")
+    n = q.shape[0]
+    if n == 0 or n % pg.n_seqs:
+        raise _lib.Invalid(f"{what}: {n} rows for {pg.n_seqs} sequences")
+    return n // pg.n_seqs, q.stride(0) if n > 1 else max(q.stride(0), width)
+
+
+def _vec(pg, t, n, what):
+    """An optional contiguous float32 vector of n values on the pages' device -> its address."""
+    if t is None:
+        return None
+    if not (t.dtype == torch.float32 and t.device == pg.data.device and t.numel() == n and t.is_contiguous()):
+        raise _lib.Invalid(f"{what}: {n} contiguous float32 values on the pages' device")
+    return t.data_ptr()
+
+
+def rope_kv_paged(q, k, v, pg, layer, n_heads, theta, neox=False, n_new=None, q_norm=None, k_norm=None, eps=0.0, out=None):
+    """(Qwen3: per-head RMSNorm of q and k,) rotation of q and k and the append of k and v into the pages of `layer`: q, k, v
+    are [n_seqs * rows, heads * head_dim] (column slices are fine), row i of sequence s goes to position lens[s] + i; rows from
+    n_new[s] on are skipped.  -> the rotated q (`out` may be q itself where its rows are packed); k stays as it is."""
+    hd = pg.head_dim
+    rows, q_ld = _rows_of(pg, q, n_heads * hd, "rope_kv_paged: q")
+    for t in (k, v):
+        if _rows_of(pg, t, pg.n_kv * hd, "rope_kv_paged: k, v")[0] != rows:
+            raise _lib.Invalid("rope_kv_paged: q, k and v have the same number of rows")
+    one = q.shape[0] == 1
+    if out is None:
+        out = torch.empty((q.shape[0], n_heads * hd), dtype=torch.float32, device=q.device)
+    elif not (out.shape == q.shape and out.dtype == torch.float32 and out.device == q.device and out.is_contiguous()):
+        raise _lib.Invalid("rope_kv_paged: out is a contiguous float32 tensor of q's shape")
+    check(lib().fk_rope_kv_paged(pg._ctx, _stream(q.device), pg._p, int(layer), q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ld,
+                                 k.stride(0) if not one else pg.n_kv * hd, v.stride(0) if not one else pg.n_kv * hd, rows,
+                                 _n_new(pg, n_new)[0] if n_new is not None else None, n_heads, float(theta), int(neox),
+                                 _vec(pg, q_norm, hd, "rope_kv_paged: q_norm"), _vec(pg, k_norm, hd, "rope_kv_paged: k_norm"), float(eps), out.data_ptr()))
+    return out
+
+
+def attention_paged(q, pg, layer, n_heads, n_new=None, scale=None, window=0, first=0, sinks=None, out=None):
+    """Attention over the pages of `layer`: q [n_seqs * rows, n_heads * head_dim] (rotated; any row stride that is a multiple
+    of 4), row i of sequence s at position lens[s] + i, its own key and value appended already.  window > 0: the `window` most
+    recent keys and the `first` earliest; sinks [n_heads]: a logit per head in the softmax's denominator.  Rows from n_new[s]
+    (int32 [n_seqs]) on are left as they were in `out`."""
+    rows, ld = _rows_of(pg, q, n_heads * pg.head_dim, "attention_paged: q")
+    if out is None:
+        out = torch.empty((q.shape[0], q.shape[1]), dtype=torch.float32, device=q.device)
+    elif not (out.shape == q.shape and out.dtype == torch.float32 and out.device == q.device and out.is_contiguous()):
+        raise _lib.Invalid("attention_paged: out is a contiguous float32 tensor of q's shape")
+    check(lib().fk_attention_paged(pg._ctx, _stream(q.device), pg._p, int(layer), q.data_ptr(), ld, rows,
+                                   _n_new(pg, n_new)[0] if n_new is not None else None, n_heads,
+                                   float(scale) if scale is not None else pg.head_dim ** -0.5, int(window), int(first),
+                                   _vec(pg, sinks, n_heads, "attention_paged: sinks"), out.data_ptr()))
+    return out
+
+
+# ---- rules on logits ------------------------------------------------------------
+def logit_rules(logits, history=None, penalties=None, bias=None, mask=None, out=None, tokens=None):
+    """What a sampler does to logits [n, vocab] (or one row) before it picks, and the greedy pick -> (changed logits, tokens
+    int32 [n]).  history [n, h] int32: the tokens that came before (entries outside the vocabulary are empty places); a token
+    that occurs c > 0 times has its logit divided (if positive, else multiplied) by repeat, less c * frequency, less presence
+    (penalties: float32 [n, 3], or one triple for all rows).  bias [vocab] or [n, vocab] is added, then logits whose bit in mask
+    (int32 words [words] or [n, words], bit v % 32 of word v / 32) is clear become -inf.  tokens: the largest, ties to the lower
+    index; -1 where nothing is left."""
+    x = logits if logits.dim() == 2 else logits[None]
+    if not (x.is_cuda and x.dtype == torch.float32 and x.dim() == 2 and x.stride(1) == 1 and x.shape[0] > 0 and x.shape[1] > 0):
+        raise _lib.Invalid("logit_rules: float32 CUDA logits [n, vocab]")
+    n, V = x.shape
+
+    def rows(t, dtype, width, what):
+        # (tensor, floats or words between rows; 0: one row for all)
+        if t.dtype != dtype or t.device != x.device or t.dim() not in (1, 2) or t.stride(-1) != 1 or t.shape[-1] < width or (t.dim() == 2 and t.shape[0] != n):
+            raise _lib.Invalid(f"logit_rules: {what}")
+        return t.data_ptr(), 0 if t.dim() == 1 else t.stride(0) if n > 1 else max(t.stride(0), width)
+
+    h, hp, pen = 0, None, None
+    if history is not None:
+        hist = history if history.dim() == 2 else history[None]
+        if hist.dtype != torch.int32 or hist.device != x.device or hist.dim() != 2 or hist.shape[0] != n or not hist.is_contiguous():
+            raise _lib.Invalid("logit_rules: history is a contiguous int32 tensor [n, h] beside the logits")
+        if penalties is None:
+            raise _lib.Invalid("logit_rules: a history needs penalties (repeat, frequency, presence)")
+        if not isinstance(penalties, torch.Tensor):
+            penalties = torch.tensor([[float(v) for v in penalties]], dtype=torch.float32).to(x.device).expand(n, -1)
+        pen = penalties.contiguous()
+        if pen.dtype != torch.float32 or pen.device != x.device or pen.shape != (n, 3):
+            raise _lib.Invalid("logit_rules: penalties are float32 [n, 3]: repeat, frequency, presence")
+        h, hp = hist.shape[1], hist.data_ptr() if hist.shape[1] else None
+    bp, b_ld = rows(bias, torch.float32, V, "bias is float32 [vocab] or [n, vocab]") if bias is not None else (None, 0)
+    mp, m_ld = rows(mask, torch.int32, (V + 31) // 32, "mask is int32 words [ceil(vocab / 32)] or [n, ...]") if mask is not None else (None, 0)
+    o = torch.empty((n, V), dtype=torch.float32, device=x.device) if out is None else out if out.dim() == 2 else out[None]
+    if not (o.shape == (n, V) and o.dtype == torch.float32 and o.device == x.device and o.is_contiguous()):
+        raise _lib.Invalid("logit_rules: out is a contiguous float32 tensor of the logits' shape")
+    if tokens is None:
+        tokens = torch.empty(n, dtype=torch.int32, device=x.device)
+    elif not (tokens.shape == (n,) and tokens.dtype == torch.int32 and tokens.device == x.device and tokens.is_contiguous()):
+        raise _lib.Invalid("logit_rules: tokens is a contiguous int32 tensor [n]")
+    check(lib().fk_logit_rules(context(x.device), _stream(x.device), x.data_ptr(), x.stride(0) if n > 1 else max(x.stride(0), V), n, V, hp, h,
+                               pen.data_ptr() if pen is not None else None, bp, b_ld, mp, m_ld, o.data_ptr(), tokens.data_ptr()))
+    return (o if logits.dim() == 2 else o[0]), tokens

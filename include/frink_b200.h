@@ -376,6 +376,78 @@ int fk_argmax(fk_ctx* ctx, void* stream, const float* x_dev, int n_rows, int n, 
 /* *p += v on the device (the position word of a captured decode step). */
 int fk_add_int(fk_ctx* ctx, void* stream, int* p_dev, int v);
 
+/* ---- paged KV cache -----------------------------------------------------------
+ * The cache of many sequences cut into pages that all layers number alike (frink-core keeps paged caches of its own,
+ * crates/frink-core/src/cache*.rs; its CUDA backend has none).  All device memory belongs to the caller:
+ *   data   [n_layers][n_pages][2: K, V][n_kv][page][head_dim] of `kind`: 0 f32, 1 f16, 30 bf16 (the ggml type tags)
+ *   table  [n_seqs][max_pages]: the pages of every sequence in order, -1 behind the last one
+ *   lens   [n_seqs]: tokens every sequence holds
+ *   refs   [n_pages]: sequences that hold the page (0 = free)
+ *   ws     fk_pages_workspace(...) bytes, zeroed once by the caller, 256-byte aligned: ONE call that uses it in flight
+ *          (calls on one stream are); caches with workspaces of their own are independent
+ * page is 16, 32, 64 or 128 tokens; head_dim a multiple of 8, at most 128; n_seqs at most 4096.
+ * Which pages a call takes is fixed: the lowest free ones, in the order of the sequences (forks: of the list).
+ * Tables, lengths and counts live on the device, so a captured step may grow its sequences as it is replayed.  What a
+ * kernel finds wrong there it raises in the device error word: 95 a sequence would outgrow its table row, 96 fewer free
+ * pages than needed, 97 a page number outside the pool, 98 a fork of more tokens than its source holds or into a sequence
+ * that holds something.  grow and fork that raise change nothing; a row of attention or append whose sequence is wrong
+ * (95) is left as it was; a wrong page number (97) is read as page 0 and never written. */
+typedef struct fk_pages {
+    void* data_dev;
+    int* table_dev;
+    int* lens_dev;
+    int* refs_dev;
+    void* ws_dev;
+    size_t ws_bytes;
+    int kind;
+    int n_layers;
+    int n_pages;
+    int page;
+    int n_kv;
+    int head_dim;
+    int n_seqs;
+    int max_pages;
+} fk_pages;
+size_t fk_pages_workspace(fk_ctx* ctx, int n_pages);
+/* Gives every sequence s the pages for n_new_dev[s] (null: n_new) tokens more than it holds. */
+int fk_pages_grow(fk_ctx* ctx, void* stream, const fk_pages* pages, const int* n_new_dev, int n_new);
+/* lens[s] += n_new_dev[s] (null: n_new): the step's tokens are in. */
+int fk_pages_advance(fk_ctx* ctx, void* stream, const fk_pages* pages, const int* n_new_dev, int n_new);
+/* Sequence dst[i] becomes the first n[i] tokens of src[i] (n null or n[i] < 0: all of them): whole pages are shared, the
+ * last part of one is copied in every layer.  Host lists of m <= 64; a dst occurs once, is no src and holds nothing. */
+int fk_pages_fork(fk_ctx* ctx, void* stream, const fk_pages* pages, const int* src_host, const int* dst_host, const int* n_host, int m);
+/* The listed sequences (each once, m <= 64) give their pages back and hold nothing. */
+int fk_pages_free(fk_ctx* ctx, void* stream, const fk_pages* pages, const int* seqs_host, int m);
+/* Moves the pages in use to the front: the k-th used page at or behind position U = pages in use goes to the k-th free page
+ * before it, in every layer; tables and counts follow.  *used_dev = U. */
+int fk_pages_compact(fk_ctx* ctx, void* stream, const fk_pages* pages, int* used_dev);
+/* fk_rope_kv into pages: `rows` rows a sequence (q, k, v rows s * rows + i; q_ld, k_ld, v_ld floats apart), row i of
+ * sequence s at position lens[s] + i, rows i >= n_new_dev[s] (null: none) skipped.  The rotated q goes to q_out_dev
+ * [n_seqs * rows][n_heads * head_dim] (may be q itself, packed); k and v are left alone.  Angles are taken in 64 bits and the
+ * factors rounded to 32, so far positions keep their precision.  lens does not move: the call may be repeated. */
+int fk_rope_kv_paged(fk_ctx* ctx, void* stream, const fk_pages* pages, int layer, const float* q_dev, const float* k_dev, const float* v_dev,
+                     int q_ld, int k_ld, int v_ld, int rows, const int* n_new_dev, int n_heads, float theta, int neox, const float* q_norm_dev,
+                     const float* k_norm_dev, float norm_eps, float* q_out_dev);
+/* Attention over the pages, one new row a sequence or many: row i of sequence s sits at position p = lens[s] + i (its own key
+ * and value are in the pages already) and sees the keys j <= p with window == 0, j > p - window, or j < first: with a window
+ * the `first` earliest tokens stay visible.  sinks_dev, q_ld (0 = packed) as in fk_attention.  Rows i >= n_new_dev[s] are left
+ * as they were.  f32 precision for every kind: the cache's values meet q and the weights split into parts whose products are
+ * exact. */
+int fk_attention_paged(fk_ctx* ctx, void* stream, const fk_pages* pages, int layer, const float* q_dev, int q_ld, int rows, const int* n_new_dev,
+                       int n_heads, float scale, int window, int first, const float* sinks_dev, float* out_dev);
+
+/* ---- rules on logits ----------------------------------------------------------
+ * What a sampler does to the logits before it picks (frink-models applies it on the host), and the greedy pick, in one pass:
+ * for a token that occurs c > 0 times in its row of history_dev [n_rows][history] (entries outside [0, vocab) are empty places)
+ *   x = x > 0 ? x / repeat : x * repeat, then x -= c * frequency, then x -= presence      (penalties_dev [n_rows][3])
+ * then x += bias_dev[v] (bias_ld floats between rows, 0 = one row for all), then -inf where bit v % 32 of word v / 32 of
+ * mask_dev (mask_ld words between rows, 0 = one row for all) is clear.  out_dev [n_rows][vocab] (may be the logits, packed);
+ * tokens_dev [n_rows] (may be null): the largest, ties to the lower index, NaN never; -1 where every token is -inf.
+ * history, bias and mask may be null; ld = floats between rows of logits_dev.  One call of this or of fk_argmax in flight per context. */
+int fk_logit_rules(fk_ctx* ctx, void* stream, const float* logits_dev, size_t ld, int n_rows, int vocab, const int* history_dev, int history,
+                   const float* penalties_dev, const float* bias_dev, size_t bias_ld, const int* mask_dev, size_t mask_ld, float* out_dev,
+                   int* tokens_dev);
+
 /* ---- multi-GPU: peer-memory all-reduce ---------------------------------------
  * The reference is single-device (crates/frink-cuda/src/gpu.rs:219); these have no counterpart
  * there.  One process per GPU of one box.  Every rank creates an arena and publishes its 64-byte
