@@ -9,9 +9,13 @@
 // Matrix products.  A warp takes 16 tokens of one KV head and 8 or 16 columns; a column is one (row, query head) pair of the
 // group, so that all query heads of a KV head share one read of its keys.  Scores are K (16 tokens x 16 dims) times q
 // (16 dims x 8 columns), outputs are V^T (16 dims x 16 tokens) times w (16 tokens x 8 columns), both mma.m16n8k16 with f32
-// sums.  K and V go from global memory straight into operand registers, 16 bytes a lane: which dims a lane's piece holds is
-// free as long as both operands agree, so the order of dims is permuted instead of the data.  The scores' fragment becomes the
-// weights' operand by a transposition of 8 x 8 blocks inside the warp (movmatrix).
+// sums.  Which dims a lane's 16 bytes hold is free as long as both operands agree, so the order of dims is permuted instead
+// of the data.  The scores' fragment becomes the weights' operand by a transposition of 8 x 8 blocks inside the warp (movmatrix).
+//
+// Memory.  16 tokens of one head are one contiguous piece of a page.  Every warp keeps a ring of its own in shared memory and
+// fills it with asynchronous copies one tile ahead, keys and values apart, so that no warp waits for another and a tile's
+// latency is covered by the tile before it and by the SM's other warps.  The copies place 16-byte pieces so that the operand
+// reads hit every bank once.
 //
 // Precision.  The cache's 16-bit values are exact operands.  q and w are f32 and are split into parts of the cache's type:
 // three bf16 parts hold all 24 bits; two f16 parts hold 22, their range kept by a power of two per column of q and by a
@@ -32,7 +36,7 @@ using namespace fk_paged;
 namespace {
 
 constexpr int WARPS = 4;
-constexpr int MAX_ENTRIES = 2048;          // (sequence, block of columns) pairs that are dealt out in runs
+constexpr int MAX_ENTRIES = 512;           // (sequence, block of columns) pairs that are dealt out in runs
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct AttnArgs {
@@ -44,7 +48,7 @@ struct AttnArgs {
     float* rec;
     int* err;
     float scale;
-    int q_ld, rows, n_seqs, n_heads, n_kv, group, head_dim, page, n_pages, max_pages, window, first, n_cb, whole;
+    int q_ld, rows, n_seqs, n_heads, n_kv, group, head_dim, page, log_page, n_pages, max_pages, window, first, n_cb, whole;
 };
 
 // ---- operand types
@@ -87,6 +91,19 @@ template <int KIND> __device__ __forceinline__ void mma(float* d, const uint32_t
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// d = a b: the same from zero (the sums start in the zero register)
+template <int KIND> __device__ __forceinline__ void mma0(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if (KIND == KIND_F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// four 8 x 8 blocks, transposed: operand registers of 16 dims x 16 tokens from tokens' rows
+__device__ __forceinline__ void ldsm_t(uint32_t* r, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -97,9 +114,14 @@ __device__ __forceinline__ float pow2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-__device__ __forceinline__ uint4 ld16(const void* p) {
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
     uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
 }
 
@@ -131,26 +153,46 @@ template <int COLS> __device__ __forceinline__ Span span_of(const AttnArgs& a, i
     return r;
 }
 
+// A step of a warp is SUB tiles of 16 tokens (each in a page of its own, perhaps).  16-byte piece c of a tile's token r lies at
+// c ^ swizzle(r): a read of K takes 4 pieces of 2 tokens at a time (f32: 4 even pieces of 2 tokens), one of V the same piece of
+// 8 tokens (f32: 2 even pieces of 4 tokens), and with these the 8 addresses fall into 8 different groups of banks.
+// A warp's ring is 16 KB whatever the type, so that an SM holds three CTAs: bytes in flight cover HBM's latency several times.
+template <int KIND, int HDP> struct Ring {
+    static constexpr int E = KIND == KIND_F32 ? 4 : 2;
+    static constexpr int SUB = KIND == KIND_F32 ? 1 : 2;
+    static constexpr int TILE = 16 * HDP * E;                              // bytes of 16 tokens' keys (or values)
+    static constexpr int STAGES = 16384 / (2 * SUB * TILE);
+    __host__ __device__ static constexpr int swz_k(int r) { return KIND == KIND_F32 ? r & 1 : (r & 1) << 2; }
+    __host__ __device__ static constexpr int swz_v(int r) { return KIND == KIND_F32 ? ((r >> 1) & 1) | (r & 4) : r & 7; }
+};
+
 template <int KIND, int HDP, int NT> struct Smem {
+    static constexpr int PITCH = HDP + 4;              // floats between columns of a warp's sums: stores hit every bank once
+    static_assert(16384 >= NT * 8 * PITCH * 4, "a warp's sums take its ring's place at the end of an item");
+    unsigned char ring[WARPS][16384];
     uint4 q[NT][HDP / 32][Kind<KIND>::Q][32];          // q's operand registers, part by part
     float qscale[NT * 8];                              // 2^-e of a column whose q was scaled by 2^e (f16)
-    float o[WARPS][NT * 8][HDP];
     float m[WARPS][NT * 8], l[WARPS][NT * 8];
     int start[MAX_ENTRIES + 1];                        // first unit of every (sequence, block of columns)
     int part[33];
     int last;
 };
 
-template <int KIND, int HDP, int NT>
-__global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a) {
+// EXACT: heads of HDP, else shorter ones (their missing pieces are zeros)
+template <int KIND, int HDP, bool EXACT, int NT>
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel(const AttnArgs a) {
     pdl_sync();
     constexpr int COLS = 8 * NT, KB = HDP / 32, VB = HDP / 64, QP = Kind<KIND>::Q;
+    using R = Ring<KIND, HDP>;
+    constexpr int E = R::E, SUB = R::SUB, STAGES = R::STAGES, ROWB = HDP * E, TILE = R::TILE, PITCH = Smem<KIND, HDP, NT>::PITCH;
+    constexpr int STEP = WARPS * SUB;                              // tiles of a unit
     constexpr float SHIFT = KIND == KIND_F16 ? 14.0f : 0.0f;       // weights are 2^SHIFT times exp(score - m)
-    using T = typename std::conditional<KIND == KIND_F32, float, uint16_t>::type;
-    extern __shared__ __align__(16) unsigned char smem_raw[];
+    extern __shared__ __align__(128) unsigned char smem_raw[];
     Smem<KIND, HDP, NT>& sm = *reinterpret_cast<Smem<KIND, HDP, NT>*>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int hd = a.head_dim, n_e = a.n_seqs * a.n_cb;
+    const int hd = EXACT ? HDP : a.head_dim, n_e = a.n_seqs * a.n_cb;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm.ring[warp]);
+    float* const sum_o = reinterpret_cast<float*>(sm.ring[warp]);          // [COLS][PITCH] at the end of an item
 
     // ---- this CTA's run of units [u, u_end); sm.start[e]: units before entry e (per KV head), times n_kv in the global order
     int u, u_end, chunk;
@@ -162,7 +204,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a
         int total = 0;
         for (int e0 = 0; e0 < n_e; e0 += WARPS * 32) {
             const int e = e0 + tid;
-            const int units = e < n_e ? (span_of<COLS>(a, e / a.n_cb, e % a.n_cb, blockIdx.x == 0).tiles + WARPS - 1) / WARPS : 0;
+            const int units = e < n_e ? (span_of<COLS>(a, e / a.n_cb, e % a.n_cb, blockIdx.x == 0).tiles + STEP - 1) / STEP : 0;
             int sum;
             const int at = block_prefix(units, sm.part, &sum);
             if (e < n_e) sm.start[e] = total + at;
@@ -198,7 +240,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a
         }
         const int s = e / a.n_cb, cb = e % a.n_cb;
         const Span sp = span_of<COLS>(a, s, cb, a.whole && tid == 0);
-        units = (sp.tiles + WARPS - 1) / WARPS;
+        units = (sp.tiles + STEP - 1) / STEP;
         if (a.whole) {
             if (units == 0) return;
             i0 = 0;
@@ -212,29 +254,97 @@ __global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a
             u = item0 + i1;
         }
 
-        // ---- q of the item's columns into operand registers' order, scaled, split into parts
+        // ---- the warp's steps: unit i0 + j, its tiles SUB (4 (i0 + j) + warp) and on of the item's list
+        const int* tab = a.table + (size_t)s * a.max_pages;
+        const uint32_t tok_bytes = hd * E;
+        const size_t head_bytes = (size_t)a.page * tok_bytes;
+        const char* const heads = (const char*)a.data + (size_t)kvh * head_bytes;
+        const size_t half_bytes = (size_t)a.n_kv * head_bytes;     // a page's keys (or values)
+        const int n_steps = max(0, min(i1, ((sp.tiles + SUB - 1) / SUB - warp + WARPS - 1) / WARPS) - i0);
+        constexpr int NO_KEY = 0x7fffff00;                         // a tile behind the last one: no column sees it
+        auto tile_key = [&](int j, int u) {                        // first key of a tile
+            const int x = ((i0 + j) * WARPS + warp) * SUB + u;
+            return x >= sp.tiles ? NO_KEY : (x < sp.na ? x : x - sp.na + sp.b0) << 4;
+        };
+        auto page_of = [&](int j, int u) {                         // its page
+            if (j >= n_steps) return 0;
+            const int k = tile_key(j, u);
+            if (k == NO_KEY) return 0;
+            const int pg = tab[k >> a.log_page];
+            if (pg >= 0 && pg < a.n_pages) return pg;
+            if (lane == 0) fk_raise(a.err, 97);
+            return 0;
+        };
+        auto request = [&](auto values, int j, const int* pg) {    // starts the copy of a step's keys or values
+            constexpr int V = decltype(values)::value;
+            if (j < n_steps) {
+#pragma unroll
+                for (int u = 0; u < SUB; u++) {
+                    const int k = tile_key(j, u);
+                    if (k == NO_KEY) continue;
+                    const char* src = heads + (size_t)(2 * (uint32_t)pg[u] + V) * half_bytes + (uint32_t)(k & (a.page - 1)) * tok_bytes;
+                    const uint32_t dst = ring + (((j % STAGES) * 2 + V) * SUB + u) * TILE;
+                    constexpr int CH = ROWB / 16;
+#pragma unroll
+                    for (int i = 0; i < TILE / 512; i++) {
+                        const int r = i * (32 / CH) + lane / CH, c = lane % CH;
+                        const uint32_t at = r * ROWB + ((c ^ (V ? R::swz_v(r) : R::swz_k(r))) << 4);
+                        if (EXACT) copy16(dst + at, src + (i * 32 + lane) * 16);
+                        else if (c * 16 < tok_bytes) copy16(dst + at, src + r * tok_bytes + c * 16);
+                    }
+                }
+            }
+            copy_commit();
+        };
+        using Keys = std::integral_constant<int, 0>;
+        using Values = std::integral_constant<int, 1>;
+
         __syncthreads();                                           // the previous item's shared memory is read
-        if (warp < NT) {
-            const int c = cb * COLS + warp * 8 + g, row = c / a.group, h = kvh * a.group + c % a.group;
+        if (!EXACT) {
+            for (int i = lane; i < 16384 / 16; i += 32) reinterpret_cast<uint4*>(sm.ring[warp])[i] = make_uint4(0, 0, 0, 0);
+            __syncwarp();
+        }
+        {
+            int pgs[STAGES][SUB];
+#pragma unroll
+            for (int j = 0; j < STAGES; j++)
+#pragma unroll
+                for (int u = 0; u < SUB; u++) pgs[j][u] = page_of(j, u);
+#pragma unroll
+            for (int j = 0; j < STAGES; j++) {
+                request(Keys{}, j, pgs[j]);
+                request(Values{}, j, pgs[j]);
+            }
+        }
+
+        // ---- q of the item's columns into operand registers' order, scaled, split into parts
+        for (int x = warp; x < NT * KB; x += WARPS) {              // block n of columns, 32 dims kb
+            const int n = x % NT, kb = x / NT;
+            const int c = cb * COLS + n * 8 + g, row = a.rows == 1 ? (c < a.group ? 0 : 1) : c / a.group, h = kvh * a.group + (c - row * a.group);
             const bool on = row < sp.n;
             const float* qr = a.q + ((size_t)s * a.rows + row) * a.q_ld + (size_t)h * hd;
-            float v[KB][8], top = 0.0f;
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                const int d = 32 * kb + 8 * t;
+            auto eight = [&](int k, float* v) {
+                const int d = 32 * k + 8 * t;
                 float4 x = make_float4(0, 0, 0, 0), y = x;
                 if (on && d < hd) {
                     x = *(const float4*)(qr + d);
                     y = *(const float4*)(qr + d + 4);
                 }
-                const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    v[kb][j] = w[j] * (a.scale * LOG2E);
-                    top = fmaxf(top, fabsf(v[kb][j]));
-                }
-            }
+                const float sl = a.scale * LOG2E;
+                v[0] = x.x * sl; v[1] = x.y * sl; v[2] = x.z * sl; v[3] = x.w * sl;
+                v[4] = y.x * sl; v[5] = y.y * sl; v[6] = y.z * sl; v[7] = y.w * sl;
+            };
+            float v[8];
+            eight(kb, v);
             if (KIND == KIND_F16) {
+                float top = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KB; k++) {
+                    float w[8];
+                    eight(k, w);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(w[i]));
+                }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 // 2^e with top * 2^e in [2^13, 2^14): no part leaves f16's range, and the low part keeps its bits
@@ -242,39 +352,30 @@ __global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a
                 ex = max(-100, min(100, ex));
                 const float f = __uint_as_float((uint32_t)(127 + ex) << 23);
 #pragma unroll
-                for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[kb][j] *= f;
-                if (t == 0) sm.qscale[warp * 8 + g] = __uint_as_float((uint32_t)(127 - ex) << 23);
+                for (int i = 0; i < 8; i++) v[i] *= f;
+                if (t == 0 && kb == 0) sm.qscale[n * 8 + g] = __uint_as_float((uint32_t)(127 - ex) << 23);
             }
+            uint32_t p[4][3];
 #pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                uint32_t p[4][3];
+            for (int i = 0; i < 4; i++) split_pair<KIND>(v[2 * i], v[2 * i + 1], p[i]);
 #pragma unroll
-                for (int j = 0; j < 4; j++) split_pair<KIND>(v[kb][2 * j], v[kb][2 * j + 1], p[j]);
-#pragma unroll
-                for (int k = 0; k < QP; k++) sm.q[warp][kb][k][lane] = make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
-            }
+            for (int k = 0; k < QP; k++) sm.q[n][kb][k][lane] = make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
         }
         __syncthreads();
 
         // ---- this lane's columns: 2t and 2t + 1 of every block of 8
         int p_c[NT][2];                                            // position of the column's row; -1: no such column
         float cs[NT][2];
-        int p_min = 0x7fffffff, p_max = -1;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                const int row = (cb * COLS + n * 8 + 2 * t + k) / a.group;
+                const int c = cb * COLS + n * 8 + 2 * t + k, row = a.rows == 1 ? (c < a.group ? 0 : 1) : c / a.group;
                 p_c[n][k] = row < sp.n ? sp.base + row : -1;
                 cs[n][k] = KIND == KIND_F16 ? sm.qscale[n * 8 + 2 * t + k] : 1.0f;
             }
-        {
-            const int row0 = cb * COLS / a.group, row1 = min((cb * COLS + COLS - 1) / a.group, sp.n - 1);
-            p_min = sp.base + row0;
-            p_max = sp.base + row1;
-        }
+        // its first and last row's positions
+        const int p_min = sp.base + (a.rows == 1 ? 0 : cb * COLS / a.group), p_max = sp.hi - 1;
         float m[NT][2], l[NT][2], o[NT][VB * 4][4];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -284,127 +385,112 @@ __global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a
             for (int i = 0; i < VB * 4; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
         }
 
-        // ---- the warp's tiles: unit i, tile 4 i + warp of the item's list
-        const int* tab = a.table + (size_t)s * a.max_pages;
-        const size_t head_elems = (size_t)a.page * hd;
-        auto tile_key = [&](int i) {                               // first key of the warp's tile of unit i
-            const int x = i * WARPS + warp;
-            return (x < sp.na ? x : x - sp.na + sp.b0) << 4;
-        };
-        auto page_of = [&](int i) {                                // its page
-            if (i * WARPS + warp >= sp.tiles) return 0;
-            const int pg = tab[tile_key(i) / a.page];
-            if (pg >= 0 && pg < a.n_pages) return pg;
-            if (lane == 0) fk_raise(a.err, 97);
-            return 0;
-        };
-        constexpr int KR = KIND == KIND_F32 ? 2 : 1;               // 16-byte pieces of 8 values
-        uint4 kr[KB][2][KR], vr[VB][4][KR];
-        auto request_k = [&](int i, int pg) {
-            const T* base = (const T*)a.data + (2 * (size_t)pg * a.n_kv + kvh) * head_elems + (size_t)(tile_key(i) & (a.page - 1)) * hd;
+        // operand addresses: K token g, dims 32 kb + 8 t; V token lane % 8 (+ 8), dims 16 d (+ 8) (f32: token 2 t, dims 64 vb + 8 g)
+        const uint32_t k_at = ring + g * ROWB;
+        const uint32_t v_at = ring + SUB * TILE +
+                              (KIND == KIND_F32 ? 2 * t * ROWB : ((lane & 7) + 8 * (lane >> 4)) * ROWB + ((((lane >> 3) & 1) ^ (lane & 7)) << 4));
+        for (int j = 0; j < n_steps; j++) {
+            const uint32_t stage = (j % STAGES) * 2 * SUB * TILE;
+            int key0[SUB], pg_next[SUB];
+            bool edge = false;
 #pragma unroll
-            for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                for (int r = 0; r < 2; r++)
-#pragma unroll
-                    for (int k = 0; k < KR; k++) {
-                        const int d = 32 * kb + 8 * t;
-                        kr[kb][r][k] = make_uint4(0, 0, 0, 0);
-                        if (HDP == 64 && hd == 64 || d < hd) kr[kb][r][k] = ld16(base + (size_t)(g + 8 * r) * hd + d + 4 * k);
-                    }
-        };
-        auto request_v = [&](int i, int pg) {
-            const T* base = (const T*)a.data + ((2 * (size_t)pg + 1) * a.n_kv + kvh) * head_elems + (size_t)(tile_key(i) & (a.page - 1)) * hd;
-#pragma unroll
-            for (int vb = 0; vb < VB; vb++)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int k = 0; k < KR; k++) {
-                        const int d = 64 * vb + 8 * g;
-                        vr[vb][r][k] = make_uint4(0, 0, 0, 0);
-                        if (d < hd) vr[vb][r][k] = ld16(base + (size_t)(2 * t + (r & 1) + 8 * (r >> 1)) * hd + d + 4 * k);
-                    }
-        };
-        int pg = i0 < i1 ? page_of(i0) : 0;
-        if (i0 < i1 && i0 * WARPS + warp < sp.tiles) request_k(i0, pg);
-        for (int i = i0; i < i1; i++) {
-            if (i * WARPS + warp >= sp.tiles) break;               // the last unit may be short of tiles
-            const int key0 = tile_key(i);
-            request_v(i, pg);
-            const int pg_next = i + 1 < i1 ? page_of(i + 1) : 0;
-            // scores
-            float sc[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                // two steps of 16 dims: registers 0, 1 and 2, 3 of both rows' pieces
-                uint32_t ka[KIND == KIND_F32 ? 3 : 1][2][4];
-                if (KIND == KIND_F32) {
-#pragma unroll
-                    for (int r = 0; r < 2; r++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const uint4 x = kr[kb][r][KR - 1 == 0 ? 0 : j >> 1];
-                            uint32_t p[3];
-                            split_pair<FK_BF16>(__uint_as_float(j & 1 ? x.z : x.x), __uint_as_float(j & 1 ? x.w : x.y), p);
-#pragma unroll
-                            for (int k = 0; k < 3; k++) ka[KIND == KIND_F32 ? k : 0][j >> 1][r + 2 * (j & 1)] = p[k];
-                        }
-                } else {
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        ka[0][h][0] = h ? kr[kb][0][0].z : kr[kb][0][0].x;
-                        ka[0][h][1] = h ? kr[kb][1][0].z : kr[kb][1][0].x;
-                        ka[0][h][2] = h ? kr[kb][0][0].w : kr[kb][0][0].y;
-                        ka[0][h][3] = h ? kr[kb][1][0].w : kr[kb][1][0].y;
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int k = QP - 1; k >= 0; k--) {            // the small parts first
-                        const uint4 qv = sm.q[n][kb][k][lane];
-#pragma unroll
-                        for (int kk = (KIND == KIND_F32 ? 2 - k : 0); kk >= 0; kk--) {
-                            mma<KIND>(x, ka[kk][0], qv.x, qv.y);
-                            mma<KIND>(x, ka[kk][1], qv.z, qv.w);
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; k++) sc[n][k] += x[k];
-                }
+            for (int u = 0; u < SUB; u++) {
+                key0[u] = tile_key(j, u);
+                pg_next[u] = page_of(j + STAGES, u);
+                // a tile that reaches over the newest key or the window's start
+                edge = edge || key0[u] + 15 > p_min || (a.window > 0 && key0[u] <= p_max - a.window && key0[u] + 15 >= a.first);
             }
-            if (KIND != KIND_F32 && (i + 1) * WARPS + warp < sp.tiles && i + 1 < i1) request_k(i + 1, pg_next);
-            // masks: only where a tile reaches over an edge
-            const bool edge = key0 + 15 > p_min || (a.window > 0 && key0 <= p_max - a.window && key0 + 15 >= a.first);
+            copy_wait<2 * STAGES - 1>();
+            __syncwarp();
+            // scores
+            float sc[SUB][NT][4];
+#pragma unroll
+            for (int u = 0; u < SUB; u++)
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++) {
+                    // two steps of 16 dims: registers 0, 1 and 2, 3 of both rows' pieces
+                    uint32_t ka[KIND == KIND_F32 ? 3 : 1][2][4];
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const uint32_t row = k_at + stage + u * TILE + 8 * r * ROWB;
+                        if (KIND == KIND_F32) {
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const uint4 x = lds16(row + (((8 * kb + 2 * t + h) ^ R::swz_k(g)) << 4));
+                                uint32_t p[3], q[3];
+                                split_pair<FK_BF16>(__uint_as_float(x.x), __uint_as_float(x.y), p);
+                                split_pair<FK_BF16>(__uint_as_float(x.z), __uint_as_float(x.w), q);
+#pragma unroll
+                                for (int k = 0; k < 3; k++) {
+                                    ka[KIND == KIND_F32 ? k : 0][h][r] = p[k];
+                                    ka[KIND == KIND_F32 ? k : 0][h][r + 2] = q[k];
+                                }
+                            }
+                        } else {
+                            const uint4 x = lds16(row + (((4 * kb + t) ^ R::swz_k(g)) << 4));
+                            ka[0][0][r] = x.x;
+                            ka[0][0][r + 2] = x.y;
+                            ka[0][1][r] = x.z;
+                            ka[0][1][r + 2] = x.w;
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        float x[4];
+#pragma unroll
+                        for (int k = QP - 1; k >= 0; k--) {        // the small parts first
+                            const uint4 qv = sm.q[n][kb][k][lane];
+#pragma unroll
+                            for (int kk = (KIND == KIND_F32 ? 2 - k : 0); kk >= 0; kk--) {
+                                if (k == QP - 1 && kk == (KIND == KIND_F32 ? 2 - k : 0)) mma0<KIND>(x, ka[kk][0], qv.x, qv.y);
+                                else mma<KIND>(x, ka[kk][0], qv.x, qv.y);
+                                mma<KIND>(x, ka[kk][1], qv.z, qv.w);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; k++) sc[u][n][k] = kb == 0 ? x[k] : sc[u][n][k] + x[k];
+                    }
+                }
+            __syncwarp();
+            request(Keys{}, j + STAGES, pg_next);
+            if (KIND == KIND_F16) {
+#pragma unroll
+                for (int u = 0; u < SUB; u++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) sc[u][n][k] *= cs[n][k & 1];
+            }
             if (edge) {
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int u = 0; u < SUB; u++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const int j = key0 + g + 8 * (k >> 1), p = p_c[n][k & 1];
-                        const bool vis = j <= p && (a.window <= 0 || j > p - a.window || j < a.first);
-                        sc[n][k] = vis ? sc[n][k] * cs[n][k & 1] : -INFINITY;
-                    }
-            } else if (KIND == KIND_F16) {
+                    for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) sc[n][k] *= cs[n][k & 1];
+                        for (int k = 0; k < 4; k++) {
+                            const int x = key0[u] + g + 8 * (k >> 1), p = p_c[n][k & 1];
+                            const bool vis = x <= p && (a.window <= 0 || x > p - a.window || x < a.first);
+                            if (!vis) sc[u][n][k] = -INFINITY;
+                        }
             }
             // a new maximum anywhere in the warp: find it and rescale (rare once a sequence is under way)
+            float top[NT][2];
             bool up = false;
 #pragma unroll
-            for (int n = 0; n < NT; n++) up = up || fmaxf(sc[n][0], sc[n][2]) > m[n][0] || fmaxf(sc[n][1], sc[n][3]) > m[n][1];
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    float x = fmaxf(sc[0][n][k], sc[0][n][2 + k]);
+                    if (SUB == 2) x = fmaxf(x, fmaxf(sc[SUB - 1][n][k], sc[SUB - 1][n][2 + k]));
+                    top[n][k] = x;
+                    up = up || x > m[n][k];
+                }
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
-                        float x = fmaxf(fmaxf(sc[n][k], sc[n][2 + k]), m[n][k]);
+                        float x = fmaxf(top[n][k], m[n][k]);
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -419,64 +505,90 @@ __global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a
                     }
             }
             // weights, as parts in the layout of the second product's operand
-            uint32_t wp[NT][QP][2];
+            uint32_t wp[SUB][NT][QP][2];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0] - SHIFT, m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1] - SHIFT;
-                const float w0 = pow2(sc[n][0] - m0), w1 = pow2(sc[n][1] - m1), w2 = pow2(sc[n][2] - m0), w3 = pow2(sc[n][3] - m1);
-                l[n][0] += w0 + w2;
-                l[n][1] += w1 + w3;
-                uint32_t a0[3], a1[3];
-                split_pair<KIND>(w0, w1, a0);
-                split_pair<KIND>(w2, w3, a1);
 #pragma unroll
-                for (int k = 0; k < QP; k++) {
-                    wp[n][k][0] = transposed(a0[k]);
-                    wp[n][k][1] = transposed(a1[k]);
+                for (int u = 0; u < SUB; u++) {
+                    const float w0 = pow2(sc[u][n][0] - m0), w1 = pow2(sc[u][n][1] - m1), w2 = pow2(sc[u][n][2] - m0), w3 = pow2(sc[u][n][3] - m1);
+                    l[n][0] += w0 + w2;
+                    l[n][1] += w1 + w3;
+                    uint32_t a0[3], a1[3];
+                    split_pair<KIND>(w0, w1, a0);
+                    split_pair<KIND>(w2, w3, a1);
+#pragma unroll
+                    for (int k = 0; k < QP; k++) {
+                        wp[u][n][k][0] = transposed(a0[k]);
+                        wp[u][n][k][1] = transposed(a1[k]);
+                    }
                 }
             }
-            // A value whose key no column of the item sees may be anything, NaN among it: it must not meet a weight of 0.
-            // Values that some columns see and others do not are finite in any sane model; where one is not, the columns'
-            // rows are taken one by one, each with the values it does not see as zeros.
-            int passes = 1;
-            if (edge) {
-                bool odd = false;
+            copy_wait<2 * STAGES - 1>();
+            __syncwarp();
+            // o += V^T w.  MODE 0: every column sees every token.  MODE 1: values whose keys no column sees become zeros, whatever
+            // they are (stale memory, NaN): they must not meet a weight of 0.  MODE 2: the columns of one row, with the values
+            // that it does not see as zeros.
+            auto fold = [&](auto mode, int p_lo, int p_hi) {
+                constexpr int MODE = decltype(mode)::value;
+                uint32_t keep[SUB][2];
+                bool mine[NT];
+                if (MODE) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int j = key0 + 2 * t + (r & 1) + 8 * (r >> 1);
-                    const bool some = j <= p_max && (a.window <= 0 || j > p_min - a.window || j < a.first);
-                    const bool every = j <= p_min && (a.window <= 0 || j > p_max - a.window || j < a.first);
+                    for (int u = 0; u < SUB; u++) {
+                        keep[u][0] = keep[u][1] = 0xffffffffu;
 #pragma unroll
-                    for (int vb = 0; vb < VB; vb++)
+                        for (int r = 0; r < 4; r++) {
+                            const int k = key0[u] + 2 * t + (r & 1) + 8 * (r >> 1);
+                            if (!(k <= p_hi && (a.window <= 0 || k > p_lo - a.window || k < a.first))) keep[u][r >> 1] &= r & 1 ? 0x0000ffffu : 0xffff0000u;
+                        }
+                    }
 #pragma unroll
-                        for (int k = 0; k < KR; k++) {
-                            uint4& x = vr[vb][r][k];
-                            if (!some) x = make_uint4(0, 0, 0, 0);
-                            else if (!every) {
-                                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                    for (int n = 0; n < NT; n++) mine[n] = MODE != 2 || sp.base + (cb * COLS + n * 8 + g) / a.group == p_lo;      // the operand's column g
+                }
+                auto block = [&](int d, uint32_t (&va)[SUB][KIND == KIND_F32 ? 3 : 1][4]) {
+                    if (MODE) {
 #pragma unroll
-                                for (int q = 0; q < 4; q++) {
-                                    if (KIND == KIND_F32) odd = odd || (w[q] & 0x7f800000u) == 0x7f800000u;
-                                    else if (KIND == KIND_F16) odd = odd || (w[q] & 0x7c00u) == 0x7c00u || (w[q] & 0x7c000000u) == 0x7c000000u;
-                                    else odd = odd || (w[q] & 0x7f80u) == 0x7f80u || (w[q] & 0x7f800000u) == 0x7f800000u;
+                        for (int u = 0; u < SUB; u++)
+#pragma unroll
+                            for (int q = 0; q < (KIND == KIND_F32 ? 3 : 1); q++)
+#pragma unroll
+                                for (int h = 0; h < 4; h++) va[u][q][h] &= keep[u][h >> 1];
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        float x[4];
+#pragma unroll
+                        for (int k = QP - 1; k >= 0; k--)
+#pragma unroll
+                            for (int u = 0; u < SUB; u++) {
+                                const uint32_t b0 = MODE != 2 || mine[n] ? wp[u][n][k][0] : 0u, b1 = MODE != 2 || mine[n] ? wp[u][n][k][1] : 0u;
+#pragma unroll
+                                for (int kk = (KIND == KIND_F32 ? 2 - k : 0); kk >= 0; kk--) {
+                                    if (k == QP - 1 && u == 0 && kk == (KIND == KIND_F32 ? 2 - k : 0)) mma0<KIND>(x, va[u][kk], b0, b1);
+                                    else mma<KIND>(x, va[u][kk], b0, b1);
                                 }
                             }
-                        }
-                }
-                if (__any_sync(0xffffffffu, odd)) passes = p_max - p_min + 1;
-            }
-            for (int ps = 0; ps < passes; ps++) {
-                const int p_row = p_min + ps;
 #pragma unroll
-                for (int vb = 0; vb < VB; vb++) {
+                        for (int k = 0; k < 4; k++) o[n][d][k] += x[k];
+                    }
+                };
+                if (KIND == KIND_F32) {
 #pragma unroll
-                    for (int d = 0; d < 4; d++) {                  // dims 64 vb + 8 g + 2 d and + 1
-                        uint32_t va[KIND == KIND_F32 ? 3 : 1][4];
-                        if (KIND == KIND_F32) {
+                    for (int vb = 0; vb < VB; vb++) {
+                        uint4 v[4][2];
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++)
+                                v[r][h] = lds16(v_at + stage + ((r & 1) + 8 * (r >> 1)) * ROWB + (((2 * (8 * vb + g) + h) ^ R::swz_v(2 * t)) << 4));
+#pragma unroll
+                        for (int d = 0; d < 4; d++) {              // dims 64 vb + 8 g + 2 d and + 1
+                            uint32_t va[SUB][KIND == KIND_F32 ? 3 : 1][4];
                             float x[4][2];
 #pragma unroll
                             for (int r = 0; r < 4; r++) {
-                                const uint4 y = vr[vb][r][KR - 1 == 0 ? 0 : d >> 1];
+                                const uint4 y = v[r][d >> 1];
                                 x[r][0] = __uint_as_float(d & 1 ? y.z : y.x);
                                 x[r][1] = __uint_as_float(d & 1 ? y.w : y.y);
                             }
@@ -487,52 +599,52 @@ __global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a
                                     uint32_t p[3];
                                     split_pair<FK_BF16>(x[2 * h][k], x[2 * h + 1][k], p);
 #pragma unroll
-                                    for (int q = 0; q < 3; q++) va[KIND == KIND_F32 ? q : 0][2 * h + k] = p[q];
+                                    for (int q = 0; q < 3; q++) va[0][KIND == KIND_F32 ? q : 0][2 * h + k] = p[q];
                                 }
-                        } else {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int r = 0; r < 4; r++) w[r] = d == 0 ? vr[vb][r][0].x : d == 1 ? vr[vb][r][0].y : d == 2 ? vr[vb][r][0].z : vr[vb][r][0].w;
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                va[0][2 * h] = __byte_perm(w[2 * h], w[2 * h + 1], 0x5410);
-                                va[0][2 * h + 1] = __byte_perm(w[2 * h], w[2 * h + 1], 0x7632);
-                            }
+                            block(vb * 4 + d, va);
                         }
-                        if (passes > 1) {
-                            // tokens of this lane's operand that the row does not see
+                    }
+                } else {
 #pragma unroll
-                            for (int r = 0; r < 4; r++) {
-                                const int j = key0 + 2 * t + (r & 1) + 8 * (r >> 1);
-                                if (j <= p_row && (a.window <= 0 || j > p_row - a.window || j < a.first)) continue;
-                                const uint32_t keep = r & 1 ? 0x0000ffffu : 0xffff0000u;
+                    for (int d = 0; d < VB * 4; d++) {             // dims 16 d + g and + 8
+                        uint32_t va[SUB][KIND == KIND_F32 ? 3 : 1][4];
 #pragma unroll
-                                for (int q = 0; q < (KIND == KIND_F32 ? 3 : 1); q++) {
-                                    va[q][2 * (r >> 1)] &= keep;
-                                    va[q][2 * (r >> 1) + 1] &= keep;
-                                }
-                            }
-                        }
+                        for (int u = 0; u < SUB; u++) ldsm_t(va[u][0], (v_at + stage + u * TILE) ^ (d << 5));
+                        block(d, va);
+                    }
+                }
+            };
+            if (!edge) {
+                fold(std::integral_constant<int, 0>{}, 0, 0);
+            } else {
+                // Values that some columns see and others do not are finite in any sane model; where one is not, the columns'
+                // rows are taken one by one.
+                bool odd = false;
+                if (p_max > p_min) {
+                    for (int x = lane; x < SUB * TILE / 16; x += 32) {
+                        const int u = x / (TILE / 16), k = key0[SUB == 2 ? u : 0] + (x / (ROWB / 16)) % 16;
+                        const bool some = k <= p_max && (a.window <= 0 || k > p_min - a.window || k < a.first);
+                        const bool every = k <= p_min && (a.window <= 0 || k > p_max - a.window || k < a.first);
+                        if (!some || every) continue;
+                        const uint4 y = lds16(ring + stage + SUB * TILE + x * 16);
+                        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            // of the operand's column g only the row of this pass
-                            const bool mine = passes == 1 || sp.base + (cb * COLS + n * 8 + g) / a.group == p_row;
-                            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                            for (int k = QP - 1; k >= 0; k--) {
-                                const uint32_t b0 = mine ? wp[n][k][0] : 0u, b1 = mine ? wp[n][k][1] : 0u;
-#pragma unroll
-                                for (int kk = (KIND == KIND_F32 ? 2 - k : 0); kk >= 0; kk--) mma<KIND>(x, va[kk], b0, b1);
-                            }
-#pragma unroll
-                            for (int k = 0; k < 4; k++) o[n][vb * 4 + d][k] += x[k];
+                        for (int q = 0; q < 4; q++) {
+                            if (KIND == KIND_F32) odd = odd || (w[q] & 0x7f800000u) == 0x7f800000u;
+                            else if (KIND == KIND_F16) odd = odd || (w[q] & 0x7c00u) == 0x7c00u || (w[q] & 0x7c000000u) == 0x7c000000u;
+                            else odd = odd || (w[q] & 0x7f80u) == 0x7f80u || (w[q] & 0x7f800000u) == 0x7f800000u;
                         }
                     }
                 }
+                if (!__any_sync(0xffffffffu, odd)) fold(std::integral_constant<int, 1>{}, p_min, p_max);
+                else
+                    for (int p = p_min; p <= p_max; p++) fold(std::integral_constant<int, 2>{}, p, p);
             }
-            pg = pg_next;
-            if (KIND == KIND_F32 && (i + 1) * WARPS + warp < sp.tiles && i + 1 < i1) request_k(i + 1, pg);
+            __syncwarp();
+            request(Values{}, j + STAGES, pg_next);
         }
+        copy_wait<0>();
+        __syncwarp();
 
         // ---- join the warps
 #pragma unroll
@@ -549,8 +661,13 @@ __global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a
                 }
 #pragma unroll
                 for (int d = 0; d < VB * 4; d++) {
-                    float* dst = sm.o[warp][n * 8 + 2 * t + k] + 64 * (d >> 2) + 8 * g + 2 * (d & 3);
-                    *(float2*)dst = make_float2(o[n][d][k], o[n][d][2 + k]);
+                    float* dst = sum_o + (n * 8 + 2 * t + k) * PITCH;
+                    if (KIND == KIND_F32) {
+                        *(float2*)(dst + 64 * (d >> 2) + 8 * g + 2 * (d & 3)) = make_float2(o[n][d][k], o[n][d][2 + k]);
+                    } else {
+                        dst[16 * d + g] = o[n][d][k];
+                        dst[16 * d + 8 + g] = o[n][d][2 + k];
+                    }
                 }
             }
         __syncthreads();
@@ -567,7 +684,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a
 #pragma unroll
             for (int w = 0; w < WARPS; w++) {
                 const float f = sm.m[w][c] == -INFINITY ? (sm.l[w][c] != sm.l[w][c] ? sm.l[w][c] : 0.0f) : pow2(sm.m[w][c] - M);
-                const float4 v = *(const float4*)(sm.o[w][c] + d);
+                const float4 v = *(const float4*)(reinterpret_cast<const float*>(sm.ring[w]) + c * PITCH + d);
                 L += sm.l[w][c] * f;
                 O.x += v.x * f; O.y += v.y * f; O.z += v.z * f; O.w += v.w * f;
             }
@@ -627,8 +744,8 @@ __global__ void __launch_bounds__(WARPS * 32) attn_paged_kernel(const AttnArgs a
     }
 }
 
-template <int KIND, int HDP, int NT> int launch_attn(fk_ctx* ctx, cudaStream_t st, AttnArgs a) {
-    auto kern = attn_paged_kernel<KIND, HDP, NT>;
+template <int KIND, int HDP, bool EXACT, int NT> int launch_attn(fk_ctx* ctx, cudaStream_t st, AttnArgs a) {
+    auto kern = attn_paged_kernel<KIND, HDP, EXACT, NT>;
     const size_t smem = sizeof(Smem<KIND, HDP, NT>);
     static thread_local int resident[64] = {};                     // CTAs an SM holds, by device
     int& per_sm = resident[ctx->device & 63];
@@ -650,8 +767,9 @@ template <int KIND, int HDP, int NT> int launch_attn(fk_ctx* ctx, cudaStream_t s
 
 template <int KIND> int launch_kind(fk_ctx* ctx, cudaStream_t st, const AttnArgs& a) {
     const bool wide = (long long)a.rows * a.group > 8;
-    if (a.head_dim <= 64) return wide ? launch_attn<KIND, 64, 2>(ctx, st, a) : launch_attn<KIND, 64, 1>(ctx, st, a);
-    return wide ? launch_attn<KIND, 128, 2>(ctx, st, a) : launch_attn<KIND, 128, 1>(ctx, st, a);
+    if (a.head_dim == 64) return wide ? launch_attn<KIND, 64, true, 2>(ctx, st, a) : launch_attn<KIND, 64, true, 1>(ctx, st, a);
+    if (a.head_dim == 128) return wide ? launch_attn<KIND, 128, true, 2>(ctx, st, a) : launch_attn<KIND, 128, true, 1>(ctx, st, a);
+    return wide ? launch_attn<KIND, 128, false, 2>(ctx, st, a) : launch_attn<KIND, 128, false, 1>(ctx, st, a);
 }
 
 }  // namespace
@@ -670,7 +788,7 @@ FK_EXPORT int fk_attention_paged(fk_ctx* ctx, void* stream, const fk_pages* p, i
     FkDeviceGuard g(ctx->device);
     AttnArgs a{(const char*)p->data_dev + (size_t)layer * page_bytes(p) * p->n_pages, p->table_dev, p->lens_dev, n_new_dev, q_dev, sinks_dev, out_dev,
                (unsigned*)p->ws_dev, (float*)((char*)p->ws_dev + WS_COUNTERS), ctx->err_flag, scale, q_ld, rows, p->n_seqs, n_heads, p->n_kv,
-               n_heads / p->n_kv, p->head_dim, p->page, p->n_pages, p->max_pages, window, first, 0, 0};
+               n_heads / p->n_kv, p->head_dim, p->page, p->page == 16 ? 4 : p->page == 32 ? 5 : p->page == 64 ? 6 : 7, p->n_pages, p->max_pages, window, first, 0, 0};
     cudaStream_t st = (cudaStream_t)stream;
     rc = p->kind == KIND_F32 ? launch_kind<KIND_F32>(ctx, st, a) : p->kind == KIND_F16 ? launch_kind<KIND_F16>(ctx, st, a) : launch_kind<FK_BF16>(ctx, st, a);
     if (rc != FK_OK) return rc;
