@@ -790,7 +790,9 @@ FK_EXPORT int fk_attention_paged(fk_ctx* ctx, void* stream, const fk_pages* p, i
                (unsigned*)p->ws_dev, (float*)((char*)p->ws_dev + WS_COUNTERS), ctx->err_flag, scale, q_ld, rows, p->n_seqs, n_heads, p->n_kv,
                n_heads / p->n_kv, p->head_dim, p->page, p->page == 16 ? 4 : p->page == 32 ? 5 : p->page == 64 ? 6 : 7, p->n_pages, p->max_pages, window, first, 0, 0};
     cudaStream_t st = (cudaStream_t)stream;
-    rc = p->kind == KIND_F32 ? launch_kind<KIND_F32>(ctx, st, a) : p->kind == KIND_F16 ? launch_kind<KIND_F16>(ctx, st, a) : launch_kind<FK_BF16>(ctx, st, a);
+    if (fk_attn_prompt_takes(ctx, p, rows, n_heads))
+        rc = fk_attn_prompt_launch(ctx, st, p, layer, q_dev, q_ld, rows, n_new_dev, n_heads, scale, window, first, sinks_dev, out_dev);
+    else rc = p->kind == KIND_F32 ? launch_kind<KIND_F32>(ctx, st, a) : p->kind == KIND_F16 ? launch_kind<KIND_F16>(ctx, st, a) : launch_kind<FK_BF16>(ctx, st, a);
     if (rc != FK_OK) return rc;
     FK_CUDA(cudaGetLastError(), FK_LAUNCH);
     ctx->launches++;

@@ -1,0 +1,538 @@
+// Attention of a prompt's rows over a paged KV cache on the tensor cores (tcgen05): 16-bit pages, heads of 64 or 128.  The
+// mathematics, the masks and the precision are those of fk_attn_paged.cu.
+//
+// A CTA takes 128 (row, query head) pairs of one KV head -- 128 / group consecutive rows, so a short prompt still fills the
+// tile -- and walks the visible keys in tiles of 64:
+//
+//   S = q K^T          A = q's parts in tensor memory, B = a tile of K in shared memory, S in tensor memory (two buffers)
+//   w = 2^(S - m)      a thread per (row, half of the tile's keys); its parts go back over S as the next product's A operand
+//   O = w V            A = w's parts, B = the tile of V as it lies in memory (the major axis is its dims)
+//   o = o c + O        in registers: the running output is rescaled and added to in f32, rounded, because a sum that stayed
+//                      in the tensor core over a long prompt would be cut off thousands of times
+//
+// bf16 takes three parts of q and w, f16 two (fk_attn_paged.cu says why that is f32 precision), so a product is three (two)
+// products: the bound is the tensor cores' rate by that factor.  Per tile of 64 keys and 128 dims that is 1536 (1024) cycles of
+// MMA against some 900 issue slots of each scheduler's two softmax warps, which run beside it on the other buffer.
+//
+// Warps: 0 loads tiles (a lane per page piece, TMA with 128-byte swizzle), 1 issues the products, 2 looks over the values of
+// tiles that not every row sees, 4 to 11 are the softmax.  A value that no row sees is zeroed in shared memory (stale memory may
+// hold NaN); one that some rows see and that is not finite is zeroed too and added in plain f32 for the rows that see it.
+#include "fk_paged.cuh"
+#include "fk_tc.cuh"
+
+#include <type_traits>
+
+using namespace fk_paged;
+using namespace fk_tc;
+
+namespace {
+
+constexpr int KT = 64;                         // keys of a tile
+constexpr int THREADS = 384;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr uint32_t SPINS = 1u << 20;           // polls of a wait before it gives up
+
+struct PromptArgs {
+    CUtensorMap map;                           // the layer's pages as [tokens of all pages, halves and heads][head_dim]
+    const void* data;
+    const int *table, *lens, *n_new;
+    const float *q, *sinks;
+    float* out;
+    int* err;
+    float scale;
+    int q_ld, rows, n_seqs, n_heads, n_kv, group, page, log_page, n_pages, max_pages, window, first, rq, n_rb;
+};
+
+template <int KIND, int HD> struct Plan {
+    static constexpr int QP = KIND == KIND_F16 ? 2 : 3;            // parts of q and of the weights
+    static constexpr int TILE = KT * HD * 2;                       // bytes of a tile of K or V
+    static constexpr int STAGES = HD == 64 ? 6 : 4;
+    static constexpr int SREG = QP == 3 ? 96 : 64;                 // tensor memory columns of S (64), then of w's parts (32 each)
+    static constexpr int Q0 = 0, O0 = QP * HD / 2, S0 = O0 + HD;
+    static_assert(S0 + 2 * SREG <= 512, "tensor memory");
+};
+
+template <int KIND, int HD> struct PromptSmem {
+    using P = Plan<KIND, HD>;
+    unsigned char k[P::STAGES][P::TILE];
+    unsigned char v[P::STAGES][P::TILE];
+    float odd_w[KT][128];                      // weights of a tile's values that are not finite, by row (-1: the row does not see it)
+    float top[2][2][128];                      // a row's maximum over each half of the tile's keys, two tiles' worth
+    unsigned long long odd[P::STAGES];         // which of a tile's values are not finite
+    unsigned long long kfull[P::STAGES], kfree[P::STAGES], vfull[P::STAGES], vfree[P::STAGES], vready[P::STAGES];
+    unsigned long long sfull[2], pfull[2], ofull, ofree, qfull, done;
+    uint32_t tmem;
+    int abort;
+};
+
+// d (+)= a b, issued by the lane whose `on` is set: A in tensor memory
+__device__ __forceinline__ void mma_ts(uint32_t on, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %9, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0), "r"(on) : "memory");
+}
+// f32 sums of f16 or bf16 products; b_mn: B's major axis is N
+__host__ __device__ constexpr uint32_t idesc_of(int kind, int m, int n, int b_mn) {
+    return (1u << 4) | (kind == KIND_F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ float pow2f(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// (lo, hi) rounded to a pair of the type; lo and hi become what is left
+template <int KIND> __device__ __forceinline__ uint32_t take_part(float& lo, float& hi) {
+    uint32_t r;
+    if (KIND == KIND_F16) {
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        const __half2 h = *(const __half2*)&r;
+        lo -= __low2float(h);
+        hi -= __high2float(h);
+    } else {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        lo -= __uint_as_float(r << 16);
+        hi -= __uint_as_float(r & 0xffff0000u);
+    }
+    return r;
+}
+template <int N> __device__ __forceinline__ void tm_ld(uint32_t addr, float* v) {
+    static_assert(N == 32 || N == 64, "");
+#pragma unroll
+    for (int i = 0; i < N; i += 32) tc_ld32(addr + i, reinterpret_cast<uint32_t*>(v) + i);
+    tc_wait_ld();
+    tc_ld_fence<N>(reinterpret_cast<uint32_t*>(v));
+}
+
+template <int KIND, int HD>
+__global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_constant__ PromptArgs a) {
+    using P = Plan<KIND, HD>;
+    constexpr int QP = P::QP, STAGES = P::STAGES, HALF = HD / 2;
+    constexpr float SHIFT = KIND == KIND_F16 ? 14.0f : 0.0f;
+    extern __shared__ unsigned char smem_raw[];
+    PromptSmem<KIND, HD>& sm = *reinterpret_cast<PromptSmem<KIND, HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < STAGES; i++) {
+            mbar_init(smem_u32(&sm.kfull[i]), 1);
+            mbar_init(smem_u32(&sm.kfree[i]), 1);
+            mbar_init(smem_u32(&sm.vfull[i]), 1);
+            mbar_init(smem_u32(&sm.vfree[i]), 1);
+            mbar_init(smem_u32(&sm.vready[i]), 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_u32(&sm.sfull[i]), 1);
+            mbar_init(smem_u32(&sm.pfull[i]), 8);
+        }
+        mbar_init(smem_u32(&sm.ofull), 1);
+        mbar_init(smem_u32(&sm.ofree), 8);
+        mbar_init(smem_u32(&sm.qfull), 8);
+        mbar_init(smem_u32(&sm.done), 1);
+        sm.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // Tensor memory is taken after the previous kernel is done with its own and before the next one may start: neither can
+    // then hold what the other waits for.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // a wait gives up after SPINS polls, or at once when another one of the CTA has given up; the CTA then runs to its end
+    auto wait = [&](unsigned long long* bar, uint32_t parity) {
+        const uint32_t b = smem_u32(bar);
+        for (uint32_t i = 0; i < SPINS; i++) {
+            if (mbar_try_wait(b, parity)) return;
+            if (*(volatile int*)&sm.abort) return;
+        }
+        *(volatile int*)&sm.abort = 1;
+        fk_raise(a.err, 63);
+    };
+    auto gave_up = [&] { return __any_sync(0xffffffffu, *(volatile int*)&sm.abort) != 0; };      // the same answer for the whole warp
+
+    // ---- the item: rows [row0, row1] of sequence s, KV head kvh; long ones (late rows) come first
+    const int kvh = blockIdx.x % a.n_kv, s = (blockIdx.x / a.n_kv) % a.n_seqs, rb = a.n_rb - 1 - (int)(blockIdx.x / ((unsigned)a.n_kv * a.n_seqs));
+    int n = a.n_new ? min(max(a.n_new[s], 0), a.rows) : a.rows;
+    const int base = a.lens[s];
+    if (base < 0 || (long long)base + n > (long long)a.max_pages * a.page) {
+        if (tid == 0 && n > 0) fk_raise(a.err, 95);
+        n = 0;
+    }
+    const int row0 = rb * a.rq, row1 = min(row0 + a.rq, n) - 1;
+    // keys [0, 64 na) and [64 b0, hi)
+    const int hi = base + row1 + 1, lo = a.window > 0 ? max(0, base + row0 + 1 - a.window) : 0;
+    int b0 = lo / KT, na = (min(a.first, lo) + KT - 1) / KT;
+    if (na >= b0) na = b0 = 0;
+    const int n_tiles = row1 < row0 ? 0 : na + (hi + KT - 1) / KT - b0;
+    const int p_min = base + row0, p_max = hi - 1;
+    auto tile_key = [&](int j) { return (j < na ? j : j - na + b0) * KT; };
+    auto edge_tile = [&](int key0) { return key0 + KT - 1 > p_min || (a.window > 0 && key0 <= p_max - a.window && key0 + KT - 1 >= a.first); };
+
+    if (warp == 0) {
+        // ---- loads: lane u takes the u-th page piece of a tile
+        const int piece = min(a.page, KT), n_pc = KT / piece;
+        auto page_of = [&](int j) {
+            if (j >= n_tiles || lane >= n_pc) return 0;
+            const int key = tile_key(j) + lane * piece;
+            if (key >= hi) return -1;
+            const int pg = a.table[(size_t)s * a.max_pages + (key >> a.log_page)];
+            if (pg >= 0 && pg < a.n_pages) return pg;
+            fk_raise(a.err, 97);
+            return 0;
+        };
+        int pg = page_of(0), issued = 0;
+        for (int j = 0; j < n_tiles; j++) {
+            const int pg_next = page_of(j + 1), st = j % STAGES;
+            const int key = tile_key(j) + lane * piece;
+            const int pieces = min(n_pc, (hi - tile_key(j) + piece - 1) / piece);
+            const bool mine = lane < n_pc && pg >= 0;
+            const int y = ((2 * max(pg, 0)) * a.n_kv + kvh) * a.page + (key & (a.page - 1));
+            if (j >= STAGES) wait(&sm.kfree[st], (j / STAGES - 1) & 1);
+            if (j >= STAGES) wait(&sm.vfree[st], (j / STAGES - 1) & 1);
+            if (gave_up()) break;
+            if (lane == 0) mbar_expect_tx(smem_u32(&sm.kfull[st]), pieces * piece * HD * 2);
+            __syncwarp();
+            if (mine) {
+#pragma unroll
+                for (int h = 0; h < HD / 64; h++)
+                    tma_load_2d(smem_u32(sm.k[st]) + h * (KT * 128) + lane * piece * 128, &a.map, h * 64, y, smem_u32(&sm.kfull[st]));
+            }
+            if (lane == 0) mbar_expect_tx(smem_u32(&sm.vfull[st]), pieces * piece * HD * 2);
+            __syncwarp();
+            if (mine) {
+#pragma unroll
+                for (int h = 0; h < HD / 64; h++)
+                    tma_load_2d(smem_u32(sm.v[st]) + h * (KT * 128) + lane * piece * 128, &a.map, h * 64, y + a.n_kv * a.page, smem_u32(&sm.vfull[st]));
+            }
+            pg = pg_next;
+            issued = j + 1;
+        }
+        // every copy that was started has landed before the CTA ends
+        for (int j = max(0, issued - STAGES); j < issued; j++) {
+            const uint32_t par = (j / STAGES) & 1;
+            for (uint32_t i = 0; i < SPINS && !mbar_try_wait(smem_u32(&sm.kfull[j % STAGES]), par); i++) {}
+            for (uint32_t i = 0; i < SPINS && !mbar_try_wait(smem_u32(&sm.vfull[j % STAGES]), par); i++) {}
+        }
+    } else if (warp == 1) {
+        // ---- products
+        const uint32_t on = lane == 0;
+        constexpr uint32_t ID_S = idesc_of(KIND, 128, KT, 0), ID_O = idesc_of(KIND, 128, HD, 1);
+        auto scores = [&](int j) {
+            const int st = j % STAGES;
+            wait(&sm.kfull[st], (j / STAGES) & 1);
+            tc_fence_after();
+            const uint32_t d = tmem + P::S0 + (j & 1) * P::SREG;
+            uint32_t acc = 0;
+#pragma unroll
+            for (int k = QP - 1; k >= 0; k--)                      // the small parts first
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ks++) {
+                    const uint64_t b = umma_desc(smem_u32(sm.k[st]) + (ks >> 2) * (KT * 128) + (ks & 3) * 32);
+                    mma_ts(on, d, tmem + P::Q0 + k * HALF + ks * 8, b, ID_S, acc);
+                    acc = 1;
+                }
+            tc_commit_if(on, smem_u32(&sm.sfull[j & 1]));
+            tc_commit_if(on, smem_u32(&sm.kfree[st]));
+        };
+        if (n_tiles > 0) {
+            wait(&sm.qfull, 0);
+            tc_fence_after();
+            scores(0);
+        }
+        for (int j = 0; j < n_tiles && !gave_up(); j++) {
+            if (j + 1 < n_tiles) {
+                // S of tile j + 1 takes the place of w of tile j - 1: products with different results may pass one another
+                if (j > 0) wait(&sm.vfree[(j - 1) % STAGES], ((j - 1) / STAGES) & 1);
+                scores(j + 1);
+            }
+            const int st = j % STAGES;
+            wait(&sm.vready[st], (j / STAGES) & 1);
+            wait(&sm.pfull[j & 1], (j >> 1) & 1);
+            if (j > 0) wait(&sm.ofree, (j - 1) & 1);
+            tc_fence_after();
+            uint32_t acc = 0;
+#pragma unroll
+            for (int k = QP - 1; k >= 0; k--)
+#pragma unroll
+                for (int ks = 0; ks < KT / 16; ks++) {
+                    // 16 keys of all dims: 64-dim halves KT * 128 bytes apart, groups of 8 keys 1024 bytes apart
+                    const uint64_t b = umma_desc_of(smem_u32(sm.v[st]) + ks * 2048, KT * 128, 1024, 2);
+                    mma_ts(on, tmem + P::O0, tmem + P::S0 + (j & 1) * P::SREG + k * 32 + ks * 8, b, ID_O, acc);
+                    acc = 1;
+                }
+            tc_commit_if(on, smem_u32(&sm.ofull));
+            tc_commit_if(on, smem_u32(&sm.vfree[st]));
+        }
+        // tensor memory is given back only when no product is under way
+        tc_commit_if(on, smem_u32(&sm.done));
+        for (uint32_t i = 0; i < SPINS && !mbar_try_wait(smem_u32(&sm.done), 0); i++) {}
+    } else if (warp == 2) {
+        // ---- values that not every row sees
+        for (int j = 0; j < n_tiles && !gave_up(); j++) {
+            const int st = j % STAGES, key0 = tile_key(j);
+            wait(&sm.vfull[st], (j / STAGES) & 1);
+            if (edge_tile(key0)) {
+                unsigned long long odd = 0;
+                for (int r = lane; r < KT; r += 32) {
+                    const int k = key0 + r;
+                    const bool some = k <= p_max && (a.window <= 0 || k > p_min - a.window || k < a.first);
+                    const bool every = k <= p_min && (a.window <= 0 || k > p_max - a.window || k < a.first);
+                    bool bad = false;
+                    if (some && !every) {
+                        for (int c = 0; c < HD / 8; c++) {
+                            const uint4 x = *(const uint4*)(sm.v[st] + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                if (KIND == KIND_F16) bad = bad || (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
+                                else bad = bad || (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
+                            }
+                        }
+                    }
+                    if (bad) odd |= 1ull << r;
+                    if (bad || !some)
+                        for (int c = 0; c < HD / 8; c++) *(uint4*)(sm.v[st] + (c >> 3) * (KT * 128) + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                }
+                uint32_t half[2] = {(uint32_t)odd, (uint32_t)(odd >> 32)};
+                half[0] = __reduce_or_sync(0xffffffffu, half[0]);
+                half[1] = __reduce_or_sync(0xffffffffu, half[1]);
+                if (lane == 0) sm.odd[st] = half[0] | (unsigned long long)half[1] << 32;
+                fence_proxy_async();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.vready[st]));
+        }
+    } else if (warp >= 4) {
+        // ---- softmax: thread = (row r of the 128, half w of the keys and of the output's dims)
+        const int w = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int row = row0 + r / a.group, h = kvh * a.group + r % a.group;
+        const bool on = r < a.rq * a.group && row <= row1;
+        const int p = on ? base + row : -1;
+        auto both = [&] { asm volatile("bar.sync 1, 256;" ::: "memory"); };    // the softmax warps
+        auto any_of = [&](bool x) {
+            uint32_t r;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                         : "=r"(r) : "r"((uint32_t)x) : "memory");
+            return r != 0;
+        };
+        float qs = 1.0f;
+        {
+            // q's half into tensor memory, scaled, part by part
+            const float* qr = a.q + ((size_t)s * a.rows + row) * a.q_ld + (size_t)h * HD + w * HALF;
+            const float sl = a.scale * LOG2E;
+            float x[HALF];
+            float top = 0.0f;
+#pragma unroll
+            for (int d = 0; d < HALF; d += 4) {
+                const float4 y = on ? *(const float4*)(qr + d) : make_float4(0, 0, 0, 0);
+                x[d] = y.x * sl; x[d + 1] = y.y * sl; x[d + 2] = y.z * sl; x[d + 3] = y.w * sl;
+#pragma unroll
+                for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(x[d + i]));
+            }
+            if (KIND == KIND_F16) {
+                sm.top[1][w][r] = top;
+                both();
+                top = fmaxf(top, sm.top[1][1 - w][r]);
+                int ex = top > 0.0f && top < INFINITY ? 13 - (int)((__float_as_uint(top) >> 23) & 255) + 127 : 0;
+                ex = max(-100, min(100, ex));
+                const float f = __uint_as_float((uint32_t)(127 + ex) << 23);
+#pragma unroll
+                for (int d = 0; d < HALF; d++) x[d] *= f;
+                qs = __uint_as_float((uint32_t)(127 - ex) << 23);
+            }
+#pragma unroll
+            for (int k = 0; k < QP; k++)
+#pragma unroll
+                for (int c = 0; c < HALF / 2; c += 16) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) pk[i] = take_part<KIND>(x[2 * (c + i)], x[2 * (c + i) + 1]);
+                    tc_st16(tmem + lanes + P::Q0 + k * HALF + w * (HALF / 2) + c, pk);
+                }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.qfull));
+        }
+        float m = -INFINITY, l = 0.0f, c_prev = 0.0f, o[HALF];
+#pragma unroll
+        for (int d = 0; d < HALF; d++) o[d] = 0.0f;
+        // o = o c + O of tile j
+        auto fold = [&](int j, float c) {
+            wait(&sm.ofull, j & 1);
+            tc_fence_after();
+            float x[HALF];
+            tm_ld<HALF>(tmem + lanes + P::O0 + w * HALF, x);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.ofree));
+#pragma unroll
+            for (int d = 0; d < HALF; d++) o[d] = fmaf(o[d], c, x[d]);
+        };
+        bool pending = false;                                      // O of the last tile is not in o yet
+        for (int j = 0; j < n_tiles; j++) {                        // every warp goes through every tile: they meet at barriers
+            const int b = j & 1, key0 = tile_key(j) + w * 32;
+            wait(&sm.sfull[b], (j >> 1) & 1);
+            tc_fence_after();
+            float v[32];
+            tm_ld<32>(tmem + lanes + P::S0 + b * P::SREG + w * 32, v);
+            if (KIND == KIND_F16) {
+#pragma unroll
+                for (int i = 0; i < 32; i++) v[i] *= qs;
+            }
+            const bool edge = edge_tile(tile_key(j));
+            if (edge) {
+                const int up = p - key0, dn = a.window > 0 ? p - a.window - key0 : -1, fi = a.first - key0;
+#pragma unroll
+                for (int i = 0; i < 32; i++) v[i] = i <= up && (a.window <= 0 || i > dn || i < fi) ? v[i] : -INFINITY;
+            }
+            float top = v[0];
+#pragma unroll
+            for (int i = 1; i < 32; i++) top = fmaxf(top, v[i]);
+            sm.top[b][w][r] = top;
+            tc_fence_before();
+            both();                                                // both halves of S are in registers now, too
+            tc_fence_after();
+            const float m_new = fmaxf(fmaxf(m, top), sm.top[b][1 - w][r]);
+            const float c = m == -INFINITY ? 0.0f : pow2f(m - m_new), ms = m_new == -INFINITY ? 0.0f : m_new - SHIFT;
+            m = m_new;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                v[i] = pow2f(v[i] - ms);
+                sum[i & 3] += v[i];
+            }
+            l = fmaf(l, c, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+            unsigned long long odd = 0;
+            bool any_odd = false;
+            if (edge) {
+                wait(&sm.vready[j % STAGES], (j / STAGES) & 1);
+                odd = sm.odd[j % STAGES];
+                any_odd = any_of(odd != 0);
+                if (any_odd) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (odd >> (w * 32 + i) & 1) {
+                            const int k = key0 + i;
+                            sm.odd_w[w * 32 + i][r] = k <= p && (a.window <= 0 || k > p - a.window || k < a.first) ? v[i] : -1.0f;
+                        }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < QP; k++) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) pk[i] = take_part<KIND>(v[2 * i], v[2 * i + 1]);
+                tc_st16(tmem + lanes + P::S0 + b * P::SREG + k * 32 + w * 16, pk);
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.pfull[b]));
+            if (pending) fold(j - 1, c_prev);
+            pending = true;
+            c_prev = c;
+            if (any_odd) {
+                // rare: this tile's O at once, then the values that are not finite, for the rows that see them
+                fold(j, c);
+                pending = false;
+                both();
+                for (int i = 0; i < KT; i++) {
+                    if (!(odd >> i & 1)) continue;
+                    const float wt = sm.odd_w[i][r];
+                    if (wt < 0.0f) continue;
+                    const int k = tile_key(j) + i, pg = min(max(a.table[(size_t)s * a.max_pages + (k >> a.log_page)], 0), a.n_pages - 1);
+                    const uint16_t* vr = (const uint16_t*)a.data + ((((size_t)2 * pg + 1) * a.n_kv + kvh) * a.page + (k & (a.page - 1))) * HD + w * HALF;
+#pragma unroll
+                    for (int d = 0; d < HALF; d++) o[d] = fmaf(wt, KIND == KIND_F16 ? fk_h2f(vr[d]) : __uint_as_float((uint32_t)vr[d] << 16), o[d]);
+                }
+                both();
+            }
+        }
+        if (pending) fold(n_tiles - 1, c_prev);
+        // ---- the two halves' denominators, the sink, the output
+        if (n_tiles > 0) {
+            both();
+            sm.top[0][w][r] = l;
+            both();
+            l += sm.top[0][1 - w][r];
+            if (on) {
+                if (a.sinks) l += m == -INFINITY ? 1.0f : pow2f(a.sinks[h] * LOG2E - m + SHIFT);
+                const float inv = 1.0f / l;
+                float* dst = a.out + (((size_t)s * a.rows + row) * a.n_heads + h) * HD + w * HALF;
+#pragma unroll
+                for (int d = 0; d < HALF; d += 4) *(float4*)(dst + d) = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int KIND, int HD> int launch_prompt(fk_ctx* ctx, cudaStream_t st, const PromptArgs& a, unsigned grid) {
+    auto kern = attn_prompt_kernel<KIND, HD>;
+    const size_t smem = sizeof(PromptSmem<KIND, HD>) + 1024;
+    static thread_local bool ready[64] = {};
+    if (!ready[ctx->device & 63]) {
+        FK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), FK_KERNEL);
+        FK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared), FK_KERNEL);
+        ready[ctx->device & 63] = true;
+    }
+    FK_CUDA(launch(kern, dim3(grid), dim3(THREADS), smem, st, a), FK_LAUNCH);
+    return FK_OK;
+}
+
+}  // namespace
+
+// Whether this kernel takes the call, else attn_paged_kernel does.
+bool fk_attn_prompt_takes(fk_ctx* ctx, const fk_pages* p, int rows, int n_heads) {
+    const int group = n_heads / p->n_kv;
+    if (p->kind == KIND_F32 || (p->head_dim != 64 && p->head_dim != 128) || group > 128) return false;
+    if ((long long)p->n_pages * 2 * p->n_kv * p->page > 0x7fffffffLL) return false;      // a token's row number is 32 bits
+    return (long long)rows * group >= 128;
+}
+
+int fk_attn_prompt_launch(fk_ctx* ctx, cudaStream_t st, const fk_pages* p, int layer, const float* q, int q_ld, int rows, const int* n_new, int n_heads,
+                          float scale, int window, int first, const float* sinks, float* out) {
+    PromptArgs a{};
+    char* data = (char*)p->data_dev + (size_t)layer * page_bytes(p) * p->n_pages;
+    const int rc = fk_make_map_2d(&a.map, 1, data, p->head_dim, (uint64_t)p->n_pages * 2 * p->n_kv * p->page, 64, p->page < KT ? p->page : KT, 3);
+    if (rc != FK_OK) return rc;
+    a.data = data;
+    a.table = p->table_dev;
+    a.lens = p->lens_dev;
+    a.n_new = n_new;
+    a.q = q;
+    a.sinks = sinks;
+    a.out = out;
+    a.err = ctx->err_flag;
+    a.scale = scale;
+    a.q_ld = q_ld;
+    a.rows = rows;
+    a.n_seqs = p->n_seqs;
+    a.n_heads = n_heads;
+    a.n_kv = p->n_kv;
+    a.group = n_heads / p->n_kv;
+    a.page = p->page;
+    a.log_page = p->page == 16 ? 4 : p->page == 32 ? 5 : p->page == 64 ? 6 : 7;
+    a.n_pages = p->n_pages;
+    a.max_pages = p->max_pages;
+    a.window = window;
+    a.first = first;
+    a.rq = 128 / a.group;
+    a.n_rb = (rows + a.rq - 1) / a.rq;
+    const long long grid = (long long)a.n_rb * a.n_seqs * a.n_kv;
+    if (grid > 0x7fffffffLL) return fk_fail(FK_UNSUPPORTED, "attention_paged: %d rows of %d sequences", rows, p->n_seqs);
+    if (p->kind == KIND_F16) return p->head_dim == 64 ? launch_prompt<KIND_F16, 64>(ctx, st, a, (unsigned)grid) : launch_prompt<KIND_F16, 128>(ctx, st, a, (unsigned)grid);
+    return p->head_dim == 64 ? launch_prompt<FK_BF16, 64>(ctx, st, a, (unsigned)grid) : launch_prompt<FK_BF16, 128>(ctx, st, a, (unsigned)grid);
+}

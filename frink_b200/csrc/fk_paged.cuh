@@ -2,6 +2,11 @@
 #pragma once
 #include "fk_common.cuh"
 
+// attention of many rows on the tensor cores' tcgen05 form (fk_attn_prompt.cu)
+bool fk_attn_prompt_takes(fk_ctx* ctx, const fk_pages* p, int rows, int n_heads);
+int fk_attn_prompt_launch(fk_ctx* ctx, cudaStream_t st, const fk_pages* p, int layer, const float* q, int q_ld, int rows, const int* n_new, int n_heads,
+                          float scale, int window, int first, const float* sinks, float* out);
+
 namespace fk_paged {
 
 constexpr int MAX_SEQS = 4096, MAX_LIST = 64;

@@ -442,3 +442,90 @@ def test_a_server_round():
         feed(pg.seq(s), s, 9)
     feed(pg.seq(2), 2, 20)
     assert device.device_error() == 0
+
+
+# ---- prompts: 128 (row, head) pairs and more of a KV head go to the tensor cores' tcgen05 kernel
+def attend_fast(lens, counts, rows, heads, n_kv, hd, page, dtype, window=0, first=0, sinks=False, seed=0, bad=()):
+    """`attend` with the 64-bit restatement as matrix products on the GPU (long prompts); bad: (sequence, key, value) to plant."""
+    from frink_b200 import device
+    pg, data = cache(lens, counts, n_kv, hd, page, dtype, seed)
+    S, grp = len(lens), heads // n_kv
+    for s, j, x in bad:
+        pg.data[0, pg.table[s, j // page].long(), :, :, j % page] = x
+    q = queries(S * rows, heads * hd, seed).cuda()
+    sk = torch.randn(heads, generator=torch.Generator().manual_seed(seed)).cuda() if sinks else None
+    out = torch.full((S * rows, heads * hd), 7.0, device="cuda")
+    device.attention_paged(q, pg, 0, heads, n_new=torch.tensor(counts, dtype=torch.int32).cuda(), window=window, first=first, sinks=sk, out=out)
+    assert device.device_error() == 0
+    worst = 0.0
+    for s in range(S):
+        n, T = counts[s], lens[s] + counts[s]
+        got = out[s * rows:(s + 1) * rows].view(rows, heads, hd)
+        assert (got[n:] == 7.0).all()
+        if n == 0:
+            continue
+        kv = pg.data[0, pg.table[s, :-(-T // page)].long()].permute(1, 2, 0, 3, 4).reshape(2, n_kv, -1, hd)[:, :, :T].double()
+        p, j = torch.arange(lens[s], T, device="cuda")[:, None], torch.arange(T, device="cuda")[None]
+        hide = (j > p) | ((j <= p - window) & (j >= first) if window else torch.zeros_like(j > p))
+        clean = torch.ones(n, dtype=torch.bool, device="cuda")
+        for ss, jj, _ in bad:
+            if ss == s and jj < T:
+                clean &= hide[:, jj]
+                kv[:, :, jj] = 0
+        for h in range(heads):
+            x = q[s * rows:s * rows + n, h * hd:(h + 1) * hd].double() @ kv[0, h // grp].T * hd ** -0.5
+            x = x.masked_fill(hide, float("-inf"))
+            m = x.amax(1, keepdim=True)
+            if sinks:
+                m = m.clamp(min=float(sk[h]))
+            w = (x - m).exp()
+            want = w @ kv[1, h // grp] / (w.sum(1, keepdim=True) + ((float(sk[h]) - m).exp() if sinks else 0.0))
+            worst = max(worst, rel_l2(got[:n, h][clean].cpu().numpy(), want[clean].cpu().numpy()))
+            assert not torch.isfinite(got[:n, h][~clean]).any()
+    assert worst <= TOL
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,n_kv,hd", [(24, 8, 128), (64, 8, 64), (8, 8, 128), (16, 1, 64), (130, 1, 64), (128, 1, 128)])
+@pytest.mark.parametrize("page,rows,lens,counts", [(16, 300, [0], [300]), (64, 257, [700, 3], [257, 100]), (32, 129, [0, 1000, 64], [0, 129, 128]), (128, 200, [129], [200])])
+def test_prompt(dtype, heads, n_kv, hd, page, rows, lens, counts):
+    attend_fast(lens, counts, rows, heads, n_kv, hd, page, TYPES[dtype], seed=rows)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("window,first,sinks", [(1, 0, True), (100, 4, False), (64, 64, True), (300, 70, False), (128, 1000, True), (5000, 3, False)])
+def test_prompt_windows(dtype, window, first, sinks):
+    attend_fast([900, 0], [400, 333], 400, 16, 2, 64, 32, TYPES[dtype], window=window, first=first, sinks=sinks, seed=window)
+    attend_fast([900, 0], [150, 133], 150, 6, 2, 128, 16, TYPES[dtype], window=window, first=first, sinks=sinks, seed=window)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("x", [float("nan"), float("inf")])
+def test_prompt_values_behind_a_mask_do_not_matter(dtype, x):
+    """A bad token poisons the rows that see it and no other: in the middle of a causal tile, where a window leaves it behind,
+    several at once."""
+    attend_fast([100], [300], 300, 16, 2, 64, 16, TYPES[dtype], seed=3, bad=[(0, 390, x)])
+    attend_fast([100], [300], 300, 24, 8, 128, 16, TYPES[dtype], seed=4, bad=[(0, 150, x), (0, 152, x), (0, 399, x)])
+    attend_fast([500], [300], 300, 16, 2, 64, 64, TYPES[dtype], window=70, first=3, seed=5, bad=[(0, 3, x), (0, 440, x), (0, 600, x), (0, 799, x)])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_a_long_prompt_keeps_its_precision_and_repeats(dtype):
+    a = attend_fast([20000], [256], 256, 4, 1, 128, 128, TYPES[dtype], seed=6)
+    assert torch.equal(a, attend_fast([20000], [256], 256, 4, 1, 128, 128, TYPES[dtype], seed=6))
+
+
+def test_rows_in_any_stride_and_a_wrong_page_of_a_prompt():
+    from frink_b200 import device
+    pg, data = cache([0], [200], 2, 64, 16, torch.bfloat16, seed=9, stale=0.0)
+    wide = torch.randn((200, 16 * 64 + 32), generator=torch.Generator().manual_seed(1)).cuda()
+    q = wide[:, 16:16 + 16 * 64]
+    assert torch.equal(device.attention_paged(q, pg, 0, 16), device.attention_paged(q.contiguous(), pg, 0, 16))
+    pg.table[0, 5] = 1 << 20
+    out = device.attention_paged(q, pg, 0, 16)
+    assert device.device_error() == 97 and torch.isfinite(out).all()
+    pg.table[0, 5], pg.lens[0] = 0, 100
+    out.fill_(7.0)
+    device.attention_paged(q, pg, 0, 16, out=out)
+    assert device.device_error() == 95 and (out == 7.0).all()
