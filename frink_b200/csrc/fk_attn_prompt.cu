@@ -4,19 +4,22 @@
 // A CTA takes 128 (row, query head) pairs of one KV head -- 128 / group consecutive rows, so a short prompt still fills the
 // tile -- and walks the visible keys in tiles of 64:
 //
-//   S = q K^T          A = q's parts in tensor memory, B = a tile of K in shared memory, S in tensor memory (two buffers)
-//   w = 2^(S - m)      a thread per (row, half of the tile's keys); its parts go back over S as the next product's A operand
+//   S = q K^T          A = q's parts in tensor memory, B = a tile of K in shared memory, S in tensor memory (two or three buffers)
+//   w = 2^(S - m)      a thread per row; its parts go back over S as the next product's A operand
 //   O = w V            A = w's parts, B = the tile of V as it lies in memory (the major axis is its dims)
 //   o = o c + O        in registers: the running output is rescaled and added to in f32, rounded, because a sum that stayed
 //                      in the tensor core over a long prompt would be cut off thousands of times
 //
 // bf16 takes three parts of q and w, f16 two (fk_attn_paged.cu says why that is f32 precision), so a product is three (two)
 // products: the bound is the tensor cores' rate by that factor.  Per tile of 64 keys and 128 dims that is 1536 (1024) cycles of
-// MMA against some 900 issue slots of each scheduler's two softmax warps, which run beside it on the other buffer.
+// MMA against 512 of exponentials and some 700 issue slots a scheduler for the parts and the running output.
 //
-// Warps: 0 loads tiles (a lane per page piece, TMA with 128-byte swizzle), 1 issues the products, 2 looks over the values of
-// tiles that not every row sees, 4 to 11 are the softmax.  A value that no row sees is zeroed in shared memory (stale memory may
-// hold NaN); one that some rows see and that is not finite is zeroed too and added in plain f32 for the rows that see it.
+// Warps 0 to 3 and 4 to 7 are two softmax groups that take turns: a thread has a row and all 64 keys of its group's tile, in two
+// halves, so nothing is exchanged inside a group, and between them only the row's maximum passes -- early in a tile, so that one
+// group's exponentials run beside the other's.  8 to 15 keep the running output, a thread per row and half of the dims.  16 loads
+// tiles (a lane per page piece, TMA with 128-byte swizzle), 17 issues the products, 18 looks over the values of tiles that not
+// every row sees: a value that no row sees is zeroed in shared memory (stale memory may hold NaN); one that some rows see and
+// that is not finite is zeroed too and added in plain f32 for the rows that see it.
 #include "fk_paged.cuh"
 #include "fk_tc.cuh"
 
@@ -28,7 +31,8 @@ using namespace fk_tc;
 namespace {
 
 constexpr int KT = 64;                         // keys of a tile
-constexpr int THREADS = 384;
+constexpr int THREADS = 608;                    // 19 warps: 104 registers a thread
+constexpr int LOADER = 16, ISSUER = 17, LOOKER = 18;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr uint32_t SPINS = 1u << 20;           // polls of a wait before it gives up
 
@@ -47,29 +51,42 @@ template <int KIND, int HD> struct Plan {
     static constexpr int QP = KIND == KIND_F16 ? 2 : 3;            // parts of q and of the weights
     static constexpr int TILE = KT * HD * 2;                       // bytes of a tile of K or V
     static constexpr int STAGES = HD == 64 ? 6 : 4;
-    static constexpr int SREG = QP == 3 ? 96 : 64;                 // tensor memory columns of S (64), then of w's parts (32 each)
+    // Tensor memory columns of a tile: S's 64 behind LEAD free ones; the parts of w's first half of the keys take the free ones
+    // and S's first half, those of its second half what follows, so that S is never overwritten before it is read.
+    static constexpr int SREG = QP * 32, LEAD = SREG - 64;
     static constexpr int Q0 = 0, O0 = QP * HD / 2, S0 = O0 + HD;
-    static_assert(S0 + 2 * SREG <= 512, "tensor memory");
+    // buffers of S: with three a product need not wait for the one whose operand it overwrites
+    static constexpr int NS = S0 + 3 * SREG <= 512 ? 3 : 2;
+    static_assert(S0 + NS * SREG <= 512, "tensor memory");
 };
 
 template <int KIND, int HD> struct PromptSmem {
     using P = Plan<KIND, HD>;
     unsigned char k[P::STAGES][P::TILE];
     unsigned char v[P::STAGES][P::TILE];
-    float odd_w[KT][128];                      // weights of a tile's values that are not finite, by row (-1: the row does not see it)
-    float top[2][2][128];                      // a row's maximum over each half of the tile's keys, two tiles' worth
-    unsigned long long odd[P::STAGES];         // which of a tile's values are not finite
+    float odd_w[2][KT][128];                   // per softmax group: weights of a tile's values that are not finite, by row (-1: not seen)
+    float top[2][128];                         // a row's maximum after the tile (tile number mod 2); before that, of q's halves
+    float corr[4][128];                        // what the running output is multiplied with at the tile (mod 4)
+    float fin[2][2][128];                      // per softmax group: denominator and the maximum it refers to
+    unsigned long long odd_of[4];              // which of the tile's values are not finite (mod 4)
+    unsigned long long odd[P::STAGES];         // the same, where the values lie
     unsigned long long kfull[P::STAGES], kfree[P::STAGES], vfull[P::STAGES], vfree[P::STAGES], vready[P::STAGES];
-    unsigned long long sfull[2], pfull[2], ofull, ofree, qfull, done;
+    unsigned long long sfull[P::NS], pfull[P::NS], mfull[2][4], oddfree[2], ofull, ofree, qfull, done;
     uint32_t tmem;
     int abort;
 };
 
-// d (+)= a b, issued by the lane whose `on` is set: A in tensor memory
-__device__ __forceinline__ void mma_ts(uint32_t on, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %9, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0), "r"(on) : "memory");
+// d (+)= a b: A in tensor memory.  Issued by one lane, inside `if (elected())`: the compiler then knows that one thread runs
+// and keeps the operands in uniform registers.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
+}
+__device__ __forceinline__ bool elected() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 // f32 sums of f16 or bf16 products; b_mn: B's major axis is N
 __host__ __device__ constexpr uint32_t idesc_of(int kind, int m, int n, int b_mn) {
@@ -96,9 +113,10 @@ template <int KIND> __device__ __forceinline__ uint32_t take_part(float& lo, flo
     return r;
 }
 template <int N> __device__ __forceinline__ void tm_ld(uint32_t addr, float* v) {
-    static_assert(N == 32 || N == 64, "");
+    static_assert(N == 16 || N % 32 == 0, "");
+    if (N == 16) tc_ld16(addr, reinterpret_cast<uint32_t*>(v));
 #pragma unroll
-    for (int i = 0; i < N; i += 32) tc_ld32(addr + i, reinterpret_cast<uint32_t*>(v) + i);
+    for (int i = 0; i + 32 <= N; i += 32) tc_ld32(addr + i, reinterpret_cast<uint32_t*>(v) + i);
     tc_wait_ld();
     tc_ld_fence<N>(reinterpret_cast<uint32_t*>(v));
 }
@@ -106,11 +124,11 @@ template <int N> __device__ __forceinline__ void tm_ld(uint32_t addr, float* v) 
 template <int KIND, int HD>
 __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_constant__ PromptArgs a) {
     using P = Plan<KIND, HD>;
-    constexpr int QP = P::QP, STAGES = P::STAGES, HALF = HD / 2;
+    constexpr int QP = P::QP, STAGES = P::STAGES, NS = P::NS, HALF = HD / 2;
     constexpr float SHIFT = KIND == KIND_F16 ? 14.0f : 0.0f;
     extern __shared__ unsigned char smem_raw[];
     PromptSmem<KIND, HD>& sm = *reinterpret_cast<PromptSmem<KIND, HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     if (tid == 0) {
         for (int i = 0; i < STAGES; i++) {
             mbar_init(smem_u32(&sm.kfull[i]), 1);
@@ -119,10 +137,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
             mbar_init(smem_u32(&sm.vfree[i]), 1);
             mbar_init(smem_u32(&sm.vready[i]), 1);
         }
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < NS; i++) {
             mbar_init(smem_u32(&sm.sfull[i]), 1);
-            mbar_init(smem_u32(&sm.pfull[i]), 8);
+            mbar_init(smem_u32(&sm.pfull[i]), 4);
         }
+        for (int i = 0; i < 8; i++) mbar_init(smem_u32(&sm.mfull[i >> 2][i & 3]), 1);
+        for (int i = 0; i < 2; i++) mbar_init(smem_u32(&sm.oddfree[i]), 8);
         mbar_init(smem_u32(&sm.ofull), 1);
         mbar_init(smem_u32(&sm.ofree), 8);
         mbar_init(smem_u32(&sm.qfull), 8);
@@ -133,22 +153,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
     // Tensor memory is taken after the previous kernel is done with its own and before the next one may start: neither can
     // then hold what the other waits for.
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp == 1) {
+    if (warp == ISSUER) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sm.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // a wait gives up after SPINS polls, or at once when another one of the CTA has given up; the CTA then runs to its end
     auto wait = [&](unsigned long long* bar, uint32_t parity) {
         const uint32_t b = smem_u32(bar);
+        // the warp goes on together: what it does next stays uniform for the compiler, and operands in uniform registers
         for (uint32_t i = 0; i < SPINS; i++) {
-            if (mbar_try_wait(b, parity)) return;
-            if (*(volatile int*)&sm.abort) return;
+            if (__all_sync(0xffffffffu, mbar_try_wait(b, parity))) return;
+            if (__any_sync(0xffffffffu, *(volatile int*)&sm.abort)) return;
         }
         *(volatile int*)&sm.abort = 1;
         fk_raise(a.err, 63);
@@ -168,12 +189,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
     const int hi = base + row1 + 1, lo = a.window > 0 ? max(0, base + row0 + 1 - a.window) : 0;
     int b0 = lo / KT, na = (min(a.first, lo) + KT - 1) / KT;
     if (na >= b0) na = b0 = 0;
-    const int n_tiles = row1 < row0 ? 0 : na + (hi + KT - 1) / KT - b0;
+    const int n_tiles = __shfl_sync(0xffffffffu, row1 < row0 ? 0 : na + (hi + KT - 1) / KT - b0, 0);
     const int p_min = base + row0, p_max = hi - 1;
     auto tile_key = [&](int j) { return (j < na ? j : j - na + b0) * KT; };
     auto edge_tile = [&](int key0) { return key0 + KT - 1 > p_min || (a.window > 0 && key0 <= p_max - a.window && key0 + KT - 1 >= a.first); };
 
-    if (warp == 0) {
+    if (warp == LOADER) {
         // ---- loads: lane u takes the u-th page piece of a tile
         const int piece = min(a.page, KT), n_pc = KT / piece;
         auto page_of = [&](int j) {
@@ -218,26 +239,26 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
             for (uint32_t i = 0; i < SPINS && !mbar_try_wait(smem_u32(&sm.kfull[j % STAGES]), par); i++) {}
             for (uint32_t i = 0; i < SPINS && !mbar_try_wait(smem_u32(&sm.vfull[j % STAGES]), par); i++) {}
         }
-    } else if (warp == 1) {
+    } else if (warp == ISSUER) {
         // ---- products
-        const uint32_t on = lane == 0;
         constexpr uint32_t ID_S = idesc_of(KIND, 128, KT, 0), ID_O = idesc_of(KIND, 128, HD, 1);
+        const uint64_t k_desc = umma_desc(smem_u32(sm.k[0])), v_desc = umma_desc_of(smem_u32(sm.v[0]), KT * 128, 1024, 2);
         auto scores = [&](int j) {
             const int st = j % STAGES;
             wait(&sm.kfull[st], (j / STAGES) & 1);
             tc_fence_after();
-            const uint32_t d = tmem + P::S0 + (j & 1) * P::SREG;
-            uint32_t acc = 0;
+            const uint32_t d = tmem + P::S0 + (j % NS) * P::SREG + P::LEAD;
+            const uint64_t b = k_desc + (uint32_t)(st * (P::TILE >> 4));
+            if (elected()) {
 #pragma unroll
-            for (int k = QP - 1; k >= 0; k--)                      // the small parts first
+                for (int k = QP - 1; k >= 0; k--)                  // the small parts first
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ks++) {
-                    const uint64_t b = umma_desc(smem_u32(sm.k[st]) + (ks >> 2) * (KT * 128) + (ks & 3) * 32);
-                    mma_ts(on, d, tmem + P::Q0 + k * HALF + ks * 8, b, ID_S, acc);
-                    acc = 1;
-                }
-            tc_commit_if(on, smem_u32(&sm.sfull[j & 1]));
-            tc_commit_if(on, smem_u32(&sm.kfree[st]));
+                    for (int ks = 0; ks < HD / 16; ks++)
+                        mma_ts(d, tmem + P::Q0 + k * HALF + ks * 8, b + (((ks >> 2) * (KT * 128) + (ks & 3) * 32) >> 4), ID_S, k < QP - 1 || ks > 0);
+                tc_commit(smem_u32(&sm.sfull[j % NS]));
+                tc_commit(smem_u32(&sm.kfree[st]));
+            }
+            __syncwarp();
         };
         if (n_tiles > 0) {
             wait(&sm.qfull, 0);
@@ -246,32 +267,35 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         }
         for (int j = 0; j < n_tiles && !gave_up(); j++) {
             if (j + 1 < n_tiles) {
-                // S of tile j + 1 takes the place of w of tile j - 1: products with different results may pass one another
-                if (j > 0) wait(&sm.vfree[(j - 1) % STAGES], ((j - 1) / STAGES) & 1);
+                // S of tile j + 1 takes the place of w of tile j + 1 - NS: products with different results may pass one another
+                const int x = j + 1 - NS;
+                if (x >= 0) wait(&sm.vfree[x % STAGES], (x / STAGES) & 1);
                 scores(j + 1);
             }
             const int st = j % STAGES;
             wait(&sm.vready[st], (j / STAGES) & 1);
-            wait(&sm.pfull[j & 1], (j >> 1) & 1);
+            wait(&sm.pfull[j % NS], (j / NS) & 1);
             if (j > 0) wait(&sm.ofree, (j - 1) & 1);
             tc_fence_after();
-            uint32_t acc = 0;
+            const uint32_t w = tmem + P::S0 + (j % NS) * P::SREG;
+            const uint64_t b = v_desc + (uint32_t)(st * (P::TILE >> 4));
+            if (elected()) {
 #pragma unroll
-            for (int k = QP - 1; k >= 0; k--)
+                for (int k = QP - 1; k >= 0; k--)
 #pragma unroll
-                for (int ks = 0; ks < KT / 16; ks++) {
-                    // 16 keys of all dims: 64-dim halves KT * 128 bytes apart, groups of 8 keys 1024 bytes apart
-                    const uint64_t b = umma_desc_of(smem_u32(sm.v[st]) + ks * 2048, KT * 128, 1024, 2);
-                    mma_ts(on, tmem + P::O0, tmem + P::S0 + (j & 1) * P::SREG + k * 32 + ks * 8, b, ID_O, acc);
-                    acc = 1;
-                }
-            tc_commit_if(on, smem_u32(&sm.ofull));
-            tc_commit_if(on, smem_u32(&sm.vfree[st]));
+                    for (int ks = 0; ks < KT / 16; ks++)
+                        // 16 keys of all dims: 64-dim halves KT * 128 bytes apart, groups of 8 keys 1024 bytes apart
+                        mma_ts(tmem + P::O0, w + (ks >> 1) * (QP * 16) + k * 16 + (ks & 1) * 8, b + (ks * 2048 >> 4), ID_O, k < QP - 1 || ks > 0);
+                tc_commit(smem_u32(&sm.ofull));
+                tc_commit(smem_u32(&sm.vfree[st]));
+            }
+            __syncwarp();
         }
         // tensor memory is given back only when no product is under way
-        tc_commit_if(on, smem_u32(&sm.done));
-        for (uint32_t i = 0; i < SPINS && !mbar_try_wait(smem_u32(&sm.done), 0); i++) {}
-    } else if (warp == 2) {
+        if (elected()) tc_commit(smem_u32(&sm.done));
+        __syncwarp();
+        for (uint32_t i = 0; i < SPINS && !__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&sm.done), 0)); i++) {}
+    } else if (warp == LOOKER) {
         // ---- values that not every row sees
         for (int j = 0; j < n_tiles && !gave_up(); j++) {
             const int st = j % STAGES, key0 = tile_key(j);
@@ -307,162 +331,174 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sm.vready[st]));
         }
-    } else if (warp >= 4) {
-        // ---- softmax: thread = (row r of the 128, half w of the keys and of the output's dims)
-        const int w = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
+    } else {
+        const int w = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;       // softmax group, or half of the dims; row of the 128
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const int row = row0 + r / a.group, h = kvh * a.group + r % a.group;
         const bool on = r < a.rq * a.group && row <= row1;
         const int p = on ? base + row : -1;
-        auto both = [&] { asm volatile("bar.sync 1, 256;" ::: "memory"); };    // the softmax warps
-        auto any_of = [&](bool x) {
-            uint32_t r;
-            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                         : "=r"(r) : "r"((uint32_t)x) : "memory");
-            return r != 0;
-        };
-        float qs = 1.0f;
-        {
-            // q's half into tensor memory, scaled, part by part
-            const float* qr = a.q + ((size_t)s * a.rows + row) * a.q_ld + (size_t)h * HD + w * HALF;
-            const float sl = a.scale * LOG2E;
-            float x[HALF];
-            float top = 0.0f;
+        auto sees = [&](int k) { return k <= p && (a.window <= 0 || k > p - a.window || k < a.first); };
+        if (warp < 8) {
+            // ---- softmax.  First q: a group each of the halves of its dims into tensor memory, scaled, part by part
+            float qs = 1.0f;
+            {
+                const float* qr = a.q + ((size_t)s * a.rows + row) * a.q_ld + (size_t)h * HD + w * HALF;
+                const float sl = a.scale * LOG2E;
+                float x[HALF];
+                float top = 0.0f;
 #pragma unroll
-            for (int d = 0; d < HALF; d += 4) {
-                const float4 y = on ? *(const float4*)(qr + d) : make_float4(0, 0, 0, 0);
-                x[d] = y.x * sl; x[d + 1] = y.y * sl; x[d + 2] = y.z * sl; x[d + 3] = y.w * sl;
+                for (int d = 0; d < HALF; d += 4) {
+                    const float4 y = on ? *(const float4*)(qr + d) : make_float4(0, 0, 0, 0);
+                    x[d] = y.x * sl; x[d + 1] = y.y * sl; x[d + 2] = y.z * sl; x[d + 3] = y.w * sl;
 #pragma unroll
-                for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(x[d + i]));
-            }
-            if (KIND == KIND_F16) {
-                sm.top[1][w][r] = top;
-                both();
-                top = fmaxf(top, sm.top[1][1 - w][r]);
-                int ex = top > 0.0f && top < INFINITY ? 13 - (int)((__float_as_uint(top) >> 23) & 255) + 127 : 0;
-                ex = max(-100, min(100, ex));
-                const float f = __uint_as_float((uint32_t)(127 + ex) << 23);
-#pragma unroll
-                for (int d = 0; d < HALF; d++) x[d] *= f;
-                qs = __uint_as_float((uint32_t)(127 - ex) << 23);
-            }
-#pragma unroll
-            for (int k = 0; k < QP; k++)
-#pragma unroll
-                for (int c = 0; c < HALF / 2; c += 16) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int i = 0; i < 16; i++) pk[i] = take_part<KIND>(x[2 * (c + i)], x[2 * (c + i) + 1]);
-                    tc_st16(tmem + lanes + P::Q0 + k * HALF + w * (HALF / 2) + c, pk);
+                    for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(x[d + i]));
                 }
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sm.qfull));
-        }
-        float m = -INFINITY, l = 0.0f, c_prev = 0.0f, o[HALF];
+                if (KIND == KIND_F16) {
+                    sm.top[w][r] = top;
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    top = fmaxf(top, sm.top[1 - w][r]);
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    int ex = top > 0.0f && top < INFINITY ? 13 - (int)((__float_as_uint(top) >> 23) & 255) + 127 : 0;
+                    ex = max(-100, min(100, ex));
+                    const float f = __uint_as_float((uint32_t)(127 + ex) << 23);
 #pragma unroll
-        for (int d = 0; d < HALF; d++) o[d] = 0.0f;
-        // o = o c + O of tile j
-        auto fold = [&](int j, float c) {
-            wait(&sm.ofull, j & 1);
-            tc_fence_after();
-            float x[HALF];
-            tm_ld<HALF>(tmem + lanes + P::O0 + w * HALF, x);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sm.ofree));
-#pragma unroll
-            for (int d = 0; d < HALF; d++) o[d] = fmaf(o[d], c, x[d]);
-        };
-        bool pending = false;                                      // O of the last tile is not in o yet
-        for (int j = 0; j < n_tiles; j++) {                        // every warp goes through every tile: they meet at barriers
-            const int b = j & 1, key0 = tile_key(j) + w * 32;
-            wait(&sm.sfull[b], (j >> 1) & 1);
-            tc_fence_after();
-            float v[32];
-            tm_ld<32>(tmem + lanes + P::S0 + b * P::SREG + w * 32, v);
-            if (KIND == KIND_F16) {
-#pragma unroll
-                for (int i = 0; i < 32; i++) v[i] *= qs;
-            }
-            const bool edge = edge_tile(tile_key(j));
-            if (edge) {
-                const int up = p - key0, dn = a.window > 0 ? p - a.window - key0 : -1, fi = a.first - key0;
-#pragma unroll
-                for (int i = 0; i < 32; i++) v[i] = i <= up && (a.window <= 0 || i > dn || i < fi) ? v[i] : -INFINITY;
-            }
-            float top = v[0];
-#pragma unroll
-            for (int i = 1; i < 32; i++) top = fmaxf(top, v[i]);
-            sm.top[b][w][r] = top;
-            tc_fence_before();
-            both();                                                // both halves of S are in registers now, too
-            tc_fence_after();
-            const float m_new = fmaxf(fmaxf(m, top), sm.top[b][1 - w][r]);
-            const float c = m == -INFINITY ? 0.0f : pow2f(m - m_new), ms = m_new == -INFINITY ? 0.0f : m_new - SHIFT;
-            m = m_new;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 32; i++) {
-                v[i] = pow2f(v[i] - ms);
-                sum[i & 3] += v[i];
-            }
-            l = fmaf(l, c, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-            unsigned long long odd = 0;
-            bool any_odd = false;
-            if (edge) {
-                wait(&sm.vready[j % STAGES], (j / STAGES) & 1);
-                odd = sm.odd[j % STAGES];
-                any_odd = any_of(odd != 0);
-                if (any_odd) {
-#pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (odd >> (w * 32 + i) & 1) {
-                            const int k = key0 + i;
-                            sm.odd_w[w * 32 + i][r] = k <= p && (a.window <= 0 || k > p - a.window || k < a.first) ? v[i] : -1.0f;
-                        }
+                    for (int d = 0; d < HALF; d++) x[d] *= f;
+                    qs = __uint_as_float((uint32_t)(127 - ex) << 23);
                 }
+#pragma unroll
+                for (int k = 0; k < QP; k++)
+#pragma unroll
+                    for (int c = 0; c < HALF / 2; c += 16) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) pk[i] = take_part<KIND>(x[2 * (c + i)], x[2 * (c + i) + 1]);
+                        tc_st16(tmem + lanes + P::Q0 + k * HALF + w * (HALF / 2) + c, pk);
+                    }
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sm.qfull));
             }
+            float m = -INFINITY, l = 0.0f;                         // the denominator of this group's tiles, relative to m
+            int odds = 0;
+            for (int j = w; j < n_tiles; j += 2) {
+                const int key0 = tile_key(j);
+                wait(&sm.sfull[j % NS], (j / NS) & 1);
+                tc_fence_after();
+                const uint32_t at = tmem + lanes + P::S0 + (j % NS) * P::SREG;
+                const bool edge = edge_tile(key0);
+                const int up = p - key0, dn = a.window > 0 ? p - a.window - key0 : -1, fi = a.window > 0 ? a.first - key0 : 0;
+                auto scores = [&](int c, float* v) {               // half c of the row, what it does not see at -infinity
+                    tm_ld<32>(at + P::LEAD + c * 32, v);
+                    if (edge) {
 #pragma unroll
-            for (int k = 0; k < QP; k++) {
-                uint32_t pk[16];
+                        for (int i = 0; i < 32; i++) v[i] = 32 * c + i <= up && (32 * c + i > dn || 32 * c + i < fi) ? v[i] : -INFINITY;
+                    }
+                };
+                float v[32], top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 16; i++) pk[i] = take_part<KIND>(v[2 * i], v[2 * i + 1]);
-                tc_st16(tmem + lanes + P::S0 + b * P::SREG + k * 32 + w * 16, pk);
-            }
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sm.pfull[b]));
-            if (pending) fold(j - 1, c_prev);
-            pending = true;
-            c_prev = c;
-            if (any_odd) {
-                // rare: this tile's O at once, then the values that are not finite, for the rows that see them
-                fold(j, c);
-                pending = false;
-                both();
-                for (int i = 0; i < KT; i++) {
-                    if (!(odd >> i & 1)) continue;
-                    const float wt = sm.odd_w[i][r];
-                    if (wt < 0.0f) continue;
-                    const int k = tile_key(j) + i, pg = min(max(a.table[(size_t)s * a.max_pages + (k >> a.log_page)], 0), a.n_pages - 1);
-                    const uint16_t* vr = (const uint16_t*)a.data + ((((size_t)2 * pg + 1) * a.n_kv + kvh) * a.page + (k & (a.page - 1))) * HD + w * HALF;
+                for (int c = 1; c >= 0; c--) {
+                    scores(c, v);
 #pragma unroll
-                    for (int d = 0; d < HALF; d++) o[d] = fmaf(wt, KIND == KIND_F16 ? fk_h2f(vr[d]) : __uint_as_float((uint32_t)vr[d] << 16), o[d]);
+                    for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) top[k] = fmaxf(fmaxf(top[k], v[i + k]), v[i + 4 + k]);
                 }
-                both();
+                const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * qs;
+                // the row's maximum so far comes from the other group's warp of the same rows
+                float m_old = -INFINITY;
+                if (j > 0) {
+                    wait(&sm.mfull[1 - w][warp & 3], ((j - 1) >> 1) & 1);
+                    m_old = sm.top[1 - w][r];
+                }
+                const float m_new = fmaxf(m_old, t), ms = m_new == -INFINITY ? 0.0f : m_new - SHIFT;
+                sm.top[w][r] = m_new;
+                sm.corr[j & 3][r] = m_old == -INFINITY ? 0.0f : pow2f(m_old - m_new);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sm.mfull[w][warp & 3]));
+                l *= m == -INFINITY ? 1.0f : pow2f(m - m_new);
+                m = m_new;
+                unsigned long long odd = 0;
+                if (edge) {
+                    wait(&sm.vready[j % STAGES], (j / STAGES) & 1);
+                    odd = __shfl_sync(0xffffffffu, sm.odd[j % STAGES], 0);
+                    if (odd) {                                     // rare
+                        if (odds > 0) wait(&sm.oddfree[w], (odds - 1) & 1);
+                        odds++;
+                    }
+                }
+                if (r == 0) sm.odd_of[j & 3] = odd;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    if (c) scores(c, v);                           // half 0 is still there
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        v[i] = pow2f(fmaf(v[i], qs, -ms));
+                        sum[i & 3] += v[i];
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    if (odd) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (odd >> (32 * c + i) & 1) sm.odd_w[w][32 * c + i][r] = sees(key0 + 32 * c + i) ? v[i] : -1.0f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < QP; k++) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) pk[i] = take_part<KIND>(v[2 * i], v[2 * i + 1]);
+                        tc_st16(at + c * (QP * 16) + k * 16, pk);
+                    }
+                }
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sm.pfull[j % NS]));
             }
-        }
-        if (pending) fold(n_tiles - 1, c_prev);
-        // ---- the two halves' denominators, the sink, the output
-        if (n_tiles > 0) {
-            both();
-            sm.top[0][w][r] = l;
-            both();
-            l += sm.top[0][1 - w][r];
-            if (on) {
+            sm.fin[w][0][r] = l;
+            sm.fin[w][1][r] = m;
+            asm volatile("bar.sync 2, 512;" ::: "memory");
+        } else {
+            // ---- the running output: o = o corr + O
+            float o[HALF];
+#pragma unroll
+            for (int d = 0; d < HALF; d++) o[d] = 0.0f;
+            for (int j = 0; j < n_tiles; j++) {
+                wait(&sm.ofull, j & 1);
+                tc_fence_after();
+                const float c = sm.corr[j & 3][r];
+                const unsigned long long odd = __shfl_sync(0xffffffffu, sm.odd_of[j & 3], 0);
+                constexpr int N = HD == 64 ? 32 : 16;
+#pragma unroll
+                for (int d0 = 0; d0 < HALF; d0 += N) {
+                    float x[N];
+                    tm_ld<N>(tmem + lanes + P::O0 + w * HALF + d0, x);
+#pragma unroll
+                    for (int d = 0; d < N; d++) o[d0 + d] = fmaf(o[d0 + d], c, x[d]);
+                }
+                if (odd) {                                         // rare: values that are not finite, for the rows that see them
+                    for (int i = 0; i < KT; i++) {
+                        if (!(odd >> i & 1)) continue;
+                        const float wt = sm.odd_w[j & 1][i][r];
+                        if (wt < 0.0f) continue;
+                        const int k = tile_key(j) + i, pg = min(max(a.table[(size_t)s * a.max_pages + (k >> a.log_page)], 0), a.n_pages - 1);
+                        const uint16_t* vr = (const uint16_t*)a.data + ((((size_t)2 * pg + 1) * a.n_kv + kvh) * a.page + (k & (a.page - 1))) * HD + w * HALF;
+#pragma unroll
+                        for (int d = 0; d < HALF; d++) o[d] = fmaf(wt, KIND == KIND_F16 ? fk_h2f(vr[d]) : __uint_as_float((uint32_t)vr[d] << 16), o[d]);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sm.oddfree[j & 1]));
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sm.ofree));
+            }
+            // the two groups' denominators, the sink, the output
+            asm volatile("bar.sync 2, 512;" ::: "memory");
+            if (on && n_tiles > 0) {
+                const float m0 = sm.fin[0][1][r], m1 = sm.fin[1][1][r], m = fmaxf(m0, m1);
+                float l = sm.fin[0][0][r] * (m0 == m ? 1.0f : pow2f(m0 - m)) + sm.fin[1][0][r] * (m1 == m ? 1.0f : pow2f(m1 - m));
                 if (a.sinks) l += m == -INFINITY ? 1.0f : pow2f(a.sinks[h] * LOG2E - m + SHIFT);
                 const float inv = 1.0f / l;
                 float* dst = a.out + (((size_t)s * a.rows + row) * a.n_heads + h) * HD + w * HALF;
@@ -473,7 +509,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == ISSUER) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
