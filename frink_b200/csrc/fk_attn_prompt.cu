@@ -17,9 +17,10 @@
 // Warps 0 to 3 and 4 to 7 are two softmax groups that take turns: a thread has a row and all 64 keys of its group's tile, in two
 // halves, so nothing is exchanged inside a group, and between them only the row's maximum passes -- early in a tile, so that one
 // group's exponentials run beside the other's.  8 to 15 keep the running output, a thread per row and half of the dims.  16 loads
-// tiles (a lane per page piece, TMA with 128-byte swizzle), 17 issues the products, 18 looks over the values of tiles that not
-// every row sees: a value that no row sees is zeroed in shared memory (stale memory may hold NaN); one that some rows see and
-// that is not finite is zeroed too and added in plain f32 for the rows that see it.
+// tiles (a lane per page piece, TMA with 128-byte swizzle).  17 issues the products for S and 19 those for O, so that scores are
+// made as soon as their buffer is free and not in turn with products that wait for weights.  18 looks over the values of tiles
+// that not every row sees: a value that no row sees is zeroed in shared memory (stale memory may hold NaN); one that some rows
+// see and that is not finite is zeroed too and added in plain f32 for the rows that see it.
 #include "fk_paged.cuh"
 #include "fk_tc.cuh"
 
@@ -31,8 +32,8 @@ using namespace fk_tc;
 namespace {
 
 constexpr int KT = 64;                         // keys of a tile
-constexpr int THREADS = 608;                    // 19 warps: 104 registers a thread
-constexpr int LOADER = 16, ISSUER = 17, LOOKER = 18;
+constexpr int THREADS = 640;
+constexpr int LOADER = 16, ISSUER_S = 17, LOOKER = 18, ISSUER_O = 19;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr uint32_t SPINS = 1u << 20;           // polls of a wait before it gives up
 
@@ -71,7 +72,7 @@ template <int KIND, int HD> struct PromptSmem {
     unsigned long long odd_of[4];              // which of the tile's values are not finite (mod 4)
     unsigned long long odd[P::STAGES];         // the same, where the values lie
     unsigned long long kfull[P::STAGES], kfree[P::STAGES], vfull[P::STAGES], vfree[P::STAGES], vready[P::STAGES];
-    unsigned long long sfull[P::NS], pfull[P::NS], mfull[2][4], oddfree[2], ofull, ofree, qfull, done;
+    unsigned long long sfull[P::NS], pfull[P::NS], mfull[2][4], oddfree[2], ofull, ofree, qfull, done[2];
     uint32_t tmem;
     int abort;
 };
@@ -146,14 +147,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         mbar_init(smem_u32(&sm.ofull), 1);
         mbar_init(smem_u32(&sm.ofree), 8);
         mbar_init(smem_u32(&sm.qfull), 8);
-        mbar_init(smem_u32(&sm.done), 1);
+        mbar_init(smem_u32(&sm.done[0]), 1);
+        mbar_init(smem_u32(&sm.done[1]), 1);
         sm.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // Tensor memory is taken after the previous kernel is done with its own and before the next one may start: neither can
     // then hold what the other waits for.
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp == ISSUER) {
+    if (warp == ISSUER_S) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -239,12 +241,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
             for (uint32_t i = 0; i < SPINS && !mbar_try_wait(smem_u32(&sm.kfull[j % STAGES]), par); i++) {}
             for (uint32_t i = 0; i < SPINS && !mbar_try_wait(smem_u32(&sm.vfull[j % STAGES]), par); i++) {}
         }
-    } else if (warp == ISSUER) {
-        // ---- products
-        constexpr uint32_t ID_S = idesc_of(KIND, 128, KT, 0), ID_O = idesc_of(KIND, 128, HD, 1);
-        const uint64_t k_desc = umma_desc(smem_u32(sm.k[0])), v_desc = umma_desc_of(smem_u32(sm.v[0]), KT * 128, 1024, 2);
-        auto scores = [&](int j) {
-            const int st = j % STAGES;
+    } else if (warp == ISSUER_S) {
+        // ---- S = q K^T
+        constexpr uint32_t ID_S = idesc_of(KIND, 128, KT, 0);
+        const uint64_t k_desc = umma_desc(smem_u32(sm.k[0]));
+        if (n_tiles > 0) wait(&sm.qfull, 0);
+        for (int j = 0; j < n_tiles && !gave_up(); j++) {
+            const int st = j % STAGES, x = j - NS;
+            // S takes the place of w of tile j - NS: products with different results may pass one another, so that one is waited for
+            if (x >= 0) wait(&sm.vfree[x % STAGES], (x / STAGES) & 1);
             wait(&sm.kfull[st], (j / STAGES) & 1);
             tc_fence_after();
             const uint32_t d = tmem + P::S0 + (j % NS) * P::SREG + P::LEAD;
@@ -259,23 +264,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
                 tc_commit(smem_u32(&sm.kfree[st]));
             }
             __syncwarp();
-        };
-        if (n_tiles > 0) {
-            wait(&sm.qfull, 0);
-            tc_fence_after();
-            scores(0);
         }
+        // tensor memory is given back only when no product is under way
+        if (elected()) tc_commit(smem_u32(&sm.done[0]));
+        __syncwarp();
+        for (uint32_t i = 0; i < SPINS && !__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&sm.done[0]), 0)); i++) {}
+    } else if (warp == ISSUER_O) {
+        // ---- O = w V
+        constexpr uint32_t ID_O = idesc_of(KIND, 128, HD, 1);
+        const uint64_t v_desc = umma_desc_of(smem_u32(sm.v[0]), KT * 128, 1024, 2);
         for (int j = 0; j < n_tiles && !gave_up(); j++) {
-            if (j + 1 < n_tiles) {
-                // S of tile j + 1 takes the place of w of tile j + 1 - NS: products with different results may pass one another
-                const int x = j + 1 - NS;
-                if (x >= 0) wait(&sm.vfree[x % STAGES], (x / STAGES) & 1);
-                scores(j + 1);
-            }
             const int st = j % STAGES;
             wait(&sm.vready[st], (j / STAGES) & 1);
-            wait(&sm.pfull[j % NS], (j / NS) & 1);
             if (j > 0) wait(&sm.ofree, (j - 1) & 1);
+            wait(&sm.pfull[j % NS], (j / NS) & 1);
             tc_fence_after();
             const uint32_t w = tmem + P::S0 + (j % NS) * P::SREG;
             const uint64_t b = v_desc + (uint32_t)(st * (P::TILE >> 4));
@@ -291,10 +293,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
             }
             __syncwarp();
         }
-        // tensor memory is given back only when no product is under way
-        if (elected()) tc_commit(smem_u32(&sm.done));
+        if (elected()) tc_commit(smem_u32(&sm.done[1]));
         __syncwarp();
-        for (uint32_t i = 0; i < SPINS && !__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&sm.done), 0)); i++) {}
+        for (uint32_t i = 0; i < SPINS && !__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&sm.done[1]), 0)); i++) {}
     } else if (warp == LOOKER) {
         // ---- values that not every row sees
         for (int j = 0; j < n_tiles && !gave_up(); j++) {
@@ -337,18 +338,28 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         const int row = row0 + r / a.group, h = kvh * a.group + r % a.group;
         const bool on = r < a.rq * a.group && row <= row1;
         const int p = on ? base + row : -1;
+        // q's rows through shared memory (where odd weights will lie): read row by row, taken back a row a thread.  Piece c of row i
+        // lies at c ^ i, so that neither side meets a bank twice.
+        float4* const stage = reinterpret_cast<float4*>(sm.odd_w);
+        for (int x = tid; x < 128 * (HD / 4); x += 512) {
+            const int i = x / (HD / 4), c = x % (HD / 4), ri = row0 + i / a.group;
+            float4 y = make_float4(0, 0, 0, 0);
+            if (i < a.rq * a.group && ri <= row1)
+                y = *(const float4*)(a.q + ((size_t)s * a.rows + ri) * a.q_ld + (size_t)(kvh * a.group + i % a.group) * HD + 4 * c);
+            stage[i * (HD / 4) + (c ^ (i & (HD / 4 - 1)))] = y;
+        }
+        asm volatile("bar.sync 2, 512;" ::: "memory");
         auto sees = [&](int k) { return k <= p && (a.window <= 0 || k > p - a.window || k < a.first); };
         if (warp < 8) {
             // ---- softmax.  First q: a group each of the halves of its dims into tensor memory, scaled, part by part
             float qs = 1.0f;
             {
-                const float* qr = a.q + ((size_t)s * a.rows + row) * a.q_ld + (size_t)h * HD + w * HALF;
                 const float sl = a.scale * LOG2E;
                 float x[HALF];
                 float top = 0.0f;
 #pragma unroll
                 for (int d = 0; d < HALF; d += 4) {
-                    const float4 y = on ? *(const float4*)(qr + d) : make_float4(0, 0, 0, 0);
+                    const float4 y = stage[r * (HD / 4) + ((w * (HALF / 4) + d / 4) ^ (r & (HD / 4 - 1)))];
                     x[d] = y.x * sl; x[d + 1] = y.y * sl; x[d + 2] = y.z * sl; x[d + 3] = y.w * sl;
 #pragma unroll
                     for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(x[d + i]));
@@ -509,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == ISSUER) {
+    if (warp == ISSUER_S) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
