@@ -7,8 +7,8 @@
 //   S = q K^T          A = q's parts in tensor memory, B = a tile of K in shared memory, S in tensor memory (two or three buffers)
 //   w = 2^(S - m)      a thread per row; its parts go back over S as the next product's A operand
 //   O = w V            A = w's parts, B = the tile of V as it lies in memory (the major axis is its dims)
-//   o = o c + O        in registers: the running output is rescaled and added to in f32, rounded, because a sum that stayed
-//                      in the tensor core over a long prompt would be cut off thousands of times
+//   o = o c + O        in registers, every tile: the tensor core cuts its sums off instead of rounding them, and an O that stayed
+//                      there lost 1.1e-7 of its size every 16 keys (2e-4 at 30000 keys, measured with values of one sign)
 //
 // bf16 takes three parts of q and w, f16 two (fk_attn_paged.cu says why that is f32 precision), so a product is three (two)
 // products: the bound is the tensor cores' rate by that factor.  Per tile of 64 keys and 128 dims that is 1536 (1024) cycles of
@@ -32,10 +32,10 @@ using namespace fk_tc;
 namespace {
 
 constexpr int KT = 64;                         // keys of a tile
-constexpr int THREADS = 640;
-constexpr int LOADER = 16, ISSUER_S = 17, LOOKER = 18, ISSUER_O = 19;
+
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr uint32_t SPINS = 1u << 20;           // polls of a wait before it gives up
+constexpr uint32_t SPINS = 1u << 16;           // tests of a wait before it gives up, each of up to PARK nanoseconds
+constexpr uint32_t PARK = 10000;
 
 struct PromptArgs {
     CUtensorMap map;                           // the layer's pages as [tokens of all pages, halves and heads][head_dim]
@@ -52,12 +52,17 @@ template <int KIND, int HD> struct Plan {
     static constexpr int QP = KIND == KIND_F16 ? 2 : 3;            // parts of q and of the weights
     static constexpr int TILE = KT * HD * 2;                       // bytes of a tile of K or V
     static constexpr int STAGES = HD == 64 ? 6 : 4;
+    // warps: NG softmax groups of 4, 8 of the running output, then the four single ones
+    static constexpr int NG = 2, OUT = 4 * NG, LOADER = OUT + 8, ISSUER_S = LOADER + 1, LOOKER = LOADER + 2, ISSUER_O = LOADER + 3;
+    static constexpr int THREADS = 32 * (LOADER + 4);
     // Tensor memory columns of a tile: S's 64 behind LEAD free ones; the parts of w's first half of the keys take the free ones
     // and S's first half, those of its second half what follows, so that S is never overwritten before it is read.
     static constexpr int SREG = QP * 32, LEAD = SREG - 64;
-    static constexpr int Q0 = 0, O0 = QP * HD / 2, S0 = O0 + HD;
-    // buffers of S: with three a product need not wait for the one whose operand it overwrites
-    static constexpr int NS = S0 + 3 * SREG <= 512 ? 3 : 2;
+    // buffers of O and of S, as tensor memory allows: with two of O a product need not wait for the running output to take the
+    // last one, with three of S not for the product whose operand it overwrites
+    static constexpr int NO = HD == 64 ? 2 : 1;
+    static constexpr int Q0 = 0, O0 = QP * HD / 2, S0 = O0 + NO * HD;
+    static constexpr int NS = S0 + 4 * SREG <= 512 ? 4 : S0 + 3 * SREG <= 512 ? 3 : 2;
     static_assert(S0 + NS * SREG <= 512, "tensor memory");
 };
 
@@ -65,14 +70,14 @@ template <int KIND, int HD> struct PromptSmem {
     using P = Plan<KIND, HD>;
     unsigned char k[P::STAGES][P::TILE];
     unsigned char v[P::STAGES][P::TILE];
-    float odd_w[2][KT][128];                   // per softmax group: weights of a tile's values that are not finite, by row (-1: not seen)
-    float top[2][128];                         // a row's maximum after the tile (tile number mod 2); before that, of q's halves
-    float corr[4][128];                        // what the running output is multiplied with at the tile (mod 4)
-    float fin[2][2][128];                      // per softmax group: denominator and the maximum it refers to
-    unsigned long long odd_of[4];              // which of the tile's values are not finite (mod 4)
+    float odd_w[P::NG][KT][128];                   // per softmax group: weights of a tile's values that are not finite, by row (-1: not seen)
+    float top[P::NG][128];                         // a row's maximum after the group's last tile; before that, of q's halves
+    float corr[8][128];                        // what the running output is multiplied with at the tile (mod 8)
+    float fin[P::NG][2][128];                      // per softmax group: denominator and the maximum it refers to
+    unsigned long long odd_of[8];              // which of the tile's values are not finite (mod 8)
     unsigned long long odd[P::STAGES];         // the same, where the values lie
     unsigned long long kfull[P::STAGES], kfree[P::STAGES], vfull[P::STAGES], vfree[P::STAGES], vready[P::STAGES];
-    unsigned long long sfull[P::NS], pfull[P::NS], mfull[2][4], oddfree[2], ofull, ofree, qfull, done[2];
+    unsigned long long sfull[P::NS], pfull[P::NS], mfull[P::NG][4], oddfree[P::NG], ofull[P::NO], ofree[P::NO], qfull, done[2];
     uint32_t tmem;
     int abort;
 };
@@ -83,6 +88,14 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
+}
+// Whether the phase has completed; the hardware parks the warp until it has or PARK is over, so that a dozen waiting warps do not
+// take issue slots and shared memory from the others.
+__device__ __forceinline__ bool parked(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(PARK) : "memory");
+    return ok != 0;
 }
 __device__ __forceinline__ bool elected() {
     uint32_t r;
@@ -97,6 +110,10 @@ __device__ __forceinline__ float pow2f(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+__device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 // (lo, hi) rounded to a pair of the type; lo and hi become what is left
 template <int KIND> __device__ __forceinline__ uint32_t take_part(float& lo, float& hi) {
@@ -123,9 +140,9 @@ template <int N> __device__ __forceinline__ void tm_ld(uint32_t addr, float* v) 
 }
 
 template <int KIND, int HD>
-__global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_constant__ PromptArgs a) {
+__global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kernel(const __grid_constant__ PromptArgs a) {
     using P = Plan<KIND, HD>;
-    constexpr int QP = P::QP, STAGES = P::STAGES, NS = P::NS, HALF = HD / 2;
+    constexpr int QP = P::QP, STAGES = P::STAGES, NS = P::NS, NO = P::NO, NG = P::NG, HALF = HD / 2;
     constexpr float SHIFT = KIND == KIND_F16 ? 14.0f : 0.0f;
     extern __shared__ unsigned char smem_raw[];
     PromptSmem<KIND, HD>& sm = *reinterpret_cast<PromptSmem<KIND, HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -142,42 +159,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
             mbar_init(smem_u32(&sm.sfull[i]), 1);
             mbar_init(smem_u32(&sm.pfull[i]), 4);
         }
-        for (int i = 0; i < 8; i++) mbar_init(smem_u32(&sm.mfull[i >> 2][i & 3]), 1);
-        for (int i = 0; i < 2; i++) mbar_init(smem_u32(&sm.oddfree[i]), 8);
-        mbar_init(smem_u32(&sm.ofull), 1);
-        mbar_init(smem_u32(&sm.ofree), 8);
-        mbar_init(smem_u32(&sm.qfull), 8);
+        for (int i = 0; i < 4 * NG; i++) mbar_init(smem_u32(&sm.mfull[i >> 2][i & 3]), 1);
+        for (int i = 0; i < NG; i++) mbar_init(smem_u32(&sm.oddfree[i]), 8);
+        for (int i = 0; i < NO; i++) {
+            mbar_init(smem_u32(&sm.ofull[i]), 1);
+            mbar_init(smem_u32(&sm.ofree[i]), 8);
+        }
+        mbar_init(smem_u32(&sm.qfull), 16);
         mbar_init(smem_u32(&sm.done[0]), 1);
         mbar_init(smem_u32(&sm.done[1]), 1);
         sm.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // Tensor memory is taken after the previous kernel is done with its own and before the next one may start: neither can
-    // then hold what the other waits for.
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp == ISSUER_S) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-    // a wait gives up after SPINS polls, or at once when another one of the CTA has given up; the CTA then runs to its end
-    auto wait = [&](unsigned long long* bar, uint32_t parity) {
-        const uint32_t b = smem_u32(bar);
-        // the warp goes on together: what it does next stays uniform for the compiler, and operands in uniform registers
-        for (uint32_t i = 0; i < SPINS; i++) {
-            if (__all_sync(0xffffffffu, mbar_try_wait(b, parity))) return;
-            if (__any_sync(0xffffffffu, *(volatile int*)&sm.abort)) return;
-        }
-        *(volatile int*)&sm.abort = 1;
-        fk_raise(a.err, 63);
-    };
-    auto gave_up = [&] { return __any_sync(0xffffffffu, *(volatile int*)&sm.abort) != 0; };      // the same answer for the whole warp
-
     // ---- the item: rows [row0, row1] of sequence s, KV head kvh; long ones (late rows) come first
     const int kvh = blockIdx.x % a.n_kv, s = (blockIdx.x / a.n_kv) % a.n_seqs, rb = a.n_rb - 1 - (int)(blockIdx.x / ((unsigned)a.n_kv * a.n_seqs));
     int n = a.n_new ? min(max(a.n_new[s], 0), a.rows) : a.rows;
@@ -193,55 +187,86 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
     if (na >= b0) na = b0 = 0;
     const int n_tiles = __shfl_sync(0xffffffffu, row1 < row0 ? 0 : na + (hi + KT - 1) / KT - b0, 0);
     const int p_min = base + row0, p_max = hi - 1;
+    if (n_tiles == 0) return;                  // rows that do not exist; the whole CTA leaves
     auto tile_key = [&](int j) { return (j < na ? j : j - na + b0) * KT; };
     auto edge_tile = [&](int key0) { return key0 + KT - 1 > p_min || (a.window > 0 && key0 <= p_max - a.window && key0 + KT - 1 >= a.first); };
 
-    if (warp == LOADER) {
-        // ---- loads: lane u takes the u-th page piece of a tile
-        const int piece = min(a.page, KT), n_pc = KT / piece;
-        auto page_of = [&](int j) {
-            if (j >= n_tiles || lane >= n_pc) return 0;
-            const int key = tile_key(j) + lane * piece;
-            if (key >= hi) return -1;
-            const int pg = a.table[(size_t)s * a.max_pages + (key >> a.log_page)];
-            if (pg >= 0 && pg < a.n_pages) return pg;
-            fk_raise(a.err, 97);
-            return 0;
+    // Tensor memory is taken after the previous kernel is done with its own and before the next one may start: neither can
+    // then hold what the other waits for.
+    if (warp == P::ISSUER_S) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // a wait gives up after SPINS polls, or at once when another one of the CTA has given up; the CTA then runs to its end
+    auto wait = [&](unsigned long long* bar, uint32_t parity) {
+        const uint32_t b = smem_u32(bar);
+        // the warp goes on together: what it does next stays uniform for the compiler, and operands in uniform registers
+        for (uint32_t i = 0; i < SPINS; i++) {
+            if (__all_sync(0xffffffffu, parked(b, parity))) return;
+            if (__any_sync(0xffffffffu, *(volatile int*)&sm.abort)) return;
+        }
+        *(volatile int*)&sm.abort = 1;
+        fk_raise(a.err, 63);
+    };
+    auto gave_up = [&] { return __any_sync(0xffffffffu, *(volatile int*)&sm.abort) != 0; };      // the same answer for the whole warp
+
+    if (warp == P::LOADER) {
+        // ---- loads: lane u takes the u-th page piece of a tile.  The page numbers of 32 pieces are read at once, a lane each and
+        // a block of tiles ahead: a table lookup takes longer than a tile.
+        const int log_piece = min(a.log_page, 6), log_pc = 6 - log_piece, n_pc = 1 << log_pc, ahead = 32 >> log_pc;
+        const int* const tab = a.table + (size_t)s * a.max_pages;
+        auto pages_from = [&](int j0) {
+            const int j = j0 + (lane >> log_pc);
+            const int key = j < n_tiles ? tile_key(j) + ((lane & (n_pc - 1)) << log_piece) : hi;
+            return key < hi ? tab[key >> a.log_page] : -1;
         };
-        int pg = page_of(0), issued = 0;
+        int issued = 0, block = pages_from(0), next = pages_from(ahead);
         for (int j = 0; j < n_tiles; j++) {
-            const int pg_next = page_of(j + 1), st = j % STAGES;
-            const int key = tile_key(j) + lane * piece;
-            const int pieces = min(n_pc, (hi - tile_key(j) + piece - 1) / piece);
-            const bool mine = lane < n_pc && pg >= 0;
-            const int y = ((2 * max(pg, 0)) * a.n_kv + kvh) * a.page + (key & (a.page - 1));
+            const int st = j % STAGES, in_block = j & (ahead - 1);
+            if (j > 0 && in_block == 0) {
+                block = next;
+                next = pages_from(j + ahead);
+            }
+            const int key0 = tile_key(j), key = key0 + (lane << log_piece);
+            int pg = __shfl_sync(0xffffffffu, block, (in_block << log_pc) + (lane & (n_pc - 1)));
+            const int pieces = min(n_pc, (hi - key0 + (1 << log_piece) - 1) >> log_piece);
+            const bool mine = lane < pieces;
+            if (mine && (pg < 0 || pg >= a.n_pages)) {
+                fk_raise(a.err, 97);
+                pg = 0;
+            }
+            const int y = ((2 * pg) * a.n_kv + kvh) * a.page + (key & (a.page - 1));
             if (j >= STAGES) wait(&sm.kfree[st], (j / STAGES - 1) & 1);
             if (j >= STAGES) wait(&sm.vfree[st], (j / STAGES - 1) & 1);
             if (gave_up()) break;
-            if (lane == 0) mbar_expect_tx(smem_u32(&sm.kfull[st]), pieces * piece * HD * 2);
+            if (lane == 0) {
+                mbar_expect_tx(smem_u32(&sm.kfull[st]), (pieces << log_piece) * HD * 2);
+                mbar_expect_tx(smem_u32(&sm.vfull[st]), (pieces << log_piece) * HD * 2);
+            }
             __syncwarp();
             if (mine) {
 #pragma unroll
                 for (int h = 0; h < HD / 64; h++)
-                    tma_load_2d(smem_u32(sm.k[st]) + h * (KT * 128) + lane * piece * 128, &a.map, h * 64, y, smem_u32(&sm.kfull[st]));
-            }
-            if (lane == 0) mbar_expect_tx(smem_u32(&sm.vfull[st]), pieces * piece * HD * 2);
-            __syncwarp();
-            if (mine) {
+                    tma_load_2d(smem_u32(sm.k[st]) + h * (KT * 128) + (lane << log_piece) * 128, &a.map, h * 64, y, smem_u32(&sm.kfull[st]));
 #pragma unroll
                 for (int h = 0; h < HD / 64; h++)
-                    tma_load_2d(smem_u32(sm.v[st]) + h * (KT * 128) + lane * piece * 128, &a.map, h * 64, y + a.n_kv * a.page, smem_u32(&sm.vfull[st]));
+                    tma_load_2d(smem_u32(sm.v[st]) + h * (KT * 128) + (lane << log_piece) * 128, &a.map, h * 64, y + a.n_kv * a.page, smem_u32(&sm.vfull[st]));
             }
-            pg = pg_next;
             issued = j + 1;
         }
         // every copy that was started has landed before the CTA ends
         for (int j = max(0, issued - STAGES); j < issued; j++) {
             const uint32_t par = (j / STAGES) & 1;
-            for (uint32_t i = 0; i < SPINS && !mbar_try_wait(smem_u32(&sm.kfull[j % STAGES]), par); i++) {}
-            for (uint32_t i = 0; i < SPINS && !mbar_try_wait(smem_u32(&sm.vfull[j % STAGES]), par); i++) {}
+            for (uint32_t i = 0; i < SPINS && !parked(smem_u32(&sm.kfull[j % STAGES]), par); i++) {}
+            for (uint32_t i = 0; i < SPINS && !parked(smem_u32(&sm.vfull[j % STAGES]), par); i++) {}
         }
-    } else if (warp == ISSUER_S) {
+    } else if (warp == P::ISSUER_S) {
         // ---- S = q K^T
         constexpr uint32_t ID_S = idesc_of(KIND, 128, KT, 0);
         const uint64_t k_desc = umma_desc(smem_u32(sm.k[0]));
@@ -268,18 +293,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         // tensor memory is given back only when no product is under way
         if (elected()) tc_commit(smem_u32(&sm.done[0]));
         __syncwarp();
-        for (uint32_t i = 0; i < SPINS && !__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&sm.done[0]), 0)); i++) {}
-    } else if (warp == ISSUER_O) {
+        for (uint32_t i = 0; i < SPINS && !__all_sync(0xffffffffu, parked(smem_u32(&sm.done[0]), 0)); i++) {}
+    } else if (warp == P::ISSUER_O) {
         // ---- O = w V
         constexpr uint32_t ID_O = idesc_of(KIND, 128, HD, 1);
         const uint64_t v_desc = umma_desc_of(smem_u32(sm.v[0]), KT * 128, 1024, 2);
         for (int j = 0; j < n_tiles && !gave_up(); j++) {
-            const int st = j % STAGES;
+            const int st = j % STAGES, ob = j % NO;
             wait(&sm.vready[st], (j / STAGES) & 1);
-            if (j > 0) wait(&sm.ofree, (j - 1) & 1);
+            if (j >= NO) wait(&sm.ofree[ob], (j / NO - 1) & 1);
             wait(&sm.pfull[j % NS], (j / NS) & 1);
             tc_fence_after();
-            const uint32_t w = tmem + P::S0 + (j % NS) * P::SREG;
+            const uint32_t w = tmem + P::S0 + (j % NS) * P::SREG, d = tmem + P::O0 + ob * HD;
             const uint64_t b = v_desc + (uint32_t)(st * (P::TILE >> 4));
             if (elected()) {
 #pragma unroll
@@ -287,53 +312,59 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
 #pragma unroll
                     for (int ks = 0; ks < KT / 16; ks++)
                         // 16 keys of all dims: 64-dim halves KT * 128 bytes apart, groups of 8 keys 1024 bytes apart
-                        mma_ts(tmem + P::O0, w + (ks >> 1) * (QP * 16) + k * 16 + (ks & 1) * 8, b + (ks * 2048 >> 4), ID_O, k < QP - 1 || ks > 0);
-                tc_commit(smem_u32(&sm.ofull));
+                        mma_ts(d, w + (ks >> 1) * (QP * 16) + k * 16 + (ks & 1) * 8, b + (ks * 2048 >> 4), ID_O, k < QP - 1 || ks > 0);
+                tc_commit(smem_u32(&sm.ofull[ob]));
                 tc_commit(smem_u32(&sm.vfree[st]));
             }
             __syncwarp();
         }
         if (elected()) tc_commit(smem_u32(&sm.done[1]));
         __syncwarp();
-        for (uint32_t i = 0; i < SPINS && !__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&sm.done[1]), 0)); i++) {}
-    } else if (warp == LOOKER) {
+        for (uint32_t i = 0; i < SPINS && !__all_sync(0xffffffffu, parked(smem_u32(&sm.done[1]), 0)); i++) {}
+    } else if (warp == P::LOOKER) {
         // ---- values that not every row sees
         for (int j = 0; j < n_tiles && !gave_up(); j++) {
             const int st = j % STAGES, key0 = tile_key(j);
             wait(&sm.vfull[st], (j / STAGES) & 1);
             if (edge_tile(key0)) {
-                unsigned long long odd = 0;
-                for (int r = lane; r < KT; r += 32) {
-                    const int k = key0 + r;
+                // a quarter of the warp per row of 128 bytes, so that neighbouring lanes read neighbouring pieces
+                uint32_t odd[2] = {0, 0};
+#pragma unroll 4
+                for (int x = 0; x < KT / 4; x++) {
+                    const int r = 4 * x + (lane >> 3), k = key0 + r;
                     const bool some = k <= p_max && (a.window <= 0 || k > p_min - a.window || k < a.first);
                     const bool every = k <= p_min && (a.window <= 0 || k > p_max - a.window || k < a.first);
                     bool bad = false;
                     if (some && !every) {
-                        for (int c = 0; c < HD / 8; c++) {
-                            const uint4 x = *(const uint4*)(sm.v[st] + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int h = 0; h < HD / 64; h++) {
+                            const uint4 y = *(const uint4*)(sm.v[st] + h * (KT * 128) + r * 128 + (lane & 7) * 16);
+                            const uint32_t u[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                if (KIND == KIND_F16) bad = bad || (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
-                                else bad = bad || (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
+                                if (KIND == KIND_F16) bad = bad || (u[i] & 0x7c00u) == 0x7c00u || (u[i] & 0x7c000000u) == 0x7c000000u;
+                                else bad = bad || (u[i] & 0x7f80u) == 0x7f80u || (u[i] & 0x7f800000u) == 0x7f800000u;
                             }
                         }
                     }
-                    if (bad) odd |= 1ull << r;
-                    if (bad || !some)
-                        for (int c = 0; c < HD / 8; c++) *(uint4*)(sm.v[st] + (c >> 3) * (KT * 128) + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    const uint32_t votes = __ballot_sync(0xffffffffu, bad);
+                    const bool row_bad = votes >> (lane & 24) & 0xff;
+                    if (row_bad || !some) {
+#pragma unroll
+                        for (int h = 0; h < HD / 64; h++) *(uint4*)(sm.v[st] + h * (KT * 128) + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    if (votes)
+                        for (int i = 0; i < 4; i++)
+                            if (votes >> (8 * i) & 0xff) odd[x >> 3] |= 1u << ((4 * x + i) & 31);
                 }
-                uint32_t half[2] = {(uint32_t)odd, (uint32_t)(odd >> 32)};
-                half[0] = __reduce_or_sync(0xffffffffu, half[0]);
-                half[1] = __reduce_or_sync(0xffffffffu, half[1]);
-                if (lane == 0) sm.odd[st] = half[0] | (unsigned long long)half[1] << 32;
+                if (lane == 0) sm.odd[st] = odd[0] | (unsigned long long)odd[1] << 32;
                 fence_proxy_async();
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sm.vready[st]));
         }
     } else {
-        const int w = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;       // softmax group, or half of the dims; row of the 128
+        const int w = warp < P::OUT ? warp >> 2 : (warp - P::OUT) >> 2, r = (warp & 3) * 32 + lane;       // softmax group, or half of the dims; row of the 128
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const int row = row0 + r / a.group, h = kvh * a.group + r % a.group;
         const bool on = r < a.rq * a.group && row <= row1;
@@ -341,58 +372,73 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         // q's rows through shared memory (where odd weights will lie): read row by row, taken back a row a thread.  Piece c of row i
         // lies at c ^ i, so that neither side meets a bank twice.
         float4* const stage = reinterpret_cast<float4*>(sm.odd_w);
-        for (int x = tid; x < 128 * (HD / 4); x += 512) {
-            const int i = x / (HD / 4), c = x % (HD / 4), ri = row0 + i / a.group;
-            float4 y = make_float4(0, 0, 0, 0);
-            if (i < a.rq * a.group && ri <= row1)
-                y = *(const float4*)(a.q + ((size_t)s * a.rows + ri) * a.q_ld + (size_t)(kvh * a.group + i % a.group) * HD + 4 * c);
-            stage[i * (HD / 4) + (c ^ (i & (HD / 4 - 1)))] = y;
+        constexpr int ROW4 = HD / 4, SHARE = 128 * ROW4 / 512;
+        float qs = 1.0f;
+        if (tid < 512) {
+            float4 y[SHARE];
+            const uint32_t inv = (65535 + a.group) / a.group;      // i / group = i inv / 2^16 below 128
+#pragma unroll
+            for (int u = 0; u < SHARE; u++) {
+                const int x = u * 512 + tid, i = x / ROW4, ig = (int)(i * inv >> 16), ri = row0 + ig;
+                y[u] = make_float4(0, 0, 0, 0);
+                if (i < a.rq * a.group && ri <= row1)
+                    y[u] = *(const float4*)(a.q + ((size_t)s * a.rows + ri) * a.q_ld + (size_t)(kvh * a.group + i - ig * a.group) * HD + 4 * (x % ROW4));
+            }
+#pragma unroll
+            for (int u = 0; u < SHARE; u++) {
+                const int x = u * 512 + tid, i = x / ROW4;
+                stage[i * ROW4 + ((x % ROW4) ^ (i & (ROW4 - 1)))] = y[u];
+            }
         }
-        asm volatile("bar.sync 2, 512;" ::: "memory");
-        auto sees = [&](int k) { return k <= p && (a.window <= 0 || k > p - a.window || k < a.first); };
-        if (warp < 8) {
-            // ---- softmax.  First q: a group each of the halves of its dims into tensor memory, scaled, part by part
-            float qs = 1.0f;
-            {
-                const float sl = a.scale * LOG2E;
-                float x[HALF];
-                float top = 0.0f;
+        asm volatile("bar.sync 2, %0;" ::"n"(32 * P::LOADER) : "memory");
+        {
+            // a quarter of a row a thread: scaled, split, into tensor memory part by part
+            constexpr int QUARTER = HD / 4;
+            const int qt = (warp >> 2) & 3;                        // groups beyond 16 warps repeat a quarter and keep it to themselves
+            const float sl = a.scale * LOG2E;
+            float x[QUARTER], top = 0.0f;
 #pragma unroll
-                for (int d = 0; d < HALF; d += 4) {
-                    const float4 y = stage[r * (HD / 4) + ((w * (HALF / 4) + d / 4) ^ (r & (HD / 4 - 1)))];
-                    x[d] = y.x * sl; x[d + 1] = y.y * sl; x[d + 2] = y.z * sl; x[d + 3] = y.w * sl;
+            for (int d = 0; d < QUARTER; d += 4) {
+                const float4 z = stage[r * ROW4 + ((qt * (QUARTER / 4) + d / 4) ^ (r & (ROW4 - 1)))];
+                x[d] = z.x * sl; x[d + 1] = z.y * sl; x[d + 2] = z.z * sl; x[d + 3] = z.w * sl;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(x[d + i]));
+                for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(x[d + i]));
+            }
+            if (KIND == KIND_F16) {
+                float* const tops = &sm.fin[0][0][0];              // [4][128]
+                if (warp < 16) tops[qt * 128 + r] = top;
+                asm volatile("bar.sync 2, %0;" ::"n"(32 * P::LOADER) : "memory");
+                top = fmaxf(fmaxf(tops[r], tops[128 + r]), fmaxf(tops[256 + r], tops[384 + r]));
+                // 2^e with top * 2^e in [2^13, 2^14)
+                int ex = top > 0.0f && top < INFINITY ? 13 - (int)((__float_as_uint(top) >> 23) & 255) + 127 : 0;
+                ex = max(-100, min(100, ex));
+                const float f = __uint_as_float((uint32_t)(127 + ex) << 23);
+#pragma unroll
+                for (int d = 0; d < QUARTER; d++) x[d] *= f;
+                qs = __uint_as_float((uint32_t)(127 - ex) << 23);
+            }
+            if (warp < 16) {
+#pragma unroll
+                for (int k = 0; k < QP; k++) {
+                    uint32_t pk[QUARTER / 2];
+#pragma unroll
+                    for (int i = 0; i < QUARTER / 2; i++) pk[i] = take_part<KIND>(x[2 * i], x[2 * i + 1]);
+                    const uint32_t at = tmem + lanes + P::Q0 + k * HALF + qt * (QUARTER / 2);
+                    if (HD == 128) tc_st16(at, pk);
+                    else tc_st8(at, pk);
                 }
-                if (KIND == KIND_F16) {
-                    sm.top[w][r] = top;
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    top = fmaxf(top, sm.top[1 - w][r]);
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    int ex = top > 0.0f && top < INFINITY ? 13 - (int)((__float_as_uint(top) >> 23) & 255) + 127 : 0;
-                    ex = max(-100, min(100, ex));
-                    const float f = __uint_as_float((uint32_t)(127 + ex) << 23);
-#pragma unroll
-                    for (int d = 0; d < HALF; d++) x[d] *= f;
-                    qs = __uint_as_float((uint32_t)(127 - ex) << 23);
-                }
-#pragma unroll
-                for (int k = 0; k < QP; k++)
-#pragma unroll
-                    for (int c = 0; c < HALF / 2; c += 16) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int i = 0; i < 16; i++) pk[i] = take_part<KIND>(x[2 * (c + i)], x[2 * (c + i) + 1]);
-                        tc_st16(tmem + lanes + P::Q0 + k * HALF + w * (HALF / 2) + c, pk);
-                    }
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sm.qfull));
             }
+        }
+        auto sees = [&](int k) { return k <= p && (a.window <= 0 || k > p - a.window || k < a.first); };
+        if (warp < P::OUT) {
+            // ---- softmax
             float m = -INFINITY, l = 0.0f;                         // the denominator of this group's tiles, relative to m
             int odds = 0;
-            for (int j = w; j < n_tiles; j += 2) {
+            for (int j = w; j < n_tiles; j += NG) {
                 const int key0 = tile_key(j);
                 wait(&sm.sfull[j % NS], (j / NS) & 1);
                 tc_fence_after();
@@ -416,15 +462,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
                         for (int k = 0; k < 4; k++) top[k] = fmaxf(fmaxf(top[k], v[i + k]), v[i + 4 + k]);
                 }
                 const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * qs;
-                // the row's maximum so far comes from the other group's warp of the same rows
+                // the row's maximum so far comes from the group of the tile before: its warp of the same rows
                 float m_old = -INFINITY;
                 if (j > 0) {
-                    wait(&sm.mfull[1 - w][warp & 3], ((j - 1) >> 1) & 1);
-                    m_old = sm.top[1 - w][r];
+                    const int g = w == 0 ? NG - 1 : w - 1;
+                    wait(&sm.mfull[g][warp & 3], ((j - 1) / NG) & 1);
+                    m_old = sm.top[g][r];
                 }
                 const float m_new = fmaxf(m_old, t), ms = m_new == -INFINITY ? 0.0f : m_new - SHIFT;
                 sm.top[w][r] = m_new;
-                sm.corr[j & 3][r] = m_old == -INFINITY ? 0.0f : pow2f(m_old - m_new);
+                sm.corr[j & 7][r] = m_old == -INFINITY ? 0.0f : pow2f(m_old - m_new);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sm.mfull[w][warp & 3]));
                 l *= m == -INFINITY ? 1.0f : pow2f(m - m_new);
@@ -438,7 +485,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
                         odds++;
                     }
                 }
-                if (r == 0) sm.odd_of[j & 3] = odd;
+                if (r == 0) sm.odd_of[j & 7] = odd;
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     if (c) scores(c, v);                           // half 0 is still there
@@ -469,29 +516,30 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
             }
             sm.fin[w][0][r] = l;
             sm.fin[w][1][r] = m;
-            asm volatile("bar.sync 2, 512;" ::: "memory");
+            asm volatile("bar.sync 2, %0;" ::"n"(32 * P::LOADER) : "memory");
         } else {
             // ---- the running output: o = o corr + O
             float o[HALF];
 #pragma unroll
             for (int d = 0; d < HALF; d++) o[d] = 0.0f;
             for (int j = 0; j < n_tiles; j++) {
-                wait(&sm.ofull, j & 1);
+                const int ob = j % NO;
+                wait(&sm.ofull[ob], (j / NO) & 1);
                 tc_fence_after();
-                const float c = sm.corr[j & 3][r];
-                const unsigned long long odd = __shfl_sync(0xffffffffu, sm.odd_of[j & 3], 0);
+                const float c = sm.corr[j & 7][r];
+                const unsigned long long odd = __shfl_sync(0xffffffffu, sm.odd_of[j & 7], 0);
                 constexpr int N = HD == 64 ? 32 : 16;
 #pragma unroll
                 for (int d0 = 0; d0 < HALF; d0 += N) {
                     float x[N];
-                    tm_ld<N>(tmem + lanes + P::O0 + w * HALF + d0, x);
+                    tm_ld<N>(tmem + lanes + P::O0 + ob * HD + w * HALF + d0, x);
 #pragma unroll
                     for (int d = 0; d < N; d++) o[d0 + d] = fmaf(o[d0 + d], c, x[d]);
                 }
                 if (odd) {                                         // rare: values that are not finite, for the rows that see them
                     for (int i = 0; i < KT; i++) {
                         if (!(odd >> i & 1)) continue;
-                        const float wt = sm.odd_w[j & 1][i][r];
+                        const float wt = sm.odd_w[j % NG][i][r];
                         if (wt < 0.0f) continue;
                         const int k = tile_key(j) + i, pg = min(max(a.table[(size_t)s * a.max_pages + (k >> a.log_page)], 0), a.n_pages - 1);
                         const uint16_t* vr = (const uint16_t*)a.data + ((((size_t)2 * pg + 1) * a.n_kv + kvh) * a.page + (k & (a.page - 1))) * HD + w * HALF;
@@ -499,28 +547,40 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
                         for (int d = 0; d < HALF; d++) o[d] = fmaf(wt, KIND == KIND_F16 ? fk_h2f(vr[d]) : __uint_as_float((uint32_t)vr[d] << 16), o[d]);
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&sm.oddfree[j & 1]));
+                    if (lane == 0) mbar_arrive(smem_u32(&sm.oddfree[j % NG]));
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sm.ofree));
+                if (lane == 0) mbar_arrive(smem_u32(&sm.ofree[ob]));
             }
-            // the two groups' denominators, the sink, the output
-            asm volatile("bar.sync 2, 512;" ::: "memory");
-            if (on && n_tiles > 0) {
-                const float m0 = sm.fin[0][1][r], m1 = sm.fin[1][1][r], m = fmaxf(m0, m1);
-                float l = sm.fin[0][0][r] * (m0 == m ? 1.0f : pow2f(m0 - m)) + sm.fin[1][0][r] * (m1 == m ? 1.0f : pow2f(m1 - m));
-                if (a.sinks) l += m == -INFINITY ? 1.0f : pow2f(a.sinks[h] * LOG2E - m + SHIFT);
-                const float inv = 1.0f / l;
-                float* dst = a.out + (((size_t)s * a.rows + row) * a.n_heads + h) * HD + w * HALF;
+            // the groups' denominators, the sink, the output
+            asm volatile("bar.sync 2, %0;" ::"n"(32 * P::LOADER) : "memory");
+            if (n_tiles > 0) {
+                float m = -INFINITY, l = 0.0f;
 #pragma unroll
-                for (int d = 0; d < HALF; d += 4) *(float4*)(dst + d) = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
+                for (int g = 0; g < NG; g++) m = fmaxf(m, sm.fin[g][1][r]);
+#pragma unroll
+                for (int g = 0; g < NG; g++) l += sm.fin[g][0][r] * (sm.fin[g][1][r] == m ? 1.0f : pow2f(sm.fin[g][1][r] - m));
+                if (a.sinks && on) l += m == -INFINITY ? 1.0f : pow2f(a.sinks[h] * LOG2E - m + SHIFT);
+                const float inv = 1.0f / l;
+                // through shared memory as q came, so that rows are written whole
+#pragma unroll
+                for (int d = 0; d < HALF; d += 4)
+                    stage[r * ROW4 + ((w * (HALF / 4) + d / 4) ^ (r & (ROW4 - 1)))] = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll 4
+                for (int x = tid - 32 * P::OUT; x < 128 * ROW4; x += 256) {
+                    const int i = x / ROW4, ig = (int)(i * ((65535u + a.group) / a.group) >> 16), ri = row0 + ig;
+                    if (i < a.rq * a.group && ri <= row1)
+                        *(float4*)(a.out + ((size_t)s * a.rows + ri) * a.n_heads * HD + (size_t)(kvh * a.group + i - ig * a.group) * HD + 4 * (x % ROW4)) =
+                            stage[i * ROW4 + ((x % ROW4) ^ (i & (ROW4 - 1)))];
+                }
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == ISSUER_S) {
+    if (warp == P::ISSUER_S) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
@@ -535,7 +595,7 @@ template <int KIND, int HD> int launch_prompt(fk_ctx* ctx, cudaStream_t st, cons
         FK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared), FK_KERNEL);
         ready[ctx->device & 63] = true;
     }
-    FK_CUDA(launch(kern, dim3(grid), dim3(THREADS), smem, st, a), FK_LAUNCH);
+    FK_CUDA(launch(kern, dim3(grid), dim3(Plan<KIND, HD>::THREADS), smem, st, a), FK_LAUNCH);
     return FK_OK;
 }
 
