@@ -450,6 +450,7 @@ FK_EXPORT int fk_pages_grow(fk_ctx* ctx, void* stream, const fk_pages* p, const 
 FK_EXPORT int fk_pages_advance(fk_ctx* ctx, void* stream, const fk_pages* p, const int* n_new_dev, int n_new) {
     const int rc = check("pages_advance", ctx, p);
     if (rc != FK_OK) return rc;
+    if (!n_new_dev && n_new < 0) return fk_fail(FK_INVALID, "pages_advance: %d tokens", n_new);
     FkDeviceGuard g(ctx->device);
     FK_CUDA(launch(advance_kernel, dim3((p->n_seqs + 255) / 256), dim3(256), 0, (cudaStream_t)stream, p->lens_dev, p->n_seqs, n_new_dev, n_new), FK_LAUNCH);
     FK_PAGED_LAUNCHED();

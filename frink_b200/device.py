@@ -591,6 +591,7 @@ class Pages:
         self._c = _CPages(data.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), base, _ws.numel() - (base - _ws.data_ptr()),
                           _PAGE_KINDS[data.dtype], n_layers, n_pages, page, n_kv, hd, self.n_seqs, self.max_pages)
         self._p = C.byref(self._c)
+        self._dev, self._scale = data.get_device(), hd ** -0.5
 
     @classmethod
     def alloc(cls, n_layers, n_pages, page, n_kv, head_dim, n_seqs, max_pages, dtype=torch.bfloat16, device="cuda"):
@@ -606,13 +607,24 @@ class Pages:
         return Pages(self.data, self.table[s:s + 1], self.lens[s:s + 1], self.refs, _ws=self._ws)
 
 
+# These calls are a few microseconds of GPU work: the checks read each attribute once, the stream comes as its plain handle.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda i: torch.cuda.current_stream(i).cuda_stream
+
+
 def _n_new(pg, n_new):
     """(device pointer or None, count) of the rows every sequence gets."""
     if isinstance(n_new, torch.Tensor):
-        if not (n_new.dtype == torch.int32 and n_new.device == pg.data.device and n_new.shape == (pg.n_seqs,) and n_new.is_contiguous()):
+        if n_new.dtype != torch.int32 or n_new.get_device() != pg._dev or n_new.shape != (pg.n_seqs,) or not n_new.is_contiguous():
             raise _lib.Invalid(f"pages: n_new is an int32 tensor of {pg.n_seqs} counts on the pages' device")
         return n_new.data_ptr(), 0
     return None, int(n_new)
+
+
+def _counts(pg, n_new):
+    """The optional counts of a call on rows: which of them are real."""
+    if n_new is not None and not isinstance(n_new, torch.Tensor):
+        raise _lib.Invalid("pages: the rows' counts are a device tensor (the number of rows a sequence follows from q)")
+    return None if n_new is None else _n_new(pg, n_new)[0]
 
 
 def _list(ids):
@@ -621,12 +633,12 @@ def _list(ids):
 
 def pages_grow(pg, n_new):
     """Every sequence gets the pages for n_new (an int, or int32 [n_seqs] on the device) tokens more than it holds."""
-    check(lib().fk_pages_grow(pg._ctx, _stream(pg.data.device), pg._p, *_n_new(pg, n_new)))
+    check(lib().fk_pages_grow(pg._ctx, _raw_stream(pg._dev), pg._p, *_n_new(pg, n_new)))
 
 
 def pages_advance(pg, n_new):
     """lens += n_new: the step's tokens are in."""
-    check(lib().fk_pages_advance(pg._ctx, _stream(pg.data.device), pg._p, *_n_new(pg, n_new)))
+    check(lib().fk_pages_advance(pg._ctx, _raw_stream(pg._dev), pg._p, *_n_new(pg, n_new)))
 
 
 def pages_fork(pg, src, dst, n=None):
@@ -635,37 +647,48 @@ def pages_fork(pg, src, dst, n=None):
     src, dst = list(src), list(dst)
     if len(src) != len(dst) or (n is not None and len(n) != len(src)):
         raise _lib.Invalid("pages_fork: lists of one length")
-    check(lib().fk_pages_fork(pg._ctx, _stream(pg.data.device), pg._p, _list(src), _list(dst), _list(list(n)) if n is not None else None, len(src)))
+    check(lib().fk_pages_fork(pg._ctx, _raw_stream(pg._dev), pg._p, _list(src), _list(dst), _list(list(n)) if n is not None else None, len(src)))
 
 
 def pages_free(pg, seqs):
     """The listed sequences give their pages back and hold nothing (at most 64 a call)."""
     seqs = list(seqs)
-    check(lib().fk_pages_free(pg._ctx, _stream(pg.data.device), pg._p, _list(seqs), len(seqs)))
+    check(lib().fk_pages_free(pg._ctx, _raw_stream(pg._dev), pg._p, _list(seqs), len(seqs)))
 
 
 def pages_compact(pg):
     """Moves the pages in use to the front of the pool -> their number (int32 [1] on the device)."""
     used = torch.empty(1, dtype=torch.int32, device=pg.data.device)
-    check(lib().fk_pages_compact(pg._ctx, _stream(pg.data.device), pg._p, used.data_ptr()))
+    check(lib().fk_pages_compact(pg._ctx, _raw_stream(pg._dev), pg._p, used.data_ptr()))
     return used
 
 
-def _rows_of(pg, q, width, what):
-    """q [n_seqs * rows, width], any row stride -> (rows, row stride)."""
-    if not (q.is_cuda and q.device == pg.data.device and q.dtype == torch.float32 and q.dim() == 2 and q.shape[1] == width and q.stride(1) == 1):
+def _rows_of(pg, t, width, what):
+    """t [n_seqs * rows, width], any row stride -> (number of rows, row stride)."""
+    if t.dtype != torch.float32 or t.get_device() != pg._dev or t.dim() != 2:
         raise _lib.Invalid(f"{what}: float32 rows of {width} on the pages' device")
-    n = q.shape[0]
+    (n, w), (ld, one) = t.shape, t.stride()
+    if w != width or one != 1:
+        raise _lib.Invalid(f"{what}: float32 rows of {width}, their values side by side")
     if n == 0 or n % pg.n_seqs:
         raise _lib.Invalid(f"{what}: {n} rows for {pg.n_seqs} sequences")
-    return n // pg.n_seqs, q.stride(0) if n > 1 else max(q.stride(0), width)
+    return n, ld if n > 1 else max(ld, width)
+
+
+def _out_like(pg, out, n, width, what):
+    """The result's tensor: a new one, or the caller's."""
+    if out is None:
+        return torch.empty((n, width), dtype=torch.float32, device=pg.data.device)
+    if out.dtype != torch.float32 or out.get_device() != pg._dev or out.shape != (n, width) or not out.is_contiguous():
+        raise _lib.Invalid(f"{what}: out is a contiguous float32 tensor of q's shape")
+    return out
 
 
 def _vec(pg, t, n, what):
     """An optional contiguous float32 vector of n values on the pages' device -> its address."""
     if t is None:
         return None
-    if not (t.dtype == torch.float32 and t.device == pg.data.device and t.numel() == n and t.is_contiguous()):
+    if t.dtype != torch.float32 or t.get_device() != pg._dev or t.numel() != n or not t.is_contiguous():
         raise _lib.Invalid(f"{what}: {n} contiguous float32 values on the pages' device")
     return t.data_ptr()
 
@@ -675,19 +698,17 @@ def rope_kv_paged(q, k, v, pg, layer, n_heads, theta, neox=False, n_new=None, q_
     are [n_seqs * rows, heads * head_dim] (column slices are fine), row i of sequence s goes to position lens[s] + i; rows from
     n_new[s] on are skipped.  -> the rotated q (`out` may be q itself where its rows are packed); k stays as it is."""
     hd = pg.head_dim
-    rows, q_ld = _rows_of(pg, q, n_heads * hd, "rope_kv_paged: q")
-    for t in (k, v):
-        if _rows_of(pg, t, pg.n_kv * hd, "rope_kv_paged: k, v")[0] != rows:
-            raise _lib.Invalid("rope_kv_paged: q, k and v have the same number of rows")
-    one = q.shape[0] == 1
-    if out is None:
-        out = torch.empty((q.shape[0], n_heads * hd), dtype=torch.float32, device=q.device)
-    elif not (out.shape == q.shape and out.dtype == torch.float32 and out.device == q.device and out.is_contiguous()):
-        raise _lib.Invalid("rope_kv_paged: out is a contiguous float32 tensor of q's shape")
-    check(lib().fk_rope_kv_paged(pg._ctx, _stream(q.device), pg._p, int(layer), q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ld,
-                                 k.stride(0) if not one else pg.n_kv * hd, v.stride(0) if not one else pg.n_kv * hd, rows,
-                                 _n_new(pg, n_new)[0] if n_new is not None else None, n_heads, float(theta), int(neox),
-                                 _vec(pg, q_norm, hd, "rope_kv_paged: q_norm"), _vec(pg, k_norm, hd, "rope_kv_paged: k_norm"), float(eps), out.data_ptr()))
+    n, q_ld = _rows_of(pg, q, n_heads * hd, "rope_kv_paged: q")
+    nk, k_ld = _rows_of(pg, k, pg.n_kv * hd, "rope_kv_paged: k")
+    nv, v_ld = _rows_of(pg, v, pg.n_kv * hd, "rope_kv_paged: v")
+    if nk != n or nv != n:
+        raise _lib.Invalid("rope_kv_paged: q, k and v have the same number of rows")
+    out = _out_like(pg, out, n, n_heads * hd, "rope_kv_paged")
+    if n == 1:
+        q_ld, k_ld, v_ld = n_heads * hd, pg.n_kv * hd, pg.n_kv * hd
+    check(lib().fk_rope_kv_paged(pg._ctx, _raw_stream(pg._dev), pg._p, layer, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ld, k_ld, v_ld, n // pg.n_seqs,
+                                 _counts(pg, n_new), n_heads, theta, neox, _vec(pg, q_norm, hd, "rope_kv_paged: q_norm"),
+                                 _vec(pg, k_norm, hd, "rope_kv_paged: k_norm"), eps, out.data_ptr()))
     return out
 
 
@@ -696,14 +717,11 @@ def attention_paged(q, pg, layer, n_heads, n_new=None, scale=None, window=0, fir
     of 4), row i of sequence s at position lens[s] + i, its own key and value appended already.  window > 0: the `window` most
     recent keys and the `first` earliest; sinks [n_heads]: a logit per head in the softmax's denominator.  Rows from n_new[s]
     (int32 [n_seqs]) on are left as they were in `out`."""
-    rows, ld = _rows_of(pg, q, n_heads * pg.head_dim, "attention_paged: q")
-    if out is None:
-        out = torch.empty((q.shape[0], q.shape[1]), dtype=torch.float32, device=q.device)
-    elif not (out.shape == q.shape and out.dtype == torch.float32 and out.device == q.device and out.is_contiguous()):
-        raise _lib.Invalid("attention_paged: out is a contiguous float32 tensor of q's shape")
-    check(lib().fk_attention_paged(pg._ctx, _stream(q.device), pg._p, int(layer), q.data_ptr(), ld, rows,
-                                   _n_new(pg, n_new)[0] if n_new is not None else None, n_heads,
-                                   float(scale) if scale is not None else pg.head_dim ** -0.5, int(window), int(first),
+    width = n_heads * pg.head_dim
+    n, ld = _rows_of(pg, q, width, "attention_paged: q")
+    out = _out_like(pg, out, n, width, "attention_paged")
+    check(lib().fk_attention_paged(pg._ctx, _raw_stream(pg._dev), pg._p, layer, q.data_ptr(), ld if n > 1 else width, n // pg.n_seqs,
+                                   _counts(pg, n_new), n_heads, pg._scale if scale is None else scale, window, first,
                                    _vec(pg, sinks, n_heads, "attention_paged: sinks"), out.data_ptr()))
     return out
 
@@ -717,38 +735,48 @@ def logit_rules(logits, history=None, penalties=None, bias=None, mask=None, out=
     (int32 words [words] or [n, words], bit v % 32 of word v / 32) is clear become -inf.  tokens: the largest, ties to the lower
     index; -1 where nothing is left."""
     x = logits if logits.dim() == 2 else logits[None]
-    if not (x.is_cuda and x.dtype == torch.float32 and x.dim() == 2 and x.stride(1) == 1 and x.shape[0] > 0 and x.shape[1] > 0):
+    dev = x.get_device()
+    if dev < 0 or x.dtype != torch.float32 or x.dim() != 2:
         raise _lib.Invalid("logit_rules: float32 CUDA logits [n, vocab]")
-    n, V = x.shape
-
-    def rows(t, dtype, width, what):
-        # (tensor, floats or words between rows; 0: one row for all)
-        if t.dtype != dtype or t.device != x.device or t.dim() not in (1, 2) or t.stride(-1) != 1 or t.shape[-1] < width or (t.dim() == 2 and t.shape[0] != n):
-            raise _lib.Invalid(f"logit_rules: {what}")
-        return t.data_ptr(), 0 if t.dim() == 1 else t.stride(0) if n > 1 else max(t.stride(0), width)
-
-    h, hp, pen = 0, None, None
+    (n, V), (ld, one) = x.shape, x.stride()
+    if one != 1 or n == 0 or V == 0:
+        raise _lib.Invalid("logit_rules: float32 CUDA logits [n, vocab], a row's values side by side")
+    h, hp, pen, bp, b_ld, mp, m_ld = 0, None, None, None, 0, None, 0
     if history is not None:
         hist = history if history.dim() == 2 else history[None]
-        if hist.dtype != torch.int32 or hist.device != x.device or hist.dim() != 2 or hist.shape[0] != n or not hist.is_contiguous():
+        if hist.dtype != torch.int32 or hist.get_device() != dev or hist.dim() != 2 or hist.shape[0] != n or not hist.is_contiguous():
             raise _lib.Invalid("logit_rules: history is a contiguous int32 tensor [n, h] beside the logits")
         if penalties is None:
             raise _lib.Invalid("logit_rules: a history needs penalties (repeat, frequency, presence)")
         if not isinstance(penalties, torch.Tensor):
             penalties = torch.tensor([[float(v) for v in penalties]], dtype=torch.float32).to(x.device).expand(n, -1)
-        pen = penalties.contiguous()
-        if pen.dtype != torch.float32 or pen.device != x.device or pen.shape != (n, 3):
+        pen = penalties if penalties.is_contiguous() else penalties.contiguous()
+        if pen.dtype != torch.float32 or pen.get_device() != dev or pen.shape != (n, 3):
             raise _lib.Invalid("logit_rules: penalties are float32 [n, 3]: repeat, frequency, presence")
-        h, hp = hist.shape[1], hist.data_ptr() if hist.shape[1] else None
-    bp, b_ld = rows(bias, torch.float32, V, "bias is float32 [vocab] or [n, vocab]") if bias is not None else (None, 0)
-    mp, m_ld = rows(mask, torch.int32, (V + 31) // 32, "mask is int32 words [ceil(vocab / 32)] or [n, ...]") if mask is not None else (None, 0)
-    o = torch.empty((n, V), dtype=torch.float32, device=x.device) if out is None else out if out.dim() == 2 else out[None]
-    if not (o.shape == (n, V) and o.dtype == torch.float32 and o.device == x.device and o.is_contiguous()):
-        raise _lib.Invalid("logit_rules: out is a contiguous float32 tensor of the logits' shape")
+        h = hist.shape[1]
+        hp = hist.data_ptr() if h else None
+    if bias is not None:
+        bp, b_ld = _rule_rows(bias, torch.float32, dev, n, V, "bias is float32 [vocab] or [n, vocab]")
+    if mask is not None:
+        mp, m_ld = _rule_rows(mask, torch.int32, dev, n, (V + 31) // 32, "mask is int32 words [ceil(vocab / 32)] or [n, ...]")
+    if out is None:
+        o = torch.empty((n, V), dtype=torch.float32, device=x.device)
+    else:
+        o = out if out.dim() == 2 else out[None]
+        if o.shape != (n, V) or o.dtype != torch.float32 or o.get_device() != dev or not o.is_contiguous():
+            raise _lib.Invalid("logit_rules: out is a contiguous float32 tensor of the logits' shape")
     if tokens is None:
         tokens = torch.empty(n, dtype=torch.int32, device=x.device)
-    elif not (tokens.shape == (n,) and tokens.dtype == torch.int32 and tokens.device == x.device and tokens.is_contiguous()):
+    elif tokens.shape != (n,) or tokens.dtype != torch.int32 or tokens.get_device() != dev or not tokens.is_contiguous():
         raise _lib.Invalid("logit_rules: tokens is a contiguous int32 tensor [n]")
-    check(lib().fk_logit_rules(context(x.device), _stream(x.device), x.data_ptr(), x.stride(0) if n > 1 else max(x.stride(0), V), n, V, hp, h,
+    ctx = _contexts.get(dev) or context(x.device)
+    check(lib().fk_logit_rules(ctx, _raw_stream(dev), x.data_ptr(), ld if n > 1 else max(ld, V), n, V, hp, h,
                                pen.data_ptr() if pen is not None else None, bp, b_ld, mp, m_ld, o.data_ptr(), tokens.data_ptr()))
     return (o if logits.dim() == 2 else o[0]), tokens
+
+
+def _rule_rows(t, dtype, dev, n, width, what):
+    """A row for all, or a row each -> (address, values between rows: 0 = one for all)."""
+    if t.dtype != dtype or t.get_device() != dev or t.dim() not in (1, 2) or t.stride(-1) != 1 or t.shape[-1] < width or (t.dim() == 2 and t.shape[0] != n):
+        raise _lib.Invalid(f"logit_rules: {what}")
+    return t.data_ptr(), 0 if t.dim() == 1 else t.stride(0) if n > 1 else max(t.stride(0), width)

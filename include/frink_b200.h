@@ -443,7 +443,7 @@ int fk_attention_paged(fk_ctx* ctx, void* stream, const fk_pages* pages, int lay
  * then x += bias_dev[v] (bias_ld floats between rows, 0 = one row for all), then -inf where bit v % 32 of word v / 32 of
  * mask_dev (mask_ld words between rows, 0 = one row for all) is clear.  out_dev [n_rows][vocab] (may be the logits, packed);
  * tokens_dev [n_rows] (may be null): the largest, ties to the lower index, NaN never; -1 where every token is -inf.
- * history, bias and mask may be null; ld = floats between rows of logits_dev.  One call of this or of fk_argmax in flight per context. */
+ * history (at most 65535), bias and mask may be null; ld = floats between rows of logits_dev.  One call of this or of fk_argmax in flight per context. */
 int fk_logit_rules(fk_ctx* ctx, void* stream, const float* logits_dev, size_t ld, int n_rows, int vocab, const int* history_dev, int history,
                    const float* penalties_dev, const float* bias_dev, size_t bias_ld, const int* mask_dev, size_t mask_ld, float* out_dev,
                    int* tokens_dev);

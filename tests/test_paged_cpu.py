@@ -58,6 +58,7 @@ def test_lists_are_checked():
     refused("fk_pages_fork", CTX, None, p, ints(3), ints(1), None, 1)
     refused("fk_pages_fork", CTX, None, p, None, ints(1), None, 1)
     refused("fk_pages_grow", CTX, None, p, None, -1)
+    refused("fk_pages_advance", CTX, None, p, None, -1)
 
 
 def test_rope_and_attention_arguments():
@@ -76,6 +77,7 @@ def test_logit_rule_arguments():
     ok = [CTX, None, MEM, 100, 2, 100, MEM, 5, MEM, MEM, 0, MEM, 0, MEM * 2, MEM]
     for at, v in ((0, None), (2, None), (3, 99), (4, 0), (5, 0), (6, None), (7, -1), (8, None), (10, 99), (12, 3), (13, None)):
         refused("fk_logit_rules", *(ok[:at] + [v] + ok[at + 1:]))
+    refused("fk_logit_rules", CTX, None, MEM, 100, 2, 100, MEM, 65536, MEM, None, 0, None, 0, MEM * 2, MEM, status=_lib.FK_UNSUPPORTED)
     refused("fk_logit_rules", CTX, None, MEM, 104, 2, 100, None, 0, None, None, 0, None, 0, MEM, None, match="in place")
 
 
