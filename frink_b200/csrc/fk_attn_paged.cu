@@ -37,6 +37,7 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int MAX_ENTRIES = 512;           // (sequence, block of columns) pairs that are dealt out in runs
+constexpr int MAX_CTAS = 4 * 160;           // of a grid that shares items, half as many with 16 columns: the join keeps two words a column of each
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct AttnArgs {
@@ -133,15 +134,20 @@ struct Span {
     int hi;         // keys below this
     int na, b0, tiles;
 };
-template <int COLS> __device__ __forceinline__ Span span_of(const AttnArgs& a, int s, int cb, bool raise) {
+// n: the sequence's rows, 0 where it would outgrow its table row
+__device__ __forceinline__ int2 rows_of(const AttnArgs& a, int s, bool raise) {
+    const int n = a.n_new ? min(max(a.n_new[s], 0), a.rows) : a.rows, base = a.lens[s];
+    if (base >= 0 && (long long)base + n <= (long long)a.max_pages * a.page) return make_int2(base, n);
+    if (raise && n > 0) fk_raise(a.err, 95);
+    return make_int2(base, 0);
+}
+template <int COLS> __device__ __forceinline__ Span span_of(const AttnArgs& a, int2 base_n, int cb) {
     Span r;
-    r.n = a.n_new ? min(max(a.n_new[s], 0), a.rows) : a.rows;
-    r.base = a.lens[s];
-    if (r.base < 0 || (long long)r.base + r.n > (long long)a.max_pages * a.page) {
-        if (raise && r.n > 0) fk_raise(a.err, 95);
-        r.n = 0;
-    }
-    const int row0 = cb * COLS / a.group, row1 = min((cb * COLS + COLS - 1) / a.group, r.n - 1);
+    r.base = base_n.x;
+    r.n = base_n.y;
+    // one row: no division (a block of columns behind the group's has no row)
+    const int row0 = a.rows == 1 ? (cb * COLS < a.group ? 0 : 1) : cb * COLS / a.group;
+    const int row1 = min(a.rows == 1 ? 0 : (cb * COLS + COLS - 1) / a.group, r.n - 1);
     r.lo = r.hi = r.na = r.b0 = r.tiles = 0;
     if (row1 < row0) return r;                         // no real row in the block
     r.hi = r.base + row1 + 1;
@@ -194,7 +200,11 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm.ring[warp]);
     float* const sum_o = reinterpret_cast<float*>(sm.ring[warp]);          // [COLS][PITCH] at the end of an item
 
-    // ---- this CTA's run of units [u, u_end); sm.start[e]: units before entry e (per KV head), times n_kv in the global order
+    // ---- this CTA's run of units [u, u_end); `start` of entry e: units before it (per KV head), times n_kv in the global order.
+    // Up to 32 entries are scanned by every warp for itself, without a barrier; lane e keeps entry e.
+    const bool few = n_e <= 32;
+    int2 lane_rows = make_int2(0, 0);
+    int lane_start = 0x7fffffff;
     int u, u_end, chunk;
     if (a.whole) {                                                 // one item a CTA: blockIdx.x = entry * n_kv + kv head
         u = 0;
@@ -202,17 +212,32 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
         chunk = 1;
     } else {
         int total = 0;
-        for (int e0 = 0; e0 < n_e; e0 += WARPS * 32) {
-            const int e = e0 + tid;
-            const int units = e < n_e ? (span_of<COLS>(a, e / a.n_cb, e % a.n_cb, blockIdx.x == 0).tiles + STEP - 1) / STEP : 0;
-            int sum;
-            const int at = block_prefix(units, sm.part, &sum);
-            if (e < n_e) sm.start[e] = total + at;
-            total += sum;
-            __syncthreads();
+        if (few) {
+            int units = 0;
+            if (lane < n_e) {
+                const int s = a.n_cb == 1 ? lane : lane / a.n_cb;
+                lane_rows = rows_of(a, s, blockIdx.x == 0 && warp == 0);
+                units = (span_of<COLS>(a, lane_rows, lane - s * a.n_cb).tiles + STEP - 1) / STEP;
+            }
+            int x = units;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            if (lane < n_e) lane_start = x - units;
+            total = __shfl_sync(0xffffffffu, x, 31);
+        } else {
+            for (int e0 = 0; e0 < n_e; e0 += WARPS * 32) {
+                const int e = e0 + tid;
+                const int units = e < n_e ? (span_of<COLS>(a, rows_of(a, e / a.n_cb, blockIdx.x == 0), e % a.n_cb).tiles + STEP - 1) / STEP : 0;
+                int sum;
+                const int at = block_prefix(units, sm.part, &sum);
+                if (e < n_e) sm.start[e] = total + at;
+                total += sum;
+                __syncthreads();
+            }
         }
-        if (tid == 0) sm.start[n_e] = total;
-        __syncthreads();
         const long long all = (long long)total * a.n_kv;
         if (all > 0x3fffffffLL) {                                  // no cache holds that many; table rows that share pages could claim it
             if (blockIdx.x == 0 && tid == 0) fk_raise(a.err, 95);
@@ -226,20 +251,28 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
     const int u_begin = u;
 
     while (u < u_end) {
-        int e, kvh, i0, i1, item0 = 0, units;                      // units [i0, i1) of the item, the item's first unit
+        int e, kvh, i0, i1, item0 = 0, units, start = 0;           // units [i0, i1) of the item, the item's first unit
+        int2 rows;
         if (a.whole) {
             e = blockIdx.x / a.n_kv;
             kvh = blockIdx.x % a.n_kv;
+            rows = rows_of(a, e / a.n_cb, tid == 0);
+        } else if (few) {                                          // the last entry that starts at or before u
+            e = 31 - __clz(__ballot_sync(0xffffffffu, (long long)lane_start * a.n_kv <= u));
+            start = __shfl_sync(0xffffffffu, lane_start, e);
+            rows = make_int2(__shfl_sync(0xffffffffu, lane_rows.x, e), __shfl_sync(0xffffffffu, lane_rows.y, e));
         } else {
-            int lo = 0, hi = n_e - 1;                              // the last entry that starts at or before u
+            int lo = 0, hi = n_e - 1;
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
                 if ((long long)sm.start[mid] * a.n_kv <= u) lo = mid; else hi = mid - 1;
             }
             e = lo;
+            start = sm.start[e];
+            rows = rows_of(a, e / a.n_cb, false);
         }
-        const int s = e / a.n_cb, cb = e % a.n_cb;
-        const Span sp = span_of<COLS>(a, s, cb, a.whole && tid == 0);
+        const int s = a.n_cb == 1 ? e : e / a.n_cb, cb = e - s * a.n_cb;
+        const Span sp = span_of<COLS>(a, rows, cb);
         units = (sp.tiles + STEP - 1) / STEP;
         if (a.whole) {
             if (units == 0) return;
@@ -247,8 +280,8 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
             i1 = units;
             u = 1;
         } else {
-            kvh = (u - sm.start[e] * a.n_kv) / units;
-            item0 = sm.start[e] * a.n_kv + kvh * units;
+            kvh = (u - start * a.n_kv) / units;
+            item0 = start * a.n_kv + kvh * units;
             i0 = u - item0;
             i1 = min(units, u_end - item0);
             u = item0 + i1;
@@ -266,14 +299,9 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
             const int x = ((i0 + j) * WARPS + warp) * SUB + u;
             return x >= sp.tiles ? NO_KEY : (x < sp.na ? x : x - sp.na + sp.b0) << 4;
         };
-        auto page_of = [&](int j, int u) {                         // its page
-            if (j >= n_steps) return 0;
-            const int k = tile_key(j, u);
-            if (k == NO_KEY) return 0;
-            const int pg = tab[k >> a.log_page];
-            if (pg >= 0 && pg < a.n_pages) return pg;
-            if (lane == 0) fk_raise(a.err, 97);
-            return 0;
+        auto page_of = [&](int j, int u) {                         // its page, not looked at before the copy needs it
+            const int k = j < n_steps ? tile_key(j, u) : NO_KEY;
+            return k == NO_KEY ? 0 : tab[k >> a.log_page];
         };
         auto request = [&](auto values, int j, const int* pg) {    // starts the copy of a step's keys or values
             constexpr int V = decltype(values)::value;
@@ -282,7 +310,12 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
                 for (int u = 0; u < SUB; u++) {
                     const int k = tile_key(j, u);
                     if (k == NO_KEY) continue;
-                    const char* src = heads + (size_t)(2 * (uint32_t)pg[u] + V) * half_bytes + (uint32_t)(k & (a.page - 1)) * tok_bytes;
+                    int page = pg[u];
+                    if (page < 0 || page >= a.n_pages) {
+                        if (lane == 0) fk_raise(a.err, 97);
+                        page = 0;
+                    }
+                    const char* src = heads + (size_t)(2 * (uint32_t)page + V) * half_bytes + (uint32_t)(k & (a.page - 1)) * tok_bytes;
                     const uint32_t dst = ring + (((j % STAGES) * 2 + V) * SUB + u) * TILE;
                     constexpr int CH = ROWB / 16;
 #pragma unroll
@@ -304,62 +337,72 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
             for (int i = lane; i < 16384 / 16; i += 32) reinterpret_cast<uint4*>(sm.ring[warp])[i] = make_uint4(0, 0, 0, 0);
             __syncwarp();
         }
-        {
-            int pgs[STAGES][SUB];
+        // The first pages' numbers and q are asked for ahead of the first copies, behind which they would queue.
+        int pgs[STAGES][SUB];
 #pragma unroll
-            for (int j = 0; j < STAGES; j++)
+        for (int j = 0; j < STAGES; j++)
 #pragma unroll
-                for (int u = 0; u < SUB; u++) pgs[j][u] = page_of(j, u);
-#pragma unroll
-            for (int j = 0; j < STAGES; j++) {
-                request(Keys{}, j, pgs[j]);
-                request(Values{}, j, pgs[j]);
-            }
-        }
-
-        // ---- q of the item's columns into operand registers' order, scaled, split into parts
-        for (int x = warp; x < NT * KB; x += WARPS) {              // block n of columns, 32 dims kb
+            for (int u = 0; u < SUB; u++) pgs[j][u] = page_of(j, u);
+        // q of the item's columns: scaled, split into parts, in operand registers' order.  A warp takes 32 dims of 8 columns at a
+        // time (f16: all dims are read for the column's maximum).
+        constexpr int QL = KIND == KIND_F16 ? KB : 1;
+        auto q_load = [&](int x, float4 (&v)[QL][2]) {
             const int n = x % NT, kb = x / NT;
             const int c = cb * COLS + n * 8 + g, row = a.rows == 1 ? (c < a.group ? 0 : 1) : c / a.group, h = kvh * a.group + (c - row * a.group);
-            const bool on = row < sp.n;
             const float* qr = a.q + ((size_t)s * a.rows + row) * a.q_ld + (size_t)h * hd;
-            auto eight = [&](int k, float* v) {
-                const int d = 32 * k + 8 * t;
-                float4 x = make_float4(0, 0, 0, 0), y = x;
-                if (on && d < hd) {
-                    x = *(const float4*)(qr + d);
-                    y = *(const float4*)(qr + d + 4);
+#pragma unroll
+            for (int k = 0; k < QL; k++) {
+                const int d = 32 * (QL == 1 ? kb : k) + 8 * t;
+                v[k][0] = v[k][1] = make_float4(0, 0, 0, 0);
+                if (row < sp.n && d < hd) {
+                    v[k][0] = *(const float4*)(qr + d);
+                    v[k][1] = *(const float4*)(qr + d + 4);
                 }
-                const float sl = a.scale * LOG2E;
-                v[0] = x.x * sl; v[1] = x.y * sl; v[2] = x.z * sl; v[3] = x.w * sl;
-                v[4] = y.x * sl; v[5] = y.y * sl; v[6] = y.z * sl; v[7] = y.w * sl;
-            };
-            float v[8];
-            eight(kb, v);
+            }
+        };
+        auto q_store = [&](int x, float4 (&v)[QL][2]) {
+            const int n = x % NT, kb = x / NT;
+            const float sl = a.scale * LOG2E;
+            float4 y = v[0][0], z = v[0][1];
+            float f = sl;
             if (KIND == KIND_F16) {
                 float top = 0.0f;
 #pragma unroll
-                for (int k = 0; k < KB; k++) {
-                    float w[8];
-                    eight(k, w);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(w[i]));
+                for (int k = 0; k < QL; k++) {
+                    const float4 p = v[k][0], r = v[k][1];
+                    top = fmaxf(top, fmaxf(fmaxf(fabsf(p.x), fabsf(p.y)), fmaxf(fabsf(p.z), fabsf(p.w))));
+                    top = fmaxf(top, fmaxf(fmaxf(fabsf(r.x), fabsf(r.y)), fmaxf(fabsf(r.z), fabsf(r.w))));
+                    if (k == kb) { y = p; z = r; }
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * fabsf(sl);
                 // 2^e with top * 2^e in [2^13, 2^14): no part leaves f16's range, and the low part keeps its bits
                 int ex = top > 0.0f && top < INFINITY ? 13 - (int)((__float_as_uint(top) >> 23) & 255) + 127 : 0;
                 ex = max(-100, min(100, ex));
-                const float f = __uint_as_float((uint32_t)(127 + ex) << 23);
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] *= f;
+                f = __uint_as_float((uint32_t)(127 + ex) << 23);
+                y.x *= sl; y.y *= sl; y.z *= sl; y.w *= sl;
+                z.x *= sl; z.y *= sl; z.z *= sl; z.w *= sl;
                 if (t == 0 && kb == 0) sm.qscale[n * 8 + g] = __uint_as_float((uint32_t)(127 - ex) << 23);
             }
             uint32_t p[4][3];
-#pragma unroll
-            for (int i = 0; i < 4; i++) split_pair<KIND>(v[2 * i], v[2 * i + 1], p[i]);
+            split_pair<KIND>(y.x * f, y.y * f, p[0]);
+            split_pair<KIND>(y.z * f, y.w * f, p[1]);
+            split_pair<KIND>(z.x * f, z.y * f, p[2]);
+            split_pair<KIND>(z.z * f, z.w * f, p[3]);
 #pragma unroll
             for (int k = 0; k < QP; k++) sm.q[n][kb][k][lane] = make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
+        };
+        float4 qv[QL][2];
+        if (warp < NT * KB) q_load(warp, qv);
+#pragma unroll
+        for (int j = 0; j < STAGES; j++) {
+            request(Keys{}, j, pgs[j]);
+            request(Values{}, j, pgs[j]);
+        }
+        if (warp < NT * KB) q_store(warp, qv);
+        for (int x = warp + WARPS; x < NT * KB; x += WARPS) {
+            q_load(x, qv);
+            q_store(x, qv);
         }
         __syncthreads();
 
@@ -671,6 +714,14 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
                 }
             }
         __syncthreads();
+        auto finish = [&](int c, int d, float M, float L, float4 O) {      // four dims of a column
+            const int cc = cb * COLS + c, row = a.rows == 1 ? (cc < a.group ? 0 : 1) : cc / a.group, h = kvh * a.group + (cc - row * a.group);
+            if (row >= sp.n || d >= hd) return;
+            // against a maximum far below the sink the sum overflows to infinity and the output is 0, as it should be
+            if (a.sinks) L += M == -INFINITY ? 1.0f : pow2(a.sinks[h] * LOG2E - M + SHIFT);
+            const float inv = 1.0f / L;
+            *(float4*)(a.out + ((size_t)s * a.rows + row) * a.n_heads * hd + (size_t)h * hd + d) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+        };
         const bool direct = a.whole || (i0 == 0 && i1 == units);
         // a CTA's record 1 is the item that begins in its run and goes on behind it, record 0 the one that began before
         float* rec = a.rec + ((size_t)2 * blockIdx.x + (item0 >= u_begin ? 1 : 0)) * ATTN_RECORD;
@@ -689,16 +740,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
                 O.x += v.x * f; O.y += v.y * f; O.z += v.z * f; O.w += v.w * f;
             }
             if (direct) {
-                const int cc = cb * COLS + c, row = cc / a.group, h = kvh * a.group + cc % a.group;
-                if (row < sp.n && d < hd) {
-                    if (a.sinks) {
-                        const float z = a.sinks[h] * LOG2E;
-                        // against a maximum far below the sink the sum overflows to infinity and the output is 0, as it should be
-                        L += M == -INFINITY ? 1.0f : pow2(z - M + SHIFT);
-                    }
-                    const float inv = 1.0f / L;
-                    *(float4*)(a.out + ((size_t)s * a.rows + row) * a.n_heads * hd + (size_t)h * hd + d) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
-                }
+                finish(c, d, M, L, O);
             } else {
                 *(float4*)(rec + c * 128 + d) = O;
                 if (d == 0) {
@@ -709,36 +751,94 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
         }
         if (direct) continue;
 
-        // ---- the last CTA of the item joins the records of CTAs [c0, c1]
-        const int c0 = item0 / chunk, c1 = (item0 + units - 1) / chunk;
-        __threadfence();
+        // ---- the last CTA of the item joins the records of CTAs [c0, c1]: weights of all of them first, then the sums
+        const int c0 = item0 / chunk, n_rec = (item0 + units - 1) / chunk - c0 + 1;
         __syncthreads();
-        if (tid == 0) sm.last = atomicAdd(&a.cnt[c0], 1u) == (unsigned)(c1 - c0);
+        if (tid == 0) {
+            // the CTA's record goes out by way of the barrier and this release, the others' come in by the acquire
+            unsigned before;
+            asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.cnt + c0) : "memory");
+            sm.last = before == (unsigned)(n_rec - 1);
+        }
         __syncthreads();
         if (!sm.last) continue;
-        __threadfence();
+        // record 1 of the CTA in which the item begins, record 0 of the others
+        auto record = [&](int k) { return a.rec + ((size_t)2 * (c0 + k) + (k == 0 ? 1 : 0)) * ATTN_RECORD; };
+        constexpr int FEW = 8;
+        if (n_rec <= FEW) {                                        // everything at once, one trip to memory
+            for (int x = tid; x < COLS * (HDP / 4); x += WARPS * 32) {
+                const int c = x / (HDP / 4), d = 4 * (x % (HDP / 4));
+                float mk[FEW], lk[FEW];
+                float4 v[FEW];
+#pragma unroll
+                for (int k = 0; k < FEW; k++) {
+                    mk[k] = -INFINITY;
+                    lk[k] = 0.0f;
+                    v[k] = make_float4(0, 0, 0, 0);
+                    if (k < n_rec) {
+                        const float* r = record(k);
+                        mk[k] = __ldcg(r + 16 * 128 + c);
+                        lk[k] = __ldcg(r + 16 * 129 + c);
+                        v[k] = __ldcg((const float4*)(r + c * 128 + d));
+                    }
+                }
+                float M = -INFINITY, L = 0.0f;
+                float4 O = make_float4(0, 0, 0, 0);
+#pragma unroll
+                for (int k = 0; k < FEW; k++) M = fmaxf(M, mk[k]);
+#pragma unroll
+                for (int k = 0; k < FEW; k++) {
+                    const float f = mk[k] == -INFINITY ? (lk[k] != lk[k] ? lk[k] : 0.0f) : pow2(mk[k] - M);
+                    L += lk[k] * f;
+                    O.x += v[k].x * f; O.y += v[k].y * f; O.z += v[k].z * f; O.w += v[k].w * f;
+                }
+                finish(c, d, M, L, O);
+            }
+            if (tid == 0) a.cnt[c0] = 0;
+            continue;
+        }
+        float* const wts = reinterpret_cast<float*>(sm.ring);      // [n_rec][COLS]
+        float* const red = reinterpret_cast<float*>(sm.q);         // [2][threads]
+        static_assert(sizeof(sm.q) >= 2 * WARPS * 32 * 4 && sizeof(sm.ring) >= (size_t)2 * MAX_CTAS / NT * COLS * 4, "");
+        constexpr int PER = WARPS * 32 / COLS;                     // threads of a column
+        const int my_c = tid % COLS;
+        float most = -INFINITY;
+        for (int k = tid / COLS; k < n_rec; k += PER) {
+            const float* r = record(k) + 16 * 128 + my_c;
+            const float mk = __ldcg(r), lk = __ldcg(r + 16);
+            wts[2 * (k * COLS + my_c)] = mk;
+            wts[2 * (k * COLS + my_c) + 1] = lk;
+            most = fmaxf(most, mk);
+        }
+        red[tid] = most;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PER; i++) most = fmaxf(most, red[i * COLS + my_c]);
+        float sum = 0.0f;
+        for (int k = tid / COLS; k < n_rec; k += PER) {
+            const float mk = wts[2 * (k * COLS + my_c)], lk = wts[2 * (k * COLS + my_c) + 1];
+            const float f = mk == -INFINITY ? (lk != lk ? lk : 0.0f) : pow2(mk - most);
+            wts[2 * (k * COLS + my_c)] = f;
+            sum += lk * f;
+        }
+        red[WARPS * 32 + tid] = sum;
+        __syncthreads();
         for (int x = tid; x < COLS * (HDP / 4); x += WARPS * 32) {
             const int c = x / (HDP / 4), d = 4 * (x % (HDP / 4));
-            const int cc = cb * COLS + c, row = cc / a.group, h = kvh * a.group + cc % a.group;
-            if (row >= sp.n || d >= hd) continue;
-            float M = -INFINITY;
-            for (int k = c0; k <= c1; k++) {
-                const float* r = a.rec + ((size_t)2 * k + (k == c0 && item0 >= k * chunk ? 1 : 0)) * ATTN_RECORD;
-                M = fmaxf(M, __ldcg(r + 16 * 128 + c));
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                M = fmaxf(M, red[i * COLS + c]);
+                L += red[WARPS * 32 + i * COLS + c];
             }
-            float L = 0.0f;
             float4 O = make_float4(0, 0, 0, 0);
-            for (int k = c0; k <= c1; k++) {
-                const float* r = a.rec + ((size_t)2 * k + (k == c0 && item0 >= k * chunk ? 1 : 0)) * ATTN_RECORD;
-                const float mk = __ldcg(r + 16 * 128 + c), lk = __ldcg(r + 16 * 129 + c);
-                const float4 v = __ldcg((const float4*)(r + c * 128 + d));
-                const float f = mk == -INFINITY ? (lk != lk ? lk : 0.0f) : pow2(mk - M);
-                L += lk * f;
+#pragma unroll 16
+            for (int k = 0; k < n_rec; k++) {
+                const float4 v = __ldcg((const float4*)(record(k) + c * 128 + d));
+                const float f = wts[2 * (k * COLS + c)];
                 O.x += v.x * f; O.y += v.y * f; O.z += v.z * f; O.w += v.w * f;
             }
-            if (a.sinks) L += M == -INFINITY ? 1.0f : pow2(a.sinks[h] * LOG2E - M + SHIFT);
-            const float inv = 1.0f / L;
-            *(float4*)(a.out + ((size_t)s * a.rows + row) * a.n_heads * hd + (size_t)h * hd + d) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+            finish(c, d, M, L, O);
         }
         if (tid == 0) a.cnt[c0] = 0;
     }
@@ -760,7 +860,8 @@ template <int KIND, int HDP, bool EXACT, int NT> int launch_attn(fk_ctx* ctx, cu
     const long long entries = (long long)a.n_cb * a.n_seqs;
     if (entries * a.n_kv > 0x7fffffffLL) return fk_fail(FK_UNSUPPORTED, "attention_paged: %d rows of %d sequences", a.rows, a.n_seqs);
     a.whole = entries > MAX_ENTRIES;
-    const unsigned grid = a.whole ? (unsigned)(entries * a.n_kv) : (unsigned)(per_sm * ctx->sm_count);
+    const int ctas = per_sm * ctx->sm_count;
+    const unsigned grid = a.whole ? (unsigned)(entries * a.n_kv) : (unsigned)(ctas < MAX_CTAS / NT ? ctas : MAX_CTAS / NT);
     FK_CUDA(launch(kern, dim3(grid), dim3(WARPS * 32), smem, st, a), FK_LAUNCH);
     return FK_OK;
 }
