@@ -39,6 +39,7 @@ class DecoderConfig:
     oai: bool = False           # gpt-oss layers: biased projections, biased experts with the clamped SwiGLU, router bias
     sliding_window: int = 0     # gpt-oss: > 0 = windowed layers see only this many most recent keys
     swa_period: int = 0         # which layers are windowed: all (0), or layer i with i % period < period - 1 (gpt-oss: 2)
+    first_tokens: int = 0       # windowed layers also see this many tokens at a sequence's start (paged caches only)
 
     def window_of(self, layer):
         if self.sliding_window <= 0:
@@ -140,6 +141,116 @@ class _Merged:
             outs.append(y[:, o:o + r] if x.shape[0] == 1 else y[:, o:o + r].contiguous())
             o += r
         return outs
+
+
+class LogitRules:
+    """What a server does to n sequences' logits before it takes the largest: penalties (repeat, frequency, presence; one triple,
+    or [n, 3]) for the `last` most recent tokens, a bias [vocab] or [n, vocab], and a grammar's mask of int32 words (bit v % 32
+    of word v / 32 set: token v may follow), one row or [n, words].  bias and mask may be rewritten in place between steps, of a
+    captured step too.  A sequence that nothing may follow gets token -1."""
+
+    def __init__(self, n, penalties=(1.0, 0.0, 0.0), last=64, bias=None, mask=None, device="cuda"):
+        if last < 1:
+            raise ValueError("the history holds at least one token")
+        pen = torch.as_tensor(penalties, dtype=torch.float32)
+        if pen.shape not in ((3,), (n, 3)):
+            raise ValueError(f"penalties are (repeat, frequency, presence) or [{n}, 3]")
+        self.n, self.last, self.bias, self.mask = n, last, bias, mask
+        self.penalties = pen.expand(n, 3).contiguous().to(device)
+        self.history = torch.full((n, last), -1, dtype=torch.int32, device=device)
+        self.at = torch.zeros(n, dtype=torch.int64, device=device)
+
+    def see(self, row, ids):
+        """Tokens that row's sequence begins with (a prompt): only the most recent ones stay."""
+        ids = ids.reshape(-1)[-self.last:].to(torch.int32)
+        where = (self.at[row] + torch.arange(ids.numel(), device=ids.device)) % self.last
+        self.history[row, where] = ids
+        self.at[row] += ids.numel()
+
+    def forget(self, row):
+        self.history[row] = -1
+        self.at[row] = 0
+
+    def copy(self, src, dst):
+        """Row dst goes on from row src (a forked sequence)."""
+        self.history[dst] = self.history[src]
+        self.at[dst] = self.at[src]
+
+    def _row(self, t, row):
+        return t if t is None or t.dim() == 1 else t[row:row + 1]
+
+    def pick(self, ops, logits, row=None):
+        """logits [n, vocab] (or row's alone) -> tokens, which join the histories."""
+        if row is None:
+            h, at, pen, bias, mask = self.history, self.at, self.penalties, self.bias, self.mask
+        else:
+            h, at, pen = self.history[row:row + 1], self.at[row:row + 1], self.penalties[row:row + 1]
+            bias, mask = self._row(self.bias, row), self._row(self.mask, row)
+        _, tok = ops.logit_rules(logits, history=h, penalties=pen, bias=bias, mask=mask)
+        h.scatter_(1, (at % self.last)[:, None], tok[:, None])
+        at.add_(1)
+        return tok
+
+
+class _PoolMirror:
+    """The host's account of a page pool, by which a call that would not fit is refused before anything is launched.  Pages are
+    counted, not named: which ones a sequence gets is the device's affair."""
+
+    def __init__(self, n_seqs, n_pages, page, max_pages):
+        self.page, self.n_pages, self.max_pages = page, n_pages, max_pages
+        self.lens, self.held, self.refs, self._next = [0] * n_seqs, [[] for _ in range(n_seqs)], {}, 0
+
+    def save(self):
+        return list(self.lens), [list(h) for h in self.held], dict(self.refs), self._next
+
+    def restore(self, saved):
+        lens, held, refs, self._next = saved
+        self.lens, self.held, self.refs = list(lens), [list(h) for h in held], dict(refs)
+
+    def _take(self):
+        self._next += 1
+        self.refs[self._next] = 1
+        return self._next
+
+    def _room(self, need):
+        if need > self.n_pages - len(self.refs):
+            raise ValueError(f"{need} pages are needed and {self.n_pages - len(self.refs)} of {self.n_pages} are free")
+
+    def grow(self, n):
+        want = [-(-(l + a) // self.page) if a else len(h) for l, a, h in zip(self.lens, n, self.held)]
+        for s, w in enumerate(want):
+            if w > self.max_pages:
+                raise ValueError(f"sequence {s} would hold {self.lens[s] + n[s]} tokens: its table row has {self.max_pages} pages of {self.page}")
+        self._room(sum(max(0, w - len(h)) for w, h in zip(want, self.held)))
+        for h, w in zip(self.held, want):
+            while len(h) < w:
+                h.append(self._take())
+
+    def advance(self, n):
+        self.lens = [l + a for l, a in zip(self.lens, n)]
+
+    def free(self, seqs):
+        for s in seqs:
+            for p in self.held[s]:
+                self.refs[p] -= 1
+                if not self.refs[p]:
+                    del self.refs[p]
+            self.held[s], self.lens[s] = [], 0
+
+    def fork(self, src, dst, n):
+        for a, b, k in zip(src, dst, n):
+            if self.held[b]:
+                raise ValueError(f"sequence {b} holds {self.lens[b]} tokens: free it first")
+            if not 0 <= k <= self.lens[a]:
+                raise ValueError(f"{k} tokens of sequence {a}, which holds {self.lens[a]}")
+        self._room(sum(k % self.page != 0 for k in n))
+        for a, b, k in zip(src, dst, n):
+            self.held[b] = self.held[a][:k // self.page]
+            for p in self.held[b]:
+                self.refs[p] += 1
+            if k % self.page:
+                self.held[b].append(self._take())
+            self.lens[b] = k
 
 
 class Decoder:
@@ -257,15 +368,39 @@ class Decoder:
 
     # ---- one forward over n rows (token ids on the device); returns logits of the last row
     def forward(self, ids):
-        ops, cfg = self.ops, self.cfg
-        hd = cfg.head_dim
         n = ids.numel()
+        self._no_first_tokens()
         self._claim(n)
-        if n <= 8 and hasattr(ops, "gemv_fused") and (self.t_dense == 1 or self.comm is not None):
+        if self._fuses(n):
             return self._forward_fused(ids)
+        logits = self._forward_wide(ids)
+        self.ops.add_int_(self.pos, n)
+        return logits
+
+    def _fuses(self, n):
+        return n <= 8 and hasattr(self.ops, "gemv_fused") and (self.t_dense == 1 or self.comm is not None)
+
+    def _no_first_tokens(self):
+        if self.cfg.first_tokens and self.cfg.sliding_window:
+            raise ValueError("first tokens that stay visible under a window need the paged cache (alloc_pages)")
+
+    def _attend_paged(self, li, L, q, k, v, paged):
+        """Rotation, append and attention of one layer over the pages: paged = (pages or one sequence of them, rows' counts)."""
+        ops, cfg, (pg, n_new) = self.ops, self.cfg, paged
+        r = ops.rope_kv_paged(q, k, v, pg, li, self.h_loc, cfg.rope_theta, neox=cfg.neox, n_new=n_new, q_norm=L.get("q_norm"), k_norm=L.get("k_norm"),
+                              eps=cfg.eps)
+        # a row that is not there is left as it is: zeros, so that what the layers make of it stays finite
+        out = None if n_new is None or self._all_live else torch.zeros_like(r)
+        return ops.attention_paged(r, pg, li, self.h_loc, n_new=n_new, window=L["window"], first=cfg.first_tokens if L["window"] else 0, sinks=L["sinks"],
+                                   out=out)
+
+    def _forward_wide(self, ids, paged=None, all_rows=False):
+        """The form of many rows (GEMMs, norms and activations as launches of their own)."""
+        ops, cfg = self.ops, self.cfg
+        hd, n = cfg.head_dim, ids.numel()
         x = ops.get_rows(self.embd, ids)                    # residual stream [n, hidden]
         pending = None                                      # a block output not yet added to x
-        for L in self.layers:
+        for li, L in enumerate(self.layers):
             h = ops.rmsnorm(x, L["attn_norm"], cfg.eps, residual=pending)
             if "qkv" in L:
                 q, k, v = L["qkv"](h)
@@ -275,17 +410,20 @@ class Decoder:
                 q, k, v = L["wq"](h), L["wk"](h), L["wv"](h)
             if "bq" in L:
                 q, k, v = (ops.add_bias_(t_.contiguous(), L[b_]) for t_, b_ in ((q, "bq"), (k, "bk"), (v, "bv")))
-            if cfg.qk_norm:
-                q = ops.rmsnorm(q.view(-1, hd), L["q_norm"], cfg.eps).view(n, -1)
-                k = ops.rmsnorm(k.view(-1, hd), L["k_norm"], cfg.eps).view(n, -1)
-            if hasattr(ops, "rope_kv"):
-                ops.rope_kv(q, k, v, self.h_loc, self.kv_loc, hd, self.pos, cfg.rope_theta, cfg.neox, L["k"], L["v"])
+            if paged is not None:
+                a = self._attend_paged(li, L, q, k, v, paged)
             else:
-                ops.rope(q, self.h_loc, hd, self.pos, cfg.rope_theta, cfg.neox)
-                ops.rope(k, self.kv_loc, hd, self.pos, cfg.rope_theta, cfg.neox)
-                ops.kv_append(L["k"], k, self.pos)
-                ops.kv_append(L["v"], v, self.pos)
-            a = ops.attention(q, L["k"], L["v"], self.h_loc, self.kv_loc, hd, self.pos, window=L["window"], sinks=L["sinks"])
+                if cfg.qk_norm:
+                    q = ops.rmsnorm(q.view(-1, hd), L["q_norm"], cfg.eps).view(n, -1)
+                    k = ops.rmsnorm(k.view(-1, hd), L["k_norm"], cfg.eps).view(n, -1)
+                if hasattr(ops, "rope_kv"):
+                    ops.rope_kv(q, k, v, self.h_loc, self.kv_loc, hd, self.pos, cfg.rope_theta, cfg.neox, L["k"], L["v"])
+                else:
+                    ops.rope(q, self.h_loc, hd, self.pos, cfg.rope_theta, cfg.neox)
+                    ops.rope(k, self.kv_loc, hd, self.pos, cfg.rope_theta, cfg.neox)
+                    ops.kv_append(L["k"], k, self.pos)
+                    ops.kv_append(L["v"], v, self.pos)
+                a = ops.attention(q, L["k"], L["v"], self.h_loc, self.kv_loc, hd, self.pos, window=L["window"], sinks=L["sinks"])
             o = L["wo"](a)
             if "bo" in L:
                 ops.add_bias_(o, L["bo"])
@@ -299,11 +437,12 @@ class Decoder:
             else:
                 g_, u_ = L["gate_up"](h2) if "gate_up" in L else (L["gate"](h2), L["up"](h2))
                 pending = L["down"](ops.glu(g_.contiguous(), u_.contiguous(), 0))
+        if all_rows:
+            hn = ops.rmsnorm(x, self.out_norm, cfg.eps, residual=pending)
+            return ops.gemv(self.head, hn) if n <= 8 else ops.gemm(self.head, hn)
         last = x[n - 1:n].contiguous()
         hn = ops.rmsnorm(last, self.out_norm, cfg.eps, residual=pending[n - 1:n].contiguous())
-        logits = ops.gemv(self.head, hn)
-        ops.add_int_(self.pos, n)
-        return logits
+        return ops.gemv(self.head, hn)
 
     # ---- batched decode: several independent sequences, one token each per step
     def alloc_seqs(self, n_seqs):
@@ -337,6 +476,7 @@ class Decoder:
     def forward_seqs(self, toks):
         """toks [n_seqs] (device int32), sequence r's newest token -> logits [n_seqs, vocab]; every position advances."""
         n = toks.numel()
+        self._no_first_tokens()
         if n != len(self._seq_pos_host):
             raise ValueError(f"{n} tokens for {len(self._seq_pos_host)} sequences")
         if max(self._seq_pos_host) + 1 > self.max_seq:
@@ -368,7 +508,133 @@ class Decoder:
         self._seq_pos_host = [p + 1 for p in self._seq_pos_host]
         self._graph_seqs.replay()
 
-    def _forward_fused(self, ids, seqs=False):
+    # ---- many sequences over a paged cache
+    def alloc_pages(self, n_seqs, n_pages, page=16, dtype=torch.bfloat16, max_tokens=None):
+        """A cache of n_pages pages (all layers') for n_seqs sequences of up to max_tokens (default: max_seq) tokens each.  Any
+        number of sequences may share it and one another's prefixes; what does not fit is refused before anything is launched."""
+        cfg = self.cfg
+        max_pages = -(-(self.max_seq if max_tokens is None else max_tokens) // page)
+        self.pages = self.ops.Pages.alloc(cfg.n_layers, n_pages, page, self.kv_loc, cfg.head_dim, n_seqs, max_pages, dtype=dtype, device=self.dev)
+        self._page_seq = [self.pages.seq(s) for s in range(n_seqs)]
+        self._pool = _PoolMirror(n_seqs, n_pages, page, max_pages)
+        self.page_live = torch.zeros(n_seqs, dtype=torch.int32, device=self.dev)       # which sequences a decode step moves
+        self._graph_pages = None
+
+    @property
+    def _all_live(self):
+        return all(self._pool.lens)
+
+    def _live(self, s, on):
+        self.page_live[s:s + 1].fill_(int(on))
+
+    def forward_pages_seq(self, s, ids):
+        """More tokens of sequence s (a prompt, or its next chunk) -> logits of the last one [1, vocab]."""
+        n = ids.numel()
+        add = [n if i == s else 0 for i in range(len(self._pool.lens))]
+        self._pool.grow(add)
+        pg = self._page_seq[s]
+        self.ops.pages_grow(pg, n)
+        paged = (pg, None)
+        logits = self._forward_fused(ids, paged=paged) if self._fuses(n) else self._forward_wide(ids, paged=paged)
+        self.ops.pages_advance(pg, n)
+        self._pool.advance(add)
+        self._live(s, True)
+        return logits
+
+    def prefill_pages(self, s, prompt_ids, rules=None):
+        """Sequence s's prompt -> its first generated token (device int32 [1])."""
+        logits = self.forward_pages_seq(s, prompt_ids)
+        if rules is None:
+            return self.ops.argmax(logits)
+        rules.see(s, prompt_ids)
+        return rules.pick(self.ops, logits, row=s)
+
+    def forward_pages(self, toks):
+        """toks [n_seqs] (device int32), every sequence's newest token -> logits [n_seqs, vocab]; the sequences that hold
+        something move on by one, the other rows mean nothing."""
+        n = toks.numel()
+        if n != len(self._pool.lens):
+            raise ValueError(f"{n} tokens for {len(self._pool.lens)} sequences")
+        add = [int(l > 0) for l in self._pool.lens]
+        self._pool.grow(add)
+        logits = self._forward_pages_device(toks)
+        self._pool.advance(add)
+        return logits
+
+    def _forward_pages_device(self, toks):
+        ops, paged = self.ops, (self.pages, self.page_live)
+        ops.pages_grow(self.pages, self.page_live)
+        n = toks.numel()
+        logits = self._forward_fused(toks, paged=paged, all_rows=True) if self._fuses(n) else self._forward_wide(toks, paged=paged, all_rows=True)
+        ops.pages_advance(self.pages, self.page_live)
+        return logits
+
+    def _pick(self, logits, rules):
+        if rules is not None:
+            return rules.pick(self.ops, logits)
+        return torch.cat([self.ops.argmax(logits[i:i + 64]) for i in range(0, logits.shape[0], 64)])
+
+    def step_pages(self, toks, rules=None):
+        """`forward_pages` and the next tokens [n_seqs]: the largest logits, after the rules if there are any."""
+        return self._pick(self.forward_pages(toks), rules)
+
+    def capture_pages(self, toks, rules=None):
+        """`step_pages` captured in a CUDA graph (reads `toks`; returns the graph and the next tokens).  The graph grows the
+        sequences by itself and leaves out those that have been freed since: replay it with `replay_pages`."""
+        pg, saved = self.pages, self._pool.save()
+        kept = [t.clone() for t in (pg.table, pg.lens, pg.refs)] + ([rules.history.clone(), rules.at.clone()] if rules is not None else [])
+        state = [pg.table, pg.lens, pg.refs] + ([rules.history, rules.at] if rules is not None else [])
+
+        def back():
+            for t, k in zip(state, kept):
+                t.copy_(k)
+            self._pool.restore(saved)
+
+        for _ in range(2):                      # warm up outside the capture, then put everything back
+            self.step_pages(toks, rules)
+        back()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = self._pick(self._forward_pages_device(toks), rules)
+        self._graph_pages = g
+        return g, out
+
+    def replay_pages(self):
+        """One more step of the captured graph; the host's account moves with it."""
+        add = [int(l > 0) for l in self._pool.lens]
+        self._pool.grow(add)
+        self._graph_pages.replay()
+        self._pool.advance(add)
+
+    def fork_pages(self, src, dst, n=None):
+        """Sequence dst[i] (empty) becomes the first n[i] (default: all) tokens of src[i]; whole pages are shared."""
+        src, dst = list(src), list(dst)
+        n = [self._pool.lens[a] if n is None or n[i] is None else n[i] for i, a in enumerate(src)]
+        if len(set(dst)) != len(dst) or set(dst) & set(src):
+            raise ValueError("a sequence is forked into once, and is not a source of the same call")
+        self._pool.fork(src, dst, n)
+        for i in range(0, len(src), 64):
+            self.ops.pages_fork(self.pages, src[i:i + 64], dst[i:i + 64], n[i:i + 64])
+        for b, k in zip(dst, n):
+            self._live(b, k > 0)
+
+    def free_pages(self, seqs):
+        """The sequences give their pages back; a decode step leaves them out."""
+        seqs = list(seqs)
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence is freed once")
+        self._pool.free(seqs)
+        for i in range(0, len(seqs), 64):
+            self.ops.pages_free(self.pages, seqs[i:i + 64])
+        for s in seqs:
+            self._live(s, False)
+
+    def compact_pages(self):
+        """Moves the pages in use to the front of the pool -> their number (device int32 [1])."""
+        return self.ops.pages_compact(self.pages)
+
+    def _forward_fused(self, ids, seqs=False, paged=None, all_rows=False):
         """The decode form (at most 8 rows): each RMSNorm rides in the prologue of the matvec that
         reads it, SiLU(gate) * up in the prologue of the down projection, and wo / down add
         straight into the residual stream; q, k, v stay column slices of the merged projection's
@@ -389,7 +655,7 @@ class Decoder:
         hd, n = cfg.head_dim, ids.numel()
         hq, kvw = self.h_loc * hd, self.kv_loc * hd
         x = ops.get_rows(self.embd, ids)
-        for L in self.layers:
+        for li, L in enumerate(self.layers):
             def normed(name, bias=None):
                 # the attention norm rides in the prologue of every projection that reads it, a gpt-oss bias row in its epilogue
                 kw = {} if L.get(bias) is None else {"bias": L[bias]}
@@ -405,7 +671,9 @@ class Decoder:
             else:
                 q, k, v = normed("wq", "bq"), normed("wk", "bk"), normed("wv", "bv")
             window = getattr(L["wo"], "window", None)
-            if seqs:
+            if paged is not None:
+                a = self._attend_paged(li, L, q, k, v, paged)
+            elif seqs:
                 a = ops.attention_rope_kv_seqs(q, k, v, L["ks"], L["vs"], self.h_loc, self.kv_loc, hd, self.seq_pos, cfg.rope_theta, cfg.neox,
                                                q_norm=L.get("q_norm"), k_norm=L.get("k_norm"), eps=cfg.eps, window=L["window"], sinks=L["sinks"])
             elif n == 1 and hasattr(ops, "attention_rope_kv") and window is not None:
@@ -459,8 +727,11 @@ class Decoder:
             logits = ops.gemv_fused(self.head, x, norm_weight=self.out_norm, eps=cfg.eps)
             self.seq_pos.add_(1)
             return logits
+        if all_rows:
+            return ops.gemv_fused(self.head, x, norm_weight=self.out_norm, eps=cfg.eps)
         logits = ops.gemv_fused(self.head, x[n - 1:n], norm_weight=self.out_norm, eps=cfg.eps)
-        ops.add_int_(self.pos, n)
+        if paged is None:
+            ops.add_int_(self.pos, n)
         return logits
 
     def _ep_prefill(self, ep, h2):
@@ -499,8 +770,19 @@ class Decoder:
         self._claim(1)
         self._graph.replay()
 
-    def generate(self, prompt_ids, n_new, use_graph=False):
-        """Greedy: returns the n_new generated token ids (list of int)."""
+    def generate(self, prompt_ids, n_new, use_graph=False, rules=None):
+        """Greedy: returns the n_new generated token ids (list of int).  rules (`LogitRules` of one sequence): what happens to the
+        logits first; the token is then -1 where nothing may follow, and generation ends there."""
+        if rules is not None:
+            if use_graph:
+                raise ValueError("rules run eagerly here; a captured step with rules is capture_pages'")
+            rules.see(0, prompt_ids)
+            tok = rules.pick(self.ops, self.forward(prompt_ids))
+            outs = [int(tok.item())]
+            while len(outs) < n_new and outs[-1] >= 0:
+                tok = rules.pick(self.ops, self.forward(tok))
+                outs.append(int(tok.item()))
+            return outs
         tok = self.prefill(prompt_ids)
         outs = [tok.clone()]
         if use_graph and n_new > 1:
