@@ -1,4 +1,4 @@
-// Attention of a prompt's rows over a paged KV cache on the tensor cores (tcgen05): 16-bit pages, heads of 64 or 128.  The
+// Attention of a prompt's rows over a paged KV cache on the tensor cores (tcgen05): 16-bit pages, heads of up to 128.  The
 // mathematics, the masks and the precision are those of fk_attn_paged.cu.
 //
 // A CTA takes 128 (row, query head) pairs of one KV head -- 128 / group consecutive rows, so a short prompt still fills the
@@ -14,9 +14,11 @@
 // products: the bound is the tensor cores' rate by that factor.  Per tile of 64 keys and 128 dims that is 1536 (1024) cycles of
 // MMA against 512 of exponentials and some 700 issue slots a scheduler for the parts and the running output.
 //
-// Warps 0 to 3 and 4 to 7 are two softmax groups that take turns: a thread has a row and all 64 keys of its group's tile, in two
-// halves, so nothing is exchanged inside a group, and between them only the row's maximum passes -- early in a tile, so that one
-// group's exponentials run beside the other's.  8 to 15 keep the running output, a thread per row and half of the dims.  16 loads
+// Warps 0 to 7 are the softmax: a thread has a row and half of the tile's keys, and the halves exchange the row's maximum.
+// (Two groups that take turns with a tile each need no exchange, but a tile is then twice as long between its scores and its
+// weights, and that chain bounds the kernel: 4200 rows of 24/8 heads of 128, bf16, 398 us that way, 326 us this way = 332 TFLOP/s
+// of the formula's operations, three times that of MMA.)  8 to 15 keep the running output, a thread per row and half of the
+// dims.  16 loads
 // tiles (a lane per page piece, TMA with 128-byte swizzle).  17 issues the products for S and 19 those for O, so that scores are
 // made as soon as their buffer is free and not in turn with products that wait for weights.  18 looks over the values of tiles
 // that not every row sees: a value that no row sees is zeroed in shared memory (stale memory may hold NaN); one that some rows
@@ -45,15 +47,15 @@ struct PromptArgs {
     float* out;
     int* err;
     float scale;
-    int q_ld, rows, n_seqs, n_heads, n_kv, group, page, log_page, n_pages, max_pages, window, first, rq, n_rb;
+    int q_ld, rows, n_seqs, n_heads, n_kv, group, head_dim, page, log_page, n_pages, max_pages, window, first, rq, n_rb;
 };
 
 template <int KIND, int HD> struct Plan {
     static constexpr int QP = KIND == KIND_F16 ? 2 : 3;            // parts of q and of the weights
     static constexpr int TILE = KT * HD * 2;                       // bytes of a tile of K or V
     static constexpr int STAGES = HD == 64 ? 6 : 4;
-    // warps: NG softmax groups of 4, 8 of the running output, then the four single ones
-    static constexpr int NG = 2, OUT = 4 * NG, LOADER = OUT + 8, ISSUER_S = LOADER + 1, LOOKER = LOADER + 2, ISSUER_O = LOADER + 3;
+    // warps: 8 of the softmax, 8 of the running output, then the four single ones
+    static constexpr int OUT = 8, LOADER = 16, ISSUER_S = 17, LOOKER = 18, ISSUER_O = 19;
     static constexpr int THREADS = 32 * (LOADER + 4);
     // Tensor memory columns of a tile: S's 64 behind LEAD free ones; the parts of w's first half of the keys take the free ones
     // and S's first half, those of its second half what follows, so that S is never overwritten before it is read.
@@ -70,14 +72,15 @@ template <int KIND, int HD> struct PromptSmem {
     using P = Plan<KIND, HD>;
     unsigned char k[P::STAGES][P::TILE];
     unsigned char v[P::STAGES][P::TILE];
-    float odd_w[P::NG][KT][128];                   // per softmax group: weights of a tile's values that are not finite, by row (-1: not seen)
-    float top[P::NG][128];                         // a row's maximum after the group's last tile; before that, of q's halves
+    float stage[128 * HD];                     // rows of q and of the output on their way; between them the weights of a tile's values
+                                               // that are not finite, [key][row] (-1: the row does not see it)
+    float top[2][2][128];                      // a row's maximum over each half of the tile's keys, two tiles' worth
     float corr[8][128];                        // what the running output is multiplied with at the tile (mod 8)
-    float fin[P::NG][2][128];                      // per softmax group: denominator and the maximum it refers to
+    float fin[2][2][128];                      // denominator of each half's keys and the maximum (the same for both)
     unsigned long long odd_of[8];              // which of the tile's values are not finite (mod 8)
     unsigned long long odd[P::STAGES];         // the same, where the values lie
     unsigned long long kfull[P::STAGES], kfree[P::STAGES], vfull[P::STAGES], vfree[P::STAGES], vready[P::STAGES];
-    unsigned long long sfull[P::NS], pfull[P::NS], mfull[P::NG][4], oddfree[P::NG], ofull[P::NO], ofree[P::NO], qfull, done[2];
+    unsigned long long sfull[P::NS], pfull[P::NS], oddfree, ofull[P::NO], ofree[P::NO], qfull, done[2];
     uint32_t tmem;
     int abort;
 };
@@ -142,11 +145,11 @@ template <int N> __device__ __forceinline__ void tm_ld(uint32_t addr, float* v) 
 template <int KIND, int HD>
 __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kernel(const __grid_constant__ PromptArgs a) {
     using P = Plan<KIND, HD>;
-    constexpr int QP = P::QP, STAGES = P::STAGES, NS = P::NS, NO = P::NO, NG = P::NG, HALF = HD / 2;
+    constexpr int QP = P::QP, STAGES = P::STAGES, NS = P::NS, NO = P::NO, HALF = HD / 2;
     constexpr float SHIFT = KIND == KIND_F16 ? 14.0f : 0.0f;
     extern __shared__ unsigned char smem_raw[];
     PromptSmem<KIND, HD>& sm = *reinterpret_cast<PromptSmem<KIND, HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), hd = a.head_dim;
     if (tid == 0) {
         for (int i = 0; i < STAGES; i++) {
             mbar_init(smem_u32(&sm.kfull[i]), 1);
@@ -157,10 +160,9 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
         }
         for (int i = 0; i < NS; i++) {
             mbar_init(smem_u32(&sm.sfull[i]), 1);
-            mbar_init(smem_u32(&sm.pfull[i]), 4);
+            mbar_init(smem_u32(&sm.pfull[i]), 8);
         }
-        for (int i = 0; i < 4 * NG; i++) mbar_init(smem_u32(&sm.mfull[i >> 2][i & 3]), 1);
-        for (int i = 0; i < NG; i++) mbar_init(smem_u32(&sm.oddfree[i]), 8);
+        mbar_init(smem_u32(&sm.oddfree), 8);
         for (int i = 0; i < NO; i++) {
             mbar_init(smem_u32(&sm.ofull[i]), 1);
             mbar_init(smem_u32(&sm.ofree[i]), 8);
@@ -364,25 +366,26 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
             if (lane == 0) mbar_arrive(smem_u32(&sm.vready[st]));
         }
     } else {
-        const int w = warp < P::OUT ? warp >> 2 : (warp - P::OUT) >> 2, r = (warp & 3) * 32 + lane;       // softmax group, or half of the dims; row of the 128
+        const int w = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;      // half of the tile's keys, or of the dims; row of the 128
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const int row = row0 + r / a.group, h = kvh * a.group + r % a.group;
         const bool on = r < a.rq * a.group && row <= row1;
         const int p = on ? base + row : -1;
         // q's rows through shared memory (where odd weights will lie): read row by row, taken back a row a thread.  Piece c of row i
         // lies at c ^ i, so that neither side meets a bank twice.
-        float4* const stage = reinterpret_cast<float4*>(sm.odd_w);
+        float4* const stage = reinterpret_cast<float4*>(sm.stage);
+        float* const odd_w = sm.stage;
         constexpr int ROW4 = HD / 4, SHARE = 128 * ROW4 / 512;
         float qs = 1.0f;
-        if (tid < 512) {
+        {
             float4 y[SHARE];
             const uint32_t inv = (65535 + a.group) / a.group;      // i / group = i inv / 2^16 below 128
 #pragma unroll
             for (int u = 0; u < SHARE; u++) {
                 const int x = u * 512 + tid, i = x / ROW4, ig = (int)(i * inv >> 16), ri = row0 + ig;
                 y[u] = make_float4(0, 0, 0, 0);
-                if (i < a.rq * a.group && ri <= row1)
-                    y[u] = *(const float4*)(a.q + ((size_t)s * a.rows + ri) * a.q_ld + (size_t)(kvh * a.group + i - ig * a.group) * HD + 4 * (x % ROW4));
+                if (i < a.rq * a.group && ri <= row1 && 4 * (x % ROW4) < hd)
+                    y[u] = *(const float4*)(a.q + ((size_t)s * a.rows + ri) * a.q_ld + (size_t)(kvh * a.group + i - ig * a.group) * hd + 4 * (x % ROW4));
             }
 #pragma unroll
             for (int u = 0; u < SHARE; u++) {
@@ -390,11 +393,11 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                 stage[i * ROW4 + ((x % ROW4) ^ (i & (ROW4 - 1)))] = y[u];
             }
         }
-        asm volatile("bar.sync 2, %0;" ::"n"(32 * P::LOADER) : "memory");
+        asm volatile("bar.sync 2, 512;" ::: "memory");
         {
             // a quarter of a row a thread: scaled, split, into tensor memory part by part
             constexpr int QUARTER = HD / 4;
-            const int qt = (warp >> 2) & 3;                        // groups beyond 16 warps repeat a quarter and keep it to themselves
+            const int qt = warp >> 2;
             const float sl = a.scale * LOG2E;
             float x[QUARTER], top = 0.0f;
 #pragma unroll
@@ -406,8 +409,8 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
             }
             if (KIND == KIND_F16) {
                 float* const tops = &sm.fin[0][0][0];              // [4][128]
-                if (warp < 16) tops[qt * 128 + r] = top;
-                asm volatile("bar.sync 2, %0;" ::"n"(32 * P::LOADER) : "memory");
+                tops[qt * 128 + r] = top;
+                asm volatile("bar.sync 2, 512;" ::: "memory");
                 top = fmaxf(fmaxf(tops[r], tops[128 + r]), fmaxf(tops[256 + r], tops[384 + r]));
                 // 2^e with top * 2^e in [2^13, 2^14)
                 int ex = top > 0.0f && top < INFINITY ? 13 - (int)((__float_as_uint(top) >> 23) & 255) + 127 : 0;
@@ -417,97 +420,81 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                 for (int d = 0; d < QUARTER; d++) x[d] *= f;
                 qs = __uint_as_float((uint32_t)(127 - ex) << 23);
             }
-            if (warp < 16) {
 #pragma unroll
-                for (int k = 0; k < QP; k++) {
-                    uint32_t pk[QUARTER / 2];
+            for (int k = 0; k < QP; k++) {
+                uint32_t pk[QUARTER / 2];
 #pragma unroll
-                    for (int i = 0; i < QUARTER / 2; i++) pk[i] = take_part<KIND>(x[2 * i], x[2 * i + 1]);
-                    const uint32_t at = tmem + lanes + P::Q0 + k * HALF + qt * (QUARTER / 2);
-                    if (HD == 128) tc_st16(at, pk);
-                    else tc_st8(at, pk);
-                }
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sm.qfull));
+                for (int i = 0; i < QUARTER / 2; i++) pk[i] = take_part<KIND>(x[2 * i], x[2 * i + 1]);
+                const uint32_t at = tmem + lanes + P::Q0 + k * HALF + qt * (QUARTER / 2);
+                if (HD == 128) tc_st16(at, pk);
+                else tc_st8(at, pk);
             }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.qfull));
         }
         auto sees = [&](int k) { return k <= p && (a.window <= 0 || k > p - a.window || k < a.first); };
         if (warp < P::OUT) {
             // ---- softmax
-            float m = -INFINITY, l = 0.0f;                         // the denominator of this group's tiles, relative to m
+            float m = -INFINITY, l = 0.0f;                         // the denominator of this half's keys, relative to m
             int odds = 0;
-            for (int j = w; j < n_tiles; j += NG) {
-                const int key0 = tile_key(j);
+            for (int j = 0; j < n_tiles; j++) {
+                const int b = j & 1, key0 = tile_key(j) + 32 * w;
                 wait(&sm.sfull[j % NS], (j / NS) & 1);
                 tc_fence_after();
                 const uint32_t at = tmem + lanes + P::S0 + (j % NS) * P::SREG;
-                const bool edge = edge_tile(key0);
-                const int up = p - key0, dn = a.window > 0 ? p - a.window - key0 : -1, fi = a.window > 0 ? a.first - key0 : 0;
-                auto scores = [&](int c, float* v) {               // half c of the row, what it does not see at -infinity
-                    tm_ld<32>(at + P::LEAD + c * 32, v);
-                    if (edge) {
+                const bool edge = edge_tile(tile_key(j));
+                float v[32];
+                tm_ld<32>(at + P::LEAD + w * 32, v);
+                if (edge) {
+                    const int up = p - key0, dn = a.window > 0 ? p - a.window - key0 : -1, fi = a.window > 0 ? a.first - key0 : 0;
 #pragma unroll
-                        for (int i = 0; i < 32; i++) v[i] = 32 * c + i <= up && (32 * c + i > dn || 32 * c + i < fi) ? v[i] : -INFINITY;
-                    }
-                };
-                float v[32], top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 1; c >= 0; c--) {
-                    scores(c, v);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) top[k] = fmaxf(fmaxf(top[k], v[i + k]), v[i + 4 + k]);
+                    for (int i = 0; i < 32; i++) v[i] = i <= up && (i > dn || i < fi) ? v[i] : -INFINITY;
                 }
+                float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+                for (int i = 4; i < 28; i += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) top[k] = fmaxf(fmaxf(top[k], v[i + k]), v[i + 4 + k]);
+#pragma unroll
+                for (int k = 0; k < 4; k++) top[k] = fmaxf(top[k], v[28 + k]);
                 const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * qs;
-                // the row's maximum so far comes from the group of the tile before: its warp of the same rows
-                float m_old = -INFINITY;
-                if (j > 0) {
-                    const int g = w == 0 ? NG - 1 : w - 1;
-                    wait(&sm.mfull[g][warp & 3], ((j - 1) / NG) & 1);
-                    m_old = sm.top[g][r];
-                }
-                const float m_new = fmaxf(m_old, t), ms = m_new == -INFINITY ? 0.0f : m_new - SHIFT;
-                sm.top[w][r] = m_new;
-                sm.corr[j & 7][r] = m_old == -INFINITY ? 0.0f : pow2f(m_old - m_new);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sm.mfull[w][warp & 3]));
-                l *= m == -INFINITY ? 1.0f : pow2f(m - m_new);
+                // the row's other half; behind the barrier both halves of S are in registers
+                sm.top[b][w][r] = t;
+                tc_fence_before();
+                asm volatile("bar.sync 3, 256;" ::: "memory");
+                tc_fence_after();
+                const float m_new = fmaxf(fmaxf(m, t), sm.top[b][1 - w][r]), ms = m_new == -INFINITY ? 0.0f : m_new - SHIFT;
+                const float c = m == -INFINITY ? 0.0f : pow2f(m - m_new);
+                if (w == 0) sm.corr[j & 7][r] = c;
                 m = m_new;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    v[i] = pow2f(fmaf(v[i], qs, -ms));
+                    sum[i & 3] += v[i];
+                }
+                l = fmaf(l, c, (sum[0] + sum[1]) + (sum[2] + sum[3]));
                 unsigned long long odd = 0;
                 if (edge) {
                     wait(&sm.vready[j % STAGES], (j / STAGES) & 1);
                     odd = __shfl_sync(0xffffffffu, sm.odd[j % STAGES], 0);
                     if (odd) {                                     // rare
-                        if (odds > 0) wait(&sm.oddfree[w], (odds - 1) & 1);
+                        if (odds > 0) wait(&sm.oddfree, (odds - 1) & 1);
                         odds++;
-                    }
-                }
-                if (r == 0) sm.odd_of[j & 7] = odd;
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    if (c) scores(c, v);                           // half 0 is still there
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        v[i] = pow2f(fmaf(v[i], qs, -ms));
-                        sum[i & 3] += v[i];
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    if (odd) {
 #pragma unroll
                         for (int i = 0; i < 32; i++)
-                            if (odd >> (32 * c + i) & 1) sm.odd_w[w][32 * c + i][r] = sees(key0 + 32 * c + i) ? v[i] : -1.0f;
+                            if (odd >> (32 * w + i) & 1) odd_w[(32 * w + i) * 128 + r] = sees(key0 + i) ? v[i] : -1.0f;
                     }
+                }
+                if (tid == 0) sm.odd_of[j & 7] = odd;
 #pragma unroll
-                    for (int k = 0; k < QP; k++) {
-                        uint32_t pk[16];
+                for (int k = 0; k < QP; k++) {
+                    uint32_t pk[16];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) pk[i] = take_part<KIND>(v[2 * i], v[2 * i + 1]);
-                        tc_st16(at + c * (QP * 16) + k * 16, pk);
-                    }
+                    for (int i = 0; i < 16; i++) pk[i] = take_part<KIND>(v[2 * i], v[2 * i + 1]);
+                    tc_st16(at + w * (QP * 16) + k * 16, pk);
                 }
                 tc_wait_st();
                 tc_fence_before();
@@ -516,7 +503,7 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
             }
             sm.fin[w][0][r] = l;
             sm.fin[w][1][r] = m;
-            asm volatile("bar.sync 2, %0;" ::"n"(32 * P::LOADER) : "memory");
+            asm volatile("bar.sync 2, 512;" ::: "memory");
         } else {
             // ---- the running output: o = o corr + O
             float o[HALF];
@@ -539,28 +526,26 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                 if (odd) {                                         // rare: values that are not finite, for the rows that see them
                     for (int i = 0; i < KT; i++) {
                         if (!(odd >> i & 1)) continue;
-                        const float wt = sm.odd_w[j % NG][i][r];
+                        const float wt = odd_w[i * 128 + r];
                         if (wt < 0.0f) continue;
                         const int k = tile_key(j) + i, pg = min(max(a.table[(size_t)s * a.max_pages + (k >> a.log_page)], 0), a.n_pages - 1);
-                        const uint16_t* vr = (const uint16_t*)a.data + ((((size_t)2 * pg + 1) * a.n_kv + kvh) * a.page + (k & (a.page - 1))) * HD + w * HALF;
+                        const uint16_t* vr = (const uint16_t*)a.data + ((((size_t)2 * pg + 1) * a.n_kv + kvh) * a.page + (k & (a.page - 1))) * hd + w * HALF;
 #pragma unroll
-                        for (int d = 0; d < HALF; d++) o[d] = fmaf(wt, KIND == KIND_F16 ? fk_h2f(vr[d]) : __uint_as_float((uint32_t)vr[d] << 16), o[d]);
+                        for (int d = 0; d < HALF; d++)
+                            if (w * HALF + d < hd) o[d] = fmaf(wt, KIND == KIND_F16 ? fk_h2f(vr[d]) : __uint_as_float((uint32_t)vr[d] << 16), o[d]);
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&sm.oddfree[j % NG]));
+                    if (lane == 0) mbar_arrive(smem_u32(&sm.oddfree));
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sm.ofree[ob]));
             }
-            // the groups' denominators, the sink, the output
-            asm volatile("bar.sync 2, %0;" ::"n"(32 * P::LOADER) : "memory");
+            // the halves' denominators, the sink, the output
+            asm volatile("bar.sync 2, 512;" ::: "memory");
             if (n_tiles > 0) {
-                float m = -INFINITY, l = 0.0f;
-#pragma unroll
-                for (int g = 0; g < NG; g++) m = fmaxf(m, sm.fin[g][1][r]);
-#pragma unroll
-                for (int g = 0; g < NG; g++) l += sm.fin[g][0][r] * (sm.fin[g][1][r] == m ? 1.0f : pow2f(sm.fin[g][1][r] - m));
+                const float m = sm.fin[0][1][r];
+                float l = sm.fin[0][0][r] + sm.fin[1][0][r];
                 if (a.sinks && on) l += m == -INFINITY ? 1.0f : pow2f(a.sinks[h] * LOG2E - m + SHIFT);
                 const float inv = 1.0f / l;
                 // through shared memory as q came, so that rows are written whole
@@ -571,8 +556,8 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
 #pragma unroll 4
                 for (int x = tid - 32 * P::OUT; x < 128 * ROW4; x += 256) {
                     const int i = x / ROW4, ig = (int)(i * ((65535u + a.group) / a.group) >> 16), ri = row0 + ig;
-                    if (i < a.rq * a.group && ri <= row1)
-                        *(float4*)(a.out + ((size_t)s * a.rows + ri) * a.n_heads * HD + (size_t)(kvh * a.group + i - ig * a.group) * HD + 4 * (x % ROW4)) =
+                    if (i < a.rq * a.group && ri <= row1 && 4 * (x % ROW4) < hd)
+                        *(float4*)(a.out + ((size_t)s * a.rows + ri) * a.n_heads * hd + (size_t)(kvh * a.group + i - ig * a.group) * hd + 4 * (x % ROW4)) =
                             stage[i * ROW4 + ((x % ROW4) ^ (i & (ROW4 - 1)))];
                 }
             }
@@ -604,9 +589,15 @@ template <int KIND, int HD> int launch_prompt(fk_ctx* ctx, cudaStream_t st, cons
 // Whether this kernel takes the call, else attn_paged_kernel does.
 bool fk_attn_prompt_takes(fk_ctx* ctx, const fk_pages* p, int rows, int n_heads) {
     const int group = n_heads / p->n_kv;
-    if (p->kind == KIND_F32 || (p->head_dim != 64 && p->head_dim != 128) || group > 128) return false;
+    if (p->kind == KIND_F32 || group > 128) return false;
     if ((long long)p->n_pages * 2 * p->n_kv * p->page > 0x7fffffffLL) return false;      // a token's row number is 32 bits
-    return (long long)rows * group >= 128;
+    // This kernel takes 23 ns an SM for a key of a tile of 128 columns, whatever of the tile is filled, and does not split the
+    // keys; the other takes 14 ns an SM for a key of 16 columns and spreads over all SMs (bf16, heads of 128; f16 heads of 64: 13
+    // and 7.6).  24/8 heads of 128, one sequence after 8000 tokens, us here / there: 64 rows 196 / 82, 128 rows 200 / 157, 256
+    // rows 209 / 299; four sequences: 24 rows 198 / 140, 43 rows 204 / 250.
+    const long long tiles = (long long)p->n_seqs * p->n_kv * ((rows + 128 / group - 1) / (128 / group));
+    const long long blocks = (long long)p->n_seqs * p->n_kv * (((long long)rows * group + 15) / 16);
+    return 3 * blocks > 5 * ctx->sm_count * ((tiles + ctx->sm_count - 1) / ctx->sm_count);
 }
 
 int fk_attn_prompt_launch(fk_ctx* ctx, cudaStream_t st, const fk_pages* p, int layer, const float* q, int q_ld, int rows, const int* n_new, int n_heads,
@@ -630,6 +621,7 @@ int fk_attn_prompt_launch(fk_ctx* ctx, cudaStream_t st, const fk_pages* p, int l
     a.n_heads = n_heads;
     a.n_kv = p->n_kv;
     a.group = n_heads / p->n_kv;
+    a.head_dim = p->head_dim;
     a.page = p->page;
     a.log_page = p->page == 16 ? 4 : p->page == 32 ? 5 : p->page == 64 ? 6 : 7;
     a.n_pages = p->n_pages;
@@ -640,6 +632,7 @@ int fk_attn_prompt_launch(fk_ctx* ctx, cudaStream_t st, const fk_pages* p, int l
     a.n_rb = (rows + a.rq - 1) / a.rq;
     const long long grid = (long long)a.n_rb * a.n_seqs * a.n_kv;
     if (grid > 0x7fffffffLL) return fk_fail(FK_UNSUPPORTED, "attention_paged: %d rows of %d sequences", rows, p->n_seqs);
-    if (p->kind == KIND_F16) return p->head_dim == 64 ? launch_prompt<KIND_F16, 64>(ctx, st, a, (unsigned)grid) : launch_prompt<KIND_F16, 128>(ctx, st, a, (unsigned)grid);
-    return p->head_dim == 64 ? launch_prompt<FK_BF16, 64>(ctx, st, a, (unsigned)grid) : launch_prompt<FK_BF16, 128>(ctx, st, a, (unsigned)grid);
+    // shorter heads are zeros behind their last dim: the tiled copy fills what lies outside its tensor
+    if (p->kind == KIND_F16) return p->head_dim <= 64 ? launch_prompt<KIND_F16, 64>(ctx, st, a, (unsigned)grid) : launch_prompt<KIND_F16, 128>(ctx, st, a, (unsigned)grid);
+    return p->head_dim <= 64 ? launch_prompt<FK_BF16, 64>(ctx, st, a, (unsigned)grid) : launch_prompt<FK_BF16, 128>(ctx, st, a, (unsigned)grid);
 }

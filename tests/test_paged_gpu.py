@@ -487,7 +487,7 @@ def attend_fast(lens, counts, rows, heads, n_kv, hd, page, dtype, window=0, firs
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("heads,n_kv,hd", [(24, 8, 128), (64, 8, 64), (8, 8, 128), (16, 1, 64), (130, 1, 64), (128, 1, 128)])
+@pytest.mark.parametrize("heads,n_kv,hd", [(24, 8, 128), (64, 8, 64), (8, 8, 128), (16, 1, 64), (130, 1, 64), (128, 1, 128), (6, 2, 80), (10, 5, 96), (12, 2, 8), (4, 1, 120)])
 @pytest.mark.parametrize("page,rows,lens,counts", [(16, 300, [0], [300]), (64, 257, [700, 3], [257, 100]), (32, 129, [0, 1000, 64], [0, 129, 128]), (128, 200, [129], [200])])
 def test_prompt(dtype, heads, n_kv, hd, page, rows, lens, counts):
     attend_fast(lens, counts, rows, heads, n_kv, hd, page, TYPES[dtype], seed=rows)
@@ -507,6 +507,7 @@ def test_prompt_values_behind_a_mask_do_not_matter(dtype, x):
     several at once."""
     attend_fast([100], [300], 300, 16, 2, 64, 16, TYPES[dtype], seed=3, bad=[(0, 390, x)])
     attend_fast([100], [300], 300, 24, 8, 128, 16, TYPES[dtype], seed=4, bad=[(0, 150, x), (0, 152, x), (0, 399, x)])
+    attend_fast([100], [300], 300, 6, 2, 80, 16, TYPES[dtype], seed=4, bad=[(0, 150, x), (0, 399, x)])
     attend_fast([500], [300], 300, 16, 2, 64, 64, TYPES[dtype], window=70, first=3, seed=5, bad=[(0, 3, x), (0, 440, x), (0, 600, x), (0, 799, x)])
 
 
