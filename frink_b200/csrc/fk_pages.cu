@@ -7,6 +7,8 @@
 // 4 bytes a page and stops at the last page it needs; what costs is the copying of page data, bound by HBM.
 #include "fk_paged.cuh"
 
+#include <cmath>
+
 using namespace fk_paged;
 
 namespace {
@@ -324,7 +326,8 @@ struct RopeArgs {
     const int *table, *lens, *n_new;
     int* err;
     int q_ld, k_ld, v_ld, rows, n_heads, n_kv, head_dim, page, n_pages, max_pages, neox;
-    float theta, eps;
+    float eps;
+    double log2_theta;
 };
 
 template <int KIND> __device__ __forceinline__ void store4(void* base, size_t at, float4 v) {
@@ -357,7 +360,7 @@ template <int KIND> __global__ void __launch_bounds__(256) rope_paged_kernel(con
     if (!held && threadIdx.x == 0) fk_raise(a.err, 97);
     __shared__ float2 cs[64];
     if (threadIdx.x < half) {
-        const double turns = (double)p * (exp2(-2.0 * threadIdx.x / hd * log2((double)a.theta)) * 0.15915494309189533577);
+        const double turns = (double)p * (exp2(-2.0 * threadIdx.x / hd * a.log2_theta) * 0.15915494309189533577);
         float sn, c;
         sincospif(2.0f * (float)(turns - rint(turns)), &sn, &c);
         cs[threadIdx.x] = make_float2(c, sn);
@@ -531,7 +534,7 @@ FK_EXPORT int fk_rope_kv_paged(fk_ctx* ctx, void* stream, const fk_pages* p, int
     if (q_out_dev == q_dev && q_ld != n_heads * p->head_dim) return fk_fail(FK_INVALID, "rope_kv_paged: q is rotated in place only where its rows are packed");
     FkDeviceGuard g(ctx->device);
     RopeArgs a{q_dev, k_dev, v_dev, q_norm_dev, k_norm_dev, q_out_dev, (char*)p->data_dev + (size_t)layer * page_bytes(p) * p->n_pages, p->table_dev, p->lens_dev,
-               n_new_dev, ctx->err_flag, q_ld, k_ld, v_ld, rows, n_heads, p->n_kv, p->head_dim, p->page, p->n_pages, p->max_pages, neox, theta, norm_eps};
+               n_new_dev, ctx->err_flag, q_ld, k_ld, v_ld, rows, n_heads, p->n_kv, p->head_dim, p->page, p->n_pages, p->max_pages, neox, norm_eps, log2((double)theta)};
     auto kern = p->kind == KIND_F32 ? rope_paged_kernel<KIND_F32> : p->kind == KIND_F16 ? rope_paged_kernel<KIND_F16> : rope_paged_kernel<FK_BF16>;
     FK_CUDA(launch(kern, dim3(rows * p->n_seqs), dim3(256), 0, (cudaStream_t)stream, a), FK_LAUNCH);
     FK_PAGED_LAUNCHED();
