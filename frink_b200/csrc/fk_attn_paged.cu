@@ -569,14 +569,13 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
             }
             copy_wait<2 * STAGES - 1>();
             __syncwarp();
-            // o += V^T w.  MODE 0: every column sees every token.  MODE 1: values whose keys no column sees become zeros, whatever
-            // they are (stale memory, NaN): they must not meet a weight of 0.  MODE 2: the columns of one row, with the values
-            // that it does not see as zeros.
-            auto fold = [&](auto mode, int p_lo, int p_hi) {
-                constexpr int MODE = decltype(mode)::value;
+            // o += V^T w.  Not PLAIN: values whose keys no row at positions p_lo to p_hi sees become zeros, whatever they are (stale
+            // memory, NaN): they must not meet a weight of 0.  The columns of all rows, or of the one at p_lo.
+            auto fold = [&](auto plain, int p_lo, int p_hi, bool all) {
+                constexpr bool PLAIN = decltype(plain)::value;
                 uint32_t keep[SUB][2];
                 bool mine[NT];
-                if (MODE) {
+                if (!PLAIN) {
 #pragma unroll
                     for (int u = 0; u < SUB; u++) {
                         keep[u][0] = keep[u][1] = 0xffffffffu;
@@ -587,10 +586,10 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
                         }
                     }
 #pragma unroll
-                    for (int n = 0; n < NT; n++) mine[n] = MODE != 2 || sp.base + (cb * COLS + n * 8 + g) / a.group == p_lo;      // the operand's column g
+                    for (int n = 0; n < NT; n++) mine[n] = all || sp.base + (cb * COLS + n * 8 + g) / a.group == p_lo;      // the operand's column g
                 }
                 auto block = [&](int d, uint32_t (&va)[SUB][KIND == KIND_F32 ? 3 : 1][4]) {
-                    if (MODE) {
+                    if (!PLAIN) {
 #pragma unroll
                         for (int u = 0; u < SUB; u++)
 #pragma unroll
@@ -605,7 +604,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
                         for (int k = QP - 1; k >= 0; k--)
 #pragma unroll
                             for (int u = 0; u < SUB; u++) {
-                                const uint32_t b0 = MODE != 2 || mine[n] ? wp[u][n][k][0] : 0u, b1 = MODE != 2 || mine[n] ? wp[u][n][k][1] : 0u;
+                                const uint32_t b0 = PLAIN || mine[n] ? wp[u][n][k][0] : 0u, b1 = PLAIN || mine[n] ? wp[u][n][k][1] : 0u;
 #pragma unroll
                                 for (int kk = (KIND == KIND_F32 ? 2 - k : 0); kk >= 0; kk--) {
                                     if (k == QP - 1 && u == 0 && kk == (KIND == KIND_F32 ? 2 - k : 0)) mma0<KIND>(x, va[u][kk], b0, b1);
@@ -658,7 +657,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
                 }
             };
             if (!edge) {
-                fold(std::integral_constant<int, 0>{}, 0, 0);
+                fold(std::true_type{}, 0, 0, true);
             } else {
                 // Values that some columns see and others do not are finite in any sane model; where one is not, the columns'
                 // rows are taken one by one.
@@ -679,9 +678,8 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
                         }
                     }
                 }
-                if (!__any_sync(0xffffffffu, odd)) fold(std::integral_constant<int, 1>{}, p_min, p_max);
-                else
-                    for (int p = p_min; p <= p_max; p++) fold(std::integral_constant<int, 2>{}, p, p);
+                const bool all = !__any_sync(0xffffffffu, odd);
+                for (int p = p_min; p <= (all ? p_min : p_max); p++) fold(std::false_type{}, p, all ? p_max : p, all);
             }
             __syncwarp();
             request(Values{}, j + STAGES, pg_next);
