@@ -13,12 +13,12 @@
 namespace {
 
 constexpr int LR_THREADS = 256, LR_PER_SM = 4, LR_MAX_BLOCKS = 64, LR_ROWS = 64;      // the workspace holds keys of 64 blocks of 64 rows
-constexpr int LR_RANGE = 24576;                 // tokens of a block at most: 48 KB of counts
+constexpr int LR_RANGE = 24480;                 // tokens of a block at most: their counts and the block's other shared memory are 48 KB
 constexpr int LR_HISTORY = 65535;               // a count's 16 bits
 
 // A key whose order is that of the values, then of descending index; 0 stands for no value.
 __device__ __forceinline__ unsigned long long key_of(float v, int i) {
-    unsigned u = __float_as_uint(v);
+    unsigned u = v == 0.0f ? 0u : __float_as_uint(v);              // zeros of both signs are equal
     u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
     return ((unsigned long long)u << 32) | (unsigned)(~i);
 }

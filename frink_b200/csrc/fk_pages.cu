@@ -74,7 +74,11 @@ grow_kernel(int* __restrict__ table, const int* __restrict__ lens, int* refs, in
     __shared__ int part[33];
     __shared__ int first[MAX_SEQS], off[MAX_SEQS + 1];
     __shared__ int bad;
-    if (threadIdx.x == 0) bad = 0;
+    __shared__ unsigned long long all;               // missing pages in all: the tables together may claim more than 32 bits count
+    if (threadIdx.x == 0) {
+        bad = 0;
+        all = 0;
+    }
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int s = warp; s < n_seqs; s += BK / 32) {
@@ -99,11 +103,12 @@ grow_kernel(int* __restrict__ table, const int* __restrict__ lens, int* refs, in
         if (lane == 0) {
             first[s] = f;
             off[s] = want - f;
+            if (want > f) atomicAdd(&all, (unsigned long long)(want - f));
         }
     }
     __syncthreads();
-    if (bad) {
-        if (threadIdx.x == 0) fk_raise(err, 95);
+    if (bad || all > (unsigned long long)n_pages) {
+        if (threadIdx.x == 0) fk_raise(err, bad ? 95 : 96);
         return;
     }
     // exclusive prefix over the sequences, a run of them per thread
@@ -126,7 +131,7 @@ grow_kernel(int* __restrict__ table, const int* __restrict__ lens, int* refs, in
     if (threadIdx.x == 0) off[n_seqs] = need;
     __syncthreads();
     if (need == 0) return;
-    if (need < 0 || need > n_pages || !enough_free(refs, n_pages, need, part)) {
+    if (!enough_free(refs, n_pages, need, part)) {
         if (threadIdx.x == 0) fk_raise(err, 96);
         return;
     }
@@ -479,6 +484,7 @@ FK_EXPORT int fk_pages_fork(fk_ctx* ctx, void* stream, const fk_pages* p, const 
     if (rc == FK_OK) rc = list_ok("pages_fork: destinations", dst_host, m, p->n_seqs);
     if (rc != FK_OK) return rc;
     if (!src_host) return fk_fail(FK_INVALID, "pages_fork: null argument");
+    if (p->n_layers > 65535) return fk_fail(FK_UNSUPPORTED, "pages_fork: %d layers", p->n_layers);
     ForkList list;
     list.n = m;
     for (int i = 0; i < m; i++) {
@@ -495,7 +501,6 @@ FK_EXPORT int fk_pages_fork(fk_ctx* ctx, void* stream, const fk_pages* p, const 
                    items, ctx->err_flag), FK_LAUNCH);
     FK_PAGED_LAUNCHED();
     const int row = p->head_dim * elem_bytes(p->kind);
-    if (p->n_layers > 65535) return fk_fail(FK_UNSUPPORTED, "pages_fork: %d layers", p->n_layers);
     FK_CUDA(launch(copy_parts_kernel, dim3(m, p->n_layers), dim3(256), 0, (cudaStream_t)stream, (char*)p->data_dev, (const CopyItem*)items,
                    page_bytes(p) * p->n_pages, page_bytes(p), 2 * p->n_kv, p->page * row, row), FK_LAUNCH);
     FK_PAGED_LAUNCHED();
@@ -526,7 +531,7 @@ FK_EXPORT int fk_rope_kv_paged(fk_ctx* ctx, void* stream, const fk_pages* p, int
     if (rc != FK_OK) return rc;
     if (!q_dev || !k_dev || !v_dev || !q_out_dev) return fk_fail(FK_INVALID, "rope_kv_paged: null argument");
     if (rows < 1 || n_heads < 1 || n_heads > 65535 || (long long)rows * p->n_seqs > 0x7fffffffLL) return fk_fail(FK_INVALID, "rope_kv_paged: %d rows, %d heads", rows, n_heads);
-    if (!(theta > 0.0f)) return fk_fail(FK_INVALID, "rope_kv_paged: theta %g", (double)theta);
+    if (!(theta > 0.0f) || std::isinf(theta)) return fk_fail(FK_INVALID, "rope_kv_paged: theta %g", (double)theta);
     if ((q_norm_dev == nullptr) != (k_norm_dev == nullptr)) return fk_fail(FK_INVALID, "rope_kv_paged: q and k norm weights come together");
     if ((((uintptr_t)q_dev | (uintptr_t)k_dev | (uintptr_t)v_dev | (uintptr_t)q_out_dev | (uintptr_t)q_norm_dev | (uintptr_t)k_norm_dev) & 15) || (q_ld & 3) ||
         (k_ld & 3) || (v_ld & 3) || q_ld < n_heads * p->head_dim || k_ld < p->n_kv * p->head_dim || v_ld < p->n_kv * p->head_dim)

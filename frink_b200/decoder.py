@@ -389,8 +389,8 @@ class Decoder:
         ops, cfg, (pg, n_new) = self.ops, self.cfg, paged
         r = ops.rope_kv_paged(q, k, v, pg, li, self.h_loc, cfg.rope_theta, neox=cfg.neox, n_new=n_new, q_norm=L.get("q_norm"), k_norm=L.get("k_norm"),
                               eps=cfg.eps)
-        # a row that is not there is left as it is: zeros, so that what the layers make of it stays finite
-        out = None if n_new is None or self._all_live else torch.zeros_like(r)
+        # a row that is not there is left as it is, zero or an earlier step's, so that what the layers make of it stays finite
+        out = None if n_new is None else self._page_out
         return ops.attention_paged(r, pg, li, self.h_loc, n_new=n_new, window=L["window"], first=cfg.first_tokens if L["window"] else 0, sinks=L["sinks"],
                                    out=out)
 
@@ -518,17 +518,22 @@ class Decoder:
         self._page_seq = [self.pages.seq(s) for s in range(n_seqs)]
         self._pool = _PoolMirror(n_seqs, n_pages, page, max_pages)
         self.page_live = torch.zeros(n_seqs, dtype=torch.int32, device=self.dev)       # which sequences a decode step moves
+        self._page_out = torch.zeros((n_seqs, self.h_loc * cfg.head_dim), dtype=torch.float32, device=self.dev)     # a step's attention
         self._graph_pages = None
 
-    @property
-    def _all_live(self):
-        return all(self._pool.lens)
+    def _sequences(self, seqs):
+        seqs = list(seqs)
+        for s in seqs:
+            if not 0 <= s < len(self._pool.lens):
+                raise ValueError(f"sequence {s} of {len(self._pool.lens)}")
+        return seqs
 
     def _live(self, s, on):
         self.page_live[s:s + 1].fill_(int(on))
 
     def forward_pages_seq(self, s, ids):
         """More tokens of sequence s (a prompt, or its next chunk) -> logits of the last one [1, vocab]."""
+        self._sequences([s])
         n = ids.numel()
         add = [n if i == s else 0 for i in range(len(self._pool.lens))]
         self._pool.grow(add)
@@ -590,9 +595,11 @@ class Decoder:
                 t.copy_(k)
             self._pool.restore(saved)
 
-        for _ in range(2):                      # warm up outside the capture, then put everything back
-            self.step_pages(toks, rules)
-        back()
+        try:
+            for _ in range(2):                  # warm up outside the capture, then put everything back
+                self.step_pages(toks, rules)
+        finally:
+            back()
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
@@ -609,7 +616,9 @@ class Decoder:
 
     def fork_pages(self, src, dst, n=None):
         """Sequence dst[i] (empty) becomes the first n[i] (default: all) tokens of src[i]; whole pages are shared."""
-        src, dst = list(src), list(dst)
+        src, dst = self._sequences(src), self._sequences(dst)
+        if len(src) != len(dst) or (n is not None and len(n) != len(src)):
+            raise ValueError("lists of one length")
         n = [self._pool.lens[a] if n is None or n[i] is None else n[i] for i, a in enumerate(src)]
         if len(set(dst)) != len(dst) or set(dst) & set(src):
             raise ValueError("a sequence is forked into once, and is not a source of the same call")
@@ -621,7 +630,7 @@ class Decoder:
 
     def free_pages(self, seqs):
         """The sequences give their pages back; a decode step leaves them out."""
-        seqs = list(seqs)
+        seqs = self._sequences(seqs)
         if len(set(seqs)) != len(seqs):
             raise ValueError("a sequence is freed once")
         self._pool.free(seqs)

@@ -672,6 +672,8 @@ def _rows_of(pg, t, width, what):
         raise _lib.Invalid(f"{what}: float32 rows of {width}, their values side by side")
     if n == 0 or n % pg.n_seqs:
         raise _lib.Invalid(f"{what}: {n} rows for {pg.n_seqs} sequences")
+    if n > 1 and ld < width:
+        raise _lib.Invalid(f"{what}: rows of {width} floats that lie over one another")
     return n, ld if n > 1 else max(ld, width)
 
 
@@ -731,7 +733,7 @@ def logit_rules(logits, history=None, penalties=None, bias=None, mask=None, out=
     """What a sampler does to logits [n, vocab] (or one row) before it picks, and the greedy pick -> (changed logits, tokens
     int32 [n]).  history [n, h] int32: the tokens that came before (entries outside the vocabulary are empty places); a token
     that occurs c > 0 times has its logit divided (if positive, else multiplied) by repeat, less c * frequency, less presence
-    (penalties: float32 [n, 3], or one triple for all rows).  bias [vocab] or [n, vocab] is added, then logits whose bit in mask
+    (penalties: float32 [n, 3], or one triple for all rows: numbers of the host, so not while a graph is captured).  bias [vocab] or [n, vocab] is added, then logits whose bit in mask
     (int32 words [words] or [n, words], bit v % 32 of word v / 32) is clear become -inf.  tokens: the largest, ties to the lower
     index; -1 where nothing is left."""
     x = logits if logits.dim() == 2 else logits[None]

@@ -118,3 +118,15 @@ def test_generate_under_a_grammar_ends_where_nothing_may_follow():
     dec.reset()
     words[3] = 0
     assert dec.generate(ids(5, 4), 4, rules=LogitRules(1, mask=words, device="cpu")) == [-1]
+
+
+def test_sequences_that_are_not_there_are_refused():
+    dec = model()
+    dec.alloc_pages(3, 8, dtype=torch.float32)
+    dec.forward_pages_seq(2, ids(20, 1))
+    held = dec._pool.save()
+    for call in (lambda: dec.forward_pages_seq(-1, ids(3, 2)), lambda: dec.forward_pages_seq(3, ids(3, 2)), lambda: dec.free_pages([-1]), lambda: dec.fork_pages([-1], [0]),
+                 lambda: dec.fork_pages([2], [3]), lambda: dec.fork_pages([2], [0, 1]), lambda: dec.fork_pages([2], [0], [1, 2])):
+        with pytest.raises(ValueError):
+            call()
+    assert dec._pool.save() == held

@@ -104,3 +104,31 @@ def test_captured_and_replayed():
         graph.replay()
         o, t = device.logit_rules(x, history=hist, penalties=pen)
         assert torch.equal(o, out) and torch.equal(t, tok)
+
+
+@pytest.mark.parametrize("n,V", [(64, 9 * 24576), (64, 9 * 24480), (64, 9 * 24480 + 1), (64, 10 * 24480), (1, 64 * 24480)])
+def test_a_block_takes_as_many_logits_as_it_can(n, V):
+    """Vocabularies at which a block's counts are as many as shared memory holds."""
+    from frink_b200 import device
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn((n, V), generator=g, device="cuda")
+    hist = torch.randint(0, V, (n, 300), generator=g, device="cuda", dtype=torch.int32)
+    hist[:, 0], hist[:, 1] = V - 1, 0
+    pen = torch.tensor([[1.5, 0.25, 0.5]], device="cuda").expand(n, 3).contiguous()
+    out, tok = device.logit_rules(x, history=hist, penalties=pen)
+    c = torch.zeros((n, V), device="cuda").scatter_add_(1, hist.long(), torch.ones((n, 300), device="cuda"))
+    # (divided by a tensor: by a number, torch multiplies with its rounded reciprocal)
+    want = torch.where(c > 0, torch.where(x > 0, x / pen[:, :1], x * 1.5) - c * 0.25 - 0.5, x)
+    assert torch.equal(out, want) and torch.equal(tok.long(), want.argmax(1))
+
+
+def test_zeros_of_both_signs_are_ties():
+    from frink_b200 import device
+    x = torch.full((4, 9000), -1.0)
+    x[0, 3], x[0, 7000] = -0.0, 0.0
+    x[1, 3], x[1, 7000] = 0.0, -0.0
+    x[2, 4], x[2, 5] = -0.0, 0.0
+    x[3, 100], x[3, 150] = -0.0, 0.0
+    out, tok = device.logit_rules(x.cuda())
+    assert tok.tolist() == [3, 3, 4, 100]
+    assert torch.equal(torch.signbit(out.cpu()), torch.signbit(x))

@@ -1,6 +1,7 @@
 """Refusals of the paged cache's and the logit rules' entry points: what is wrong is said before anything is launched, so the
 checks run without a GPU (the context is a block of zeros that no refused call looks into)."""
 import ctypes as C
+import types
 
 import pytest
 import torch
@@ -57,6 +58,7 @@ def test_lists_are_checked():
     refused("fk_pages_fork", CTX, None, p, ints(0, 1), ints(1, 2), None, 2, match="source and a destination")
     refused("fk_pages_fork", CTX, None, p, ints(3), ints(1), None, 1)
     refused("fk_pages_fork", CTX, None, p, None, ints(1), None, 1)
+    refused("fk_pages_fork", CTX, None, pool(n_layers=65536), ints(0), ints(1), None, 1, status=_lib.FK_UNSUPPORTED)
     refused("fk_pages_grow", CTX, None, p, None, -1)
     refused("fk_pages_advance", CTX, None, p, None, -1)
 
@@ -64,7 +66,7 @@ def test_lists_are_checked():
 def test_rope_and_attention_arguments():
     p, f = pool(), C.c_float
     ok = [CTX, None, p, 0, MEM, MEM, MEM, 256, 128, 128, 1, None, 4, f(1e4), 0, None, None, f(0), MEM]
-    for at, v in ((3, 2), (3, -1), (4, None), (4, MEM + 4), (7, 252), (7, 258), (8, 64), (10, 0), (12, 0), (13, f(0)), (15, MEM), (18, None), (18, MEM + 8)):
+    for at, v in ((3, 2), (3, -1), (4, None), (4, MEM + 4), (7, 252), (7, 258), (8, 64), (10, 0), (12, 0), (13, f(0)), (13, f(float("inf"))), (13, f(float("nan"))), (15, MEM), (18, None), (18, MEM + 8)):
         refused("fk_rope_kv_paged", *(ok[:at] + [v] + ok[at + 1:]))
     refused("fk_rope_kv_paged", *(ok[:7] + [260] + ok[8:]), match="in place")
     ok = [CTX, None, p, 1, MEM, 0, 1, None, 4, f(1), 0, 0, None, MEM]
@@ -89,3 +91,13 @@ def test_python_layer_refuses_tensors_off_the_gpu():
         device.Pages(torch.zeros(1, 4, 2, 2, 16), t(2, 2), t(2), t(4))
     with pytest.raises(_lib.Invalid):
         device.logit_rules(torch.zeros(2, 8))
+
+
+def test_rows_that_lie_over_one_another_are_refused():
+    pg = types.SimpleNamespace(_dev=-1, n_seqs=2)                  # a pool off the GPU, as far as the check of rows looks
+    x = torch.zeros(40)
+    assert device._rows_of(pg, x[:32].view(4, 8), 8, "x") == (4, 8)
+    assert device._rows_of(pg, x.view(4, 10)[:, :8], 8, "x") == (4, 10)
+    for rows in (x[:8].expand(4, 8), x.as_strided((4, 8), (4, 1)), x.as_strided((4, 8), (1, 4)), x[:24].view(3, 8), x[:36].view(4, 9), x.double()[:32].view(4, 8)):
+        with pytest.raises(_lib.Invalid):
+            device._rows_of(pg, rows, 8, "x")

@@ -530,3 +530,45 @@ def test_rows_in_any_stride_and_a_wrong_page_of_a_prompt():
     out.fill_(7.0)
     device.attention_paged(q, pg, 0, 16, out=out)
     assert device.device_error() == 95 and (out == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n_seqs,rows,heads,n_kv,hd", [(33, 1, 4, 1, 64), (40, 1, 6, 2, 128), (300, 1, 3, 1, 8), (170, 3, 6, 1, 64), (512, 1, 8, 1, 64), (513, 1, 8, 1, 64), (200, 3, 16, 2, 64),
+                                                       (1000, 1, 2, 2, 128)])
+def test_many_sequences(dtype, n_seqs, rows, heads, n_kv, hd):
+    """More sequences than a warp's lanes, and around the number from which each item has a CTA of its own."""
+    rng = np.random.default_rng(n_seqs)
+    lens = rng.integers(0, 200, n_seqs)
+    lens[::7] = 0
+    counts = rng.integers(0, rows + 1, n_seqs)
+    attend(lens.tolist(), counts.tolist(), rows, heads, n_kv, hd, 32, TYPES[dtype], window=100, first=3, sinks=True, seed=n_seqs, ragged=True)
+
+
+@pytest.mark.parametrize("rows,lens", [(1, [3000, 5]), (300, [0, 77])])
+def test_attention_in_place(rows, lens):
+    from frink_b200 import device
+    pg, _ = cache(lens, [rows] * 2, 2, 128, 16, torch.bfloat16)
+    q = queries(2 * rows, 8 * 128, 3).cuda()
+    want = device.attention_paged(q, pg, 0, 8)
+    assert device.attention_paged(q, pg, 0, 8, out=q) is q and torch.equal(q, want)
+
+
+def test_a_row_for_all_is_refused():
+    from frink_b200 import _lib, device
+    pg, _ = cache([5, 9], [1, 1], 1, 64, 16, torch.bfloat16)
+    q = queries(1, 64, 3).cuda().expand(2, 64)
+    with pytest.raises(_lib.Invalid, match="over one another"):
+        device.attention_paged(q, pg, 0, 1)
+    with pytest.raises(_lib.Invalid, match="over one another"):
+        device.rope_kv_paged(q, q, q, pg, 0, 1, 1e4)
+
+
+def test_more_missing_pages_than_32_bits_count():
+    """4096 sequences that ask for 2^20 pages each: 2^32 in all."""
+    from frink_b200 import device
+    pg = device.Pages.alloc(1, 50, 16, 1, 8, 4096, 1 << 20)
+    device.pages_grow(pg, 1 << 24)
+    assert device.device_error() == 96
+    assert pg.table[:, :40].max().item() == -1 and pg.refs.sum().item() == 0
+    device.pages_grow(pg, torch.zeros(4096, dtype=torch.int32, device="cuda"))
+    assert device.device_error() == 0
