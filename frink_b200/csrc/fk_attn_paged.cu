@@ -37,7 +37,9 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int MAX_ENTRIES = 512;           // (sequence, block of columns) pairs that are dealt out in runs
-constexpr int MAX_CTAS = 4 * 160;           // of a grid that shares items, half as many with 16 columns: the join keeps two words a column of each
+constexpr int MAX_CTAS = 640;              // of a grid that shares items: three counters each
+static_assert(3 * MAX_CTAS * sizeof(unsigned) <= WS_COUNTERS, "");
+constexpr int FEW = 8;                     // records that are read together
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct AttnArgs {
@@ -200,8 +202,10 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm.ring[warp]);
     float* const sum_o = reinterpret_cast<float*>(sm.ring[warp]);          // [COLS][PITCH] at the end of an item
 
-    // ---- this CTA's run of units [u, u_end); `start` of entry e: units before it (per KV head), times n_kv in the global order.
+    // ---- this CTA's run of slots [u, u_end): an item has one for its way in and out and one for each unit.  `start` of entry e:
+    // slots before it (per KV head), times n_kv in the global order.
     // Up to 32 entries are scanned by every warp for itself, without a barrier; lane e keeps entry e.
+    auto slots = [](const Span& sp) { return sp.tiles == 0 ? 0 : (sp.tiles + STEP - 1) / STEP + 1; };
     const bool few = n_e <= 32;
     int2 lane_rows = make_int2(0, 0);
     int lane_start = 0x7fffffff;
@@ -217,7 +221,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
             if (lane < n_e) {
                 const int s = a.n_cb == 1 ? lane : lane / a.n_cb;
                 lane_rows = rows_of(a, s, blockIdx.x == 0 && warp == 0);
-                units = (span_of<COLS>(a, lane_rows, lane - s * a.n_cb).tiles + STEP - 1) / STEP;
+                units = slots(span_of<COLS>(a, lane_rows, lane - s * a.n_cb));
             }
             int x = units;
 #pragma unroll
@@ -230,7 +234,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
         } else {
             for (int e0 = 0; e0 < n_e; e0 += WARPS * 32) {
                 const int e = e0 + tid;
-                const int units = e < n_e ? (span_of<COLS>(a, rows_of(a, e / a.n_cb, blockIdx.x == 0), e % a.n_cb).tiles + STEP - 1) / STEP : 0;
+                const int units = e < n_e ? slots(span_of<COLS>(a, rows_of(a, e / a.n_cb, blockIdx.x == 0), e % a.n_cb)) : 0;
                 int sum;
                 const int at = block_prefix(units, sm.part, &sum);
                 if (e < n_e) sm.start[e] = total + at;
@@ -251,7 +255,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
     const int u_begin = u;
 
     while (u < u_end) {
-        int e, kvh, i0, i1, item0 = 0, units, start = 0;           // units [i0, i1) of the item, the item's first unit
+        int e, kvh, i0, i1, first = 0, units, start = 0;           // units [i0, i1) of the item, the slot of its first unit
         int2 rows;
         if (a.whole) {
             e = blockIdx.x / a.n_kv;
@@ -280,11 +284,12 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
             i1 = units;
             u = 1;
         } else {
-            kvh = (u - start * a.n_kv) / units;
-            item0 = start * a.n_kv + kvh * units;
-            i0 = u - item0;
-            i1 = min(units, u_end - item0);
-            u = item0 + i1;
+            kvh = (u - start * a.n_kv) / (units + 1);
+            first = start * a.n_kv + kvh * (units + 1) + 1;
+            i0 = max(0, u - first);
+            i1 = min(units, u_end - first);
+            u = first + i1;
+            if (i1 <= i0) break;                                   // the run ends before the item's first unit
         }
 
         // ---- the warp's steps: unit i0 + j, its tiles SUB (4 (i0 + j) + warp) and on of the item's list
@@ -722,7 +727,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
         };
         const bool direct = a.whole || (i0 == 0 && i1 == units);
         // a CTA's record 1 is the item that begins in its run and goes on behind it, record 0 the one that began before
-        float* rec = a.rec + ((size_t)2 * blockIdx.x + (item0 >= u_begin ? 1 : 0)) * ATTN_RECORD;
+        float* rec = a.rec + ((size_t)2 * blockIdx.x + (first >= u_begin ? 1 : 0)) * ATTN_RECORD;
         for (int x = tid; x < COLS * (HDP / 4); x += WARPS * 32) {
             const int c = x / (HDP / 4), d = 4 * (x % (HDP / 4));
             float M = -INFINITY;
@@ -749,96 +754,89 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) attn_paged_kernel
         }
         if (direct) continue;
 
-        // ---- the last CTA of the item joins the records of CTAs [c0, c1]: weights of all of them first, then the sums
-        const int c0 = item0 / chunk, n_rec = (item0 + units - 1) / chunk - c0 + 1;
-        __syncthreads();
-        if (tid == 0) {
-            // the CTA's record goes out by way of the barrier and this release, the others' come in by the acquire
-            unsigned before;
-            asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.cnt + c0) : "memory");
-            sm.last = before == (unsigned)(n_rec - 1);
-        }
-        __syncthreads();
-        if (!sm.last) continue;
+        // ---- join the records of CTAs [c0, c0 + n_rec).  Few: the last one to arrive takes them all.  More: groups of about the
+        // square root of their number are joined into their first record by the group's last one, and those by the last group's.
+        const int c0 = first / chunk, n_rec = (first + units - 1) / chunk - c0 + 1;
+        // whether all n have arrived; a CTA's record goes out by way of the barrier and this release, the others' come in by the acquire
+        auto arrive = [&](unsigned* cnt, int n) {
+            __syncthreads();
+            if (tid == 0) {
+                unsigned before;
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(cnt) : "memory");
+                sm.last = before == (unsigned)(n - 1);
+                if (sm.last) *cnt = 0;
+            }
+            __syncthreads();
+            return sm.last != 0;
+        };
         // record 1 of the CTA in which the item begins, record 0 of the others
-        auto record = [&](int k) { return a.rec + ((size_t)2 * (c0 + k) + (k == 0 ? 1 : 0)) * ATTN_RECORD; };
-        constexpr int FEW = 8;
-        if (n_rec <= FEW) {                                        // everything at once, one trip to memory
-            for (int x = tid; x < COLS * (HDP / 4); x += WARPS * 32) {
-                const int c = x / (HDP / 4), d = 4 * (x % (HDP / 4));
-                float mk[FEW], lk[FEW];
+        auto slot = [&](int k) { return 2 * (c0 + k) + (k == 0 ? 1 : 0); };
+        // records k0, k0 + step, ... (n of them) of four dims of a column, eight at a time
+        auto gather = [&](int k0, int step, int n, int c, int d, float& M, float& L, float4& O) {
+            M = -INFINITY;
+            L = 0.0f;
+            O = make_float4(0, 0, 0, 0);
+            for (int b = 0; b < n; b += FEW) {
+                float mk[FEW], lk[FEW], top = M;
                 float4 v[FEW];
 #pragma unroll
                 for (int k = 0; k < FEW; k++) {
                     mk[k] = -INFINITY;
                     lk[k] = 0.0f;
                     v[k] = make_float4(0, 0, 0, 0);
-                    if (k < n_rec) {
-                        const float* r = record(k);
+                    if (b + k < n) {
+                        const float* r = a.rec + (size_t)slot(k0 + (b + k) * step) * ATTN_RECORD;
                         mk[k] = __ldcg(r + 16 * 128 + c);
                         lk[k] = __ldcg(r + 16 * 129 + c);
                         v[k] = __ldcg((const float4*)(r + c * 128 + d));
                     }
                 }
-                float M = -INFINITY, L = 0.0f;
-                float4 O = make_float4(0, 0, 0, 0);
 #pragma unroll
-                for (int k = 0; k < FEW; k++) M = fmaxf(M, mk[k]);
+                for (int k = 0; k < FEW; k++) top = fmaxf(top, mk[k]);
+                const float f0 = M == -INFINITY ? 1.0f : pow2(M - top);                  // nothing yet, or NaN, which stays
+                L *= f0;
+                O.x *= f0; O.y *= f0; O.z *= f0; O.w *= f0;
 #pragma unroll
                 for (int k = 0; k < FEW; k++) {
-                    const float f = mk[k] == -INFINITY ? (lk[k] != lk[k] ? lk[k] : 0.0f) : pow2(mk[k] - M);
+                    const float f = mk[k] == -INFINITY ? (lk[k] != lk[k] ? lk[k] : 0.0f) : pow2(mk[k] - top);
                     L += lk[k] * f;
                     O.x += v[k].x * f; O.y += v[k].y * f; O.z += v[k].z * f; O.w += v[k].w * f;
                 }
-                finish(c, d, M, L, O);
+                M = top;
             }
-            if (tid == 0) a.cnt[c0] = 0;
-            continue;
+        };
+        int per = FEW;
+        while (per * per < n_rec) per++;
+        const int groups = (n_rec + per - 1) / per;
+        if (groups > 1) {
+            const int g0 = ((int)blockIdx.x - c0) / per * per, n = min(per, n_rec - g0);
+            if (!arrive(a.cnt + slot(g0), n)) continue;
+            float* const to = a.rec + (size_t)slot(g0) * ATTN_RECORD;
+            for (int x = tid; x < COLS * (HDP / 4); x += WARPS * 32) {
+                const int c = x / (HDP / 4), d = 4 * (x % (HDP / 4));
+                float M, L;
+                float4 O;
+                gather(g0, 1, n, c, d, M, L, O);
+                *(float4*)(to + c * 128 + d) = O;                  // only this thread read this place
+                if (d == 0) {
+                    sm.m[0][c] = M;
+                    sm.l[0][c] = L;
+                }
+            }
+            __syncthreads();
+            if (tid < COLS) {
+                to[16 * 128 + tid] = sm.m[0][tid];
+                to[16 * 129 + tid] = sm.l[0][tid];
+            }
         }
-        float* const wts = reinterpret_cast<float*>(sm.ring);      // [n_rec][COLS]
-        float* const red = reinterpret_cast<float*>(sm.q);         // [2][threads]
-        static_assert(sizeof(sm.q) >= 2 * WARPS * 32 * 4 && sizeof(sm.ring) >= (size_t)2 * MAX_CTAS / NT * COLS * 4, "");
-        constexpr int PER = WARPS * 32 / COLS;                     // threads of a column
-        const int my_c = tid % COLS;
-        float most = -INFINITY;
-        for (int k = tid / COLS; k < n_rec; k += PER) {
-            const float* r = record(k) + 16 * 128 + my_c;
-            const float mk = __ldcg(r), lk = __ldcg(r + 16);
-            wts[2 * (k * COLS + my_c)] = mk;
-            wts[2 * (k * COLS + my_c) + 1] = lk;
-            most = fmaxf(most, mk);
-        }
-        red[tid] = most;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < PER; i++) most = fmaxf(most, red[i * COLS + my_c]);
-        float sum = 0.0f;
-        for (int k = tid / COLS; k < n_rec; k += PER) {
-            const float mk = wts[2 * (k * COLS + my_c)], lk = wts[2 * (k * COLS + my_c) + 1];
-            const float f = mk == -INFINITY ? (lk != lk ? lk : 0.0f) : pow2(mk - most);
-            wts[2 * (k * COLS + my_c)] = f;
-            sum += lk * f;
-        }
-        red[WARPS * 32 + tid] = sum;
-        __syncthreads();
+        if (!arrive(a.cnt + 2 * MAX_CTAS + c0, groups > 1 ? groups : n_rec)) continue;
         for (int x = tid; x < COLS * (HDP / 4); x += WARPS * 32) {
             const int c = x / (HDP / 4), d = 4 * (x % (HDP / 4));
-            float M = -INFINITY, L = 0.0f;
-#pragma unroll
-            for (int i = 0; i < PER; i++) {
-                M = fmaxf(M, red[i * COLS + c]);
-                L += red[WARPS * 32 + i * COLS + c];
-            }
-            float4 O = make_float4(0, 0, 0, 0);
-#pragma unroll 16
-            for (int k = 0; k < n_rec; k++) {
-                const float4 v = __ldcg((const float4*)(record(k) + c * 128 + d));
-                const float f = wts[2 * (k * COLS + c)];
-                O.x += v.x * f; O.y += v.y * f; O.z += v.z * f; O.w += v.w * f;
-            }
+            float M, L;
+            float4 O;
+            gather(0, groups > 1 ? per : 1, groups > 1 ? groups : n_rec, c, d, M, L, O);
             finish(c, d, M, L, O);
         }
-        if (tid == 0) a.cnt[c0] = 0;
     }
 }
 
@@ -859,7 +857,7 @@ template <int KIND, int HDP, bool EXACT, int NT> int launch_attn(fk_ctx* ctx, cu
     if (entries * a.n_kv > 0x7fffffffLL) return fk_fail(FK_UNSUPPORTED, "attention_paged: %d rows of %d sequences", a.rows, a.n_seqs);
     a.whole = entries > MAX_ENTRIES;
     const int ctas = per_sm * ctx->sm_count;
-    const unsigned grid = a.whole ? (unsigned)(entries * a.n_kv) : (unsigned)(ctas < MAX_CTAS / NT ? ctas : MAX_CTAS / NT);
+    const unsigned grid = a.whole ? (unsigned)(entries * a.n_kv) : (unsigned)(ctas < MAX_CTAS ? ctas : MAX_CTAS);
     FK_CUDA(launch(kern, dim3(grid), dim3(WARPS * 32), smem, st, a), FK_LAUNCH);
     return FK_OK;
 }
