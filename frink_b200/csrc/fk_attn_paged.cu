@@ -13,9 +13,9 @@
 // of the data.  The scores' fragment becomes the weights' operand by a transposition of 8 x 8 blocks inside the warp (movmatrix).
 //
 // Memory.  16 tokens of one head are one contiguous piece of a page.  Every warp keeps a ring of its own in shared memory and
-// fills it with asynchronous copies one tile ahead, keys and values apart, so that no warp waits for another and a tile's
-// latency is covered by the tile before it and by the SM's other warps.  The copies place 16-byte pieces so that the operand
-// reads hit every bank once.
+// fills it with asynchronous copies a step (32 tokens) ahead, keys and values apart, so that no warp waits for another and a
+// step's latency is covered by the step before it and by the SM's other warps.  The copies place 16-byte pieces so that the
+// operand reads hit every bank once.  8 x 4000 tokens of 24/8 heads of 128 in bf16: loads into registers 42.9 us, rings 37.9.
 //
 // Precision.  The cache's 16-bit values are exact operands.  q and w are f32 and are split into parts of the cache's type:
 // three bf16 parts hold all 24 bits; two f16 parts hold 22, their range kept by a power of two per column of q and by a
@@ -23,10 +23,18 @@
 // cores' own running sums are cut off rather than rounded, which over thousands of tiles adds up to a bias, so a product of
 // a few steps starts from zero and joins the running sum in an ordinary, rounded addition.
 //
-// Work.  The keys of every (sequence, block of columns, KV head) are cut into units of 64 tokens (16 a warp) and all units,
-// one after another, are dealt out in equal runs to the CTAs of one grid, so that ragged lengths keep every SM busy and the
-// grid does not depend on lengths that only the device knows.  A run's first and last item may be shared with other CTAs: their
-// partial sums go to a record of the CTA, and the CTA that arrives last joins them.
+// Work.  The keys of every (sequence, block of columns, KV head) are cut into units of 128 tokens (32 a warp; f32: 64) and all
+// units, one after another, are dealt out in equal runs to the CTAs of one grid, so that ragged lengths keep every SM busy and
+// the grid does not depend on lengths that only the device knows.  An item's way in (pages' numbers, q) and out (sums of the
+// warps) takes about a unit's time and is dealt out like one: 500 sequences of 1 to 600 tokens, 8 KV heads, 155 us without, 125
+// with.  A run's first and last item may be shared with other CTAs: their partial sums go to a record of the CTA; the CTA that
+// arrives last joins up to eight of them in one trip to memory, more in groups of about the square root of their number (131071
+// tokens, 55 records an item: one CTA for all 57.2 us, groups 51.3).
+//
+// Bound by HBM where sequences are long, by its way in and out (some 10 us: launch, entries, page numbers, first copies, join)
+// where they are short.  B200: 64 sequences of 250 to 16000 tokens, window 4096, 32/4 heads of 128 in bf16, 84 us = 5.7 TB/s;
+// 131071 tokens, 64/8 heads of 64 in f16, 51.3 us = 5.2 TB/s; 8 x 4000 as above 29.7 us = 4.4 TB/s; 8 x 64000 6.4 TB/s; 17
+// tokens in f32 6.5 us.  (A plain copy moves 6.55 TB/s.)
 #include "fk_paged.cuh"
 
 #include <type_traits>
@@ -36,7 +44,11 @@ using namespace fk_paged;
 namespace {
 
 constexpr int WARPS = 4;
-constexpr int MAX_ENTRIES = 512;           // (sequence, block of columns) pairs that are dealt out in runs
+// (sequence, block of columns) pairs that are dealt out in runs; where there are more, each (pair, KV head) has a CTA.  The deal
+// costs a scan of the pairs by every CTA and keeps one long sequence from outlasting the others; 512 pairs dealt / 513 with CTAs
+// of their own, us: 100 tokens and 8 KV heads 75 / 63, 1000 and 8 329 / 305, 1000 and 1 56 / 60, 4000 and 1 172 / 204; 500
+// sequences of very different lengths (mean 8000) and 2 KV heads 639 / 1005.
+constexpr int MAX_ENTRIES = 512;
 constexpr int MAX_CTAS = 640;              // of a grid that shares items: three counters each
 static_assert(3 * MAX_CTAS * sizeof(unsigned) <= WS_COUNTERS, "");
 constexpr int FEW = 8;                     // records that are read together
@@ -863,6 +875,8 @@ template <int KIND, int HDP, bool EXACT, int NT> int launch_attn(fk_ctx* ctx, cu
 }
 
 template <int KIND> int launch_kind(fk_ctx* ctx, cudaStream_t st, const AttnArgs& a) {
+    // 16 columns a CTA read the keys once for twice the columns, with registers for two CTAs an SM instead of three.  Us with 16 /
+    // with 8: 16 columns 64 x 4000 tokens 117 / 170, 8 x 16000 69 / 91, 1 x 64000 51 / 49; 12 columns 64 x 4000 45 / 40.
     const bool wide = (long long)a.rows * a.group > 8;
     if (a.head_dim == 64) return wide ? launch_attn<KIND, 64, true, 2>(ctx, st, a) : launch_attn<KIND, 64, true, 1>(ctx, st, a);
     if (a.head_dim == 128) return wide ? launch_attn<KIND, 128, true, 2>(ctx, st, a) : launch_attn<KIND, 128, true, 1>(ctx, st, a);

@@ -18,11 +18,15 @@
 // (Two groups that take turns with a tile each need no exchange, but a tile is then twice as long between its scores and its
 // weights, and that chain bounds the kernel: 4200 rows of 24/8 heads of 128, bf16, 398 us that way, 326 us this way = 332 TFLOP/s
 // of the formula's operations, three times that of MMA.)  8 to 15 keep the running output, a thread per row and half of the
-// dims.  16 loads
-// tiles (a lane per page piece, TMA with 128-byte swizzle).  17 issues the products for S and 19 those for O, so that scores are
-// made as soon as their buffer is free and not in turn with products that wait for weights.  18 looks over the values of tiles
-// that not every row sees: a value that no row sees is zeroed in shared memory (stale memory may hold NaN); one that some rows
-// see and that is not finite is zeroed too and added in plain f32 for the rows that see it.
+// dims.  16 loads tiles (a lane per page piece, TMA with 128-byte swizzle).  17 issues the products for S and 19 those for O, so
+// that scores are made as soon as their buffer is free and not in turn with products that wait for weights.  18 looks over the
+// values of tiles that not every row sees: a value that no row sees is zeroed in shared memory (stale memory may hold NaN); one
+// that some rows see and that is not finite is zeroed too and added in plain f32 for the rows that see it.
+//
+// Measured (B200): 512 rows of 24/8 heads of 128, bf16, empty cache 23.1 us; 4200 rows 326 us, f16 296 us; 1001, 801, 601 and 401
+// rows after 2000 to 8000 tokens, window 2048, 64/8 heads of 64, f16, 431 us.  Tensor pipe 22 %, issue slots 45 %: what bounds it
+// is a tile's chain from scores to weights (some 1800 cycles of the softmax warps, f16 heads of 64; 2450 with the products' own
+// time, bf16 heads of 128) and a CTA's way in and out, some 15000 cycles (512 columns of tensor memory: one CTA an SM).
 #include "fk_paged.cuh"
 #include "fk_tc.cuh"
 

@@ -391,7 +391,8 @@ int fk_add_int(fk_ctx* ctx, void* stream, int* p_dev, int v);
  * kernel finds wrong there it raises in the device error word: 95 a sequence would outgrow its table row, 96 fewer free
  * pages than needed, 97 a page number outside the pool, 98 a fork of more tokens than its source holds or into a sequence
  * that holds something.  grow and fork that raise change nothing; a row of attention or append whose sequence is wrong
- * (95) is left as it was; a wrong page number (97) is read as page 0 and never written. */
+ * (95) is left as it was; a wrong page number (97) is read as page 0 and never written.  63: a bounded wait of the prompt
+ * kernel ran out (its rows are then undefined). */
 typedef struct fk_pages {
     void* data_dev;
     int* table_dev;
@@ -432,7 +433,8 @@ int fk_rope_kv_paged(fk_ctx* ctx, void* stream, const fk_pages* pages, int layer
  * and value are in the pages already) and sees the keys j <= p with window == 0, j > p - window, or j < first: with a window
  * the `first` earliest tokens stay visible.  sinks_dev, q_ld (0 = packed) as in fk_attention.  Rows i >= n_new_dev[s] are left
  * as they were.  f32 precision for every kind: the cache's values meet q and the weights split into parts whose products are
- * exact. */
+ * exact.  Keys and values that a row does not see are never looked at for it, whatever they hold; one that it sees and that is
+ * infinite or NaN spoils its outputs.  out_dev may be q_dev where its rows are packed. */
 int fk_attention_paged(fk_ctx* ctx, void* stream, const fk_pages* pages, int layer, const float* q_dev, int q_ld, int rows, const int* n_new_dev,
                        int n_heads, float scale, int window, int first, const float* sinks_dev, float* out_dev);
 

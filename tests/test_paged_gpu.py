@@ -572,3 +572,8 @@ def test_more_missing_pages_than_32_bits_count():
     assert pg.table[:, :40].max().item() == -1 and pg.refs.sum().item() == 0
     device.pages_grow(pg, torch.zeros(4096, dtype=torch.int32, device="cuda"))
     assert device.device_error() == 0
+
+
+def test_more_columns_than_the_deal_holds():
+    """Tens of thousands of (sequence, block of columns) pairs of 32-bit pages."""
+    attend([10, 0], [2050, 7], 2050, 130, 1, 8, 64, torch.float32, window=60, first=2, sinks=True, seed=9, ragged=True)
