@@ -1,8 +1,10 @@
 // Attention of a prompt's rows over a paged KV cache on the tensor cores (tcgen05): 16-bit pages, heads of up to 128.  The
 // mathematics, the masks and the precision are those of fk_attn_paged.cu.
 //
-// A CTA takes 128 (row, query head) pairs of one KV head -- 128 / group consecutive rows, so a short prompt still fills the
-// tile -- and walks the visible keys in tiles of 64:
+// An item is 128 (row, query head) pairs of one KV head -- 128 / group consecutive rows, so a short prompt still fills the
+// tile -- and the visible keys in tiles of 64.  There is a CTA per SM, which goes through its items with the rings running on:
+// the next item's first tiles and q are on their way while the current one ends (a CTA per item: 430 us where this takes 393,
+// see below).  A tile:
 //
 //   S = q K^T          A = q's parts in tensor memory, B = a tile of K in shared memory, S in tensor memory (two or three buffers)
 //   w = 2^(S - m)      a thread per row; its parts go back over S as the next product's A operand
@@ -16,17 +18,17 @@
 //
 // Warps 0 to 7 are the softmax: a thread has a row and half of the tile's keys, and the halves exchange the row's maximum.
 // (Two groups that take turns with a tile each need no exchange, but a tile is then twice as long between its scores and its
-// weights, and that chain bounds the kernel: 4200 rows of 24/8 heads of 128, bf16, 398 us that way, 326 us this way = 332 TFLOP/s
-// of the formula's operations, three times that of MMA.)  8 to 15 keep the running output, a thread per row and half of the
+// weights, and that chain bounds the kernel: 4200 rows of 24/8 heads of 128, bf16, 398 us that way, 326 us this way, with a CTA
+// per item.)  8 to 15 keep the running output, a thread per row and half of the
 // dims.  16 loads tiles (a lane per page piece, TMA with 128-byte swizzle).  17 issues the products for S and 19 those for O, so
 // that scores are made as soon as their buffer is free and not in turn with products that wait for weights.  18 looks over the
 // values of tiles that not every row sees: a value that no row sees is zeroed in shared memory (stale memory may hold NaN); one
 // that some rows see and that is not finite is zeroed too and added in plain f32 for the rows that see it.
 //
-// Measured (B200): 512 rows of 24/8 heads of 128, bf16, empty cache 23.1 us; 4200 rows 326 us, f16 296 us; 1001, 801, 601 and 401
-// rows after 2000 to 8000 tokens, window 2048, 64/8 heads of 64, f16, 431 us.  Tensor pipe 22 %, issue slots 45 %: what bounds it
-// is a tile's chain from scores to weights (some 1800 cycles of the softmax warps, f16 heads of 64; 2450 with the products' own
-// time, bf16 heads of 128) and a CTA's way in and out, some 15000 cycles (512 columns of tensor memory: one CTA an SM).
+// Measured (B200): 512 rows of 24/8 heads of 128, bf16, empty cache 23.9 us; 4200 rows 315 us = 344 TFLOP/s of the formula's
+// operations, three times that of MMA, f16 287 us; 1001, 801, 601 and 401 rows after 2000 to 8000 tokens, window 2048, 64/8
+// heads of 64, f16, 393 us.  What bounds it is a tile's chain from scores to weights (f16 heads of 64: tensor pipe 22 %, issue
+// slots 45 %) and, bf16 heads of 128, the products' own time on top of it; an item alone is bound by its way in and out.
 #include "fk_paged.cuh"
 #include "fk_tc.cuh"
 
@@ -87,6 +89,18 @@ template <int KIND, int HD> struct PromptSmem {
     unsigned long long sfull[P::NS], pfull[P::NS], oddfree, ofull[P::NO], ofree[P::NO], qfull, done[2];
     uint32_t tmem;
     int abort;
+};
+
+// 128 / group rows of a sequence and one KV head, and the keys they see: [0, 64 na) and [64 b0, hi)
+struct Item {
+    int kvh, s, row0, row1, base, hi, na, b0, n_tiles;
+    __device__ __forceinline__ int p_min() const { return base + row0; }
+    __device__ __forceinline__ int p_max() const { return hi - 1; }
+    __device__ __forceinline__ int key(int j) const { return (j < na ? j : j - na + b0) * KT; }
+    // whether some row does not see all of the tile
+    __device__ __forceinline__ bool edge(const PromptArgs& a, int key0) const {
+        return key0 + KT - 1 > p_min() || (a.window > 0 && key0 <= p_max() - a.window && key0 + KT - 1 >= a.first);
+    }
 };
 
 // d (+)= a b: A in tensor memory.  Issued by one lane, inside `if (elected())`: the compiler then knows that one thread runs
@@ -178,24 +192,33 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // ---- the item: rows [row0, row1] of sequence s, KV head kvh; long ones (late rows) come first
-    const int kvh = blockIdx.x % a.n_kv, s = (blockIdx.x / a.n_kv) % a.n_seqs, rb = a.n_rb - 1 - (int)(blockIdx.x / ((unsigned)a.n_kv * a.n_seqs));
-    int n = a.n_new ? min(max(a.n_new[s], 0), a.rows) : a.rows;
-    const int base = a.lens[s];
-    if (base < 0 || (long long)base + n > (long long)a.max_pages * a.page) {
-        if (tid == 0 && n > 0) fk_raise(a.err, 95);
-        n = 0;
-    }
-    const int row0 = rb * a.rq, row1 = min(row0 + a.rq, n) - 1;
-    // keys [0, 64 na) and [64 b0, hi)
-    const int hi = base + row1 + 1, lo = a.window > 0 ? max(0, base + row0 + 1 - a.window) : 0;
-    int b0 = lo / KT, na = (min(a.first, lo) + KT - 1) / KT;
-    if (na >= b0) na = b0 = 0;
-    const int n_tiles = __shfl_sync(0xffffffffu, row1 < row0 ? 0 : na + (hi + KT - 1) / KT - b0, 0);
-    const int p_min = base + row0, p_max = hi - 1;
-    if (n_tiles == 0) return;                  // rows that do not exist; the whole CTA leaves
-    auto tile_key = [&](int j) { return (j < na ? j : j - na + b0) * KT; };
-    auto edge_tile = [&](int key0) { return key0 + KT - 1 > p_min || (a.window > 0 && key0 <= p_max - a.window && key0 + KT - 1 >= a.first); };
+    // ---- this CTA's items, one after another: long ones (late rows) come first, every other round in reverse.  All warps go
+    // through them for themselves; t0 counts tiles, by which the rings go on from one item to the next.
+    const int n_items = a.n_rb * a.n_seqs * a.n_kv;
+    auto item_at = [&](int i, Item& x) {
+        const long long at = (long long)i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (at >= n_items) return false;
+        const unsigned it = (unsigned)at;
+        x.kvh = it % (unsigned)a.n_kv;
+        x.s = it / (unsigned)a.n_kv % (unsigned)a.n_seqs;
+        x.row0 = (a.n_rb - 1 - (int)(it / ((unsigned)a.n_kv * a.n_seqs))) * a.rq;
+        int n = a.n_new ? min(max(a.n_new[x.s], 0), a.rows) : a.rows;
+        x.base = a.lens[x.s];
+        if (x.base < 0 || (long long)x.base + n > (long long)a.max_pages * a.page) {
+            if (tid == 0 && n > 0) fk_raise(a.err, 95);
+            n = 0;
+        }
+        x.row1 = min(x.row0 + a.rq, n) - 1;
+        x.hi = x.base + x.row1 + 1;
+        const int lo = a.window > 0 ? max(0, x.base + x.row0 + 1 - a.window) : 0;
+        x.b0 = lo / KT;
+        x.na = (min(a.first, lo) + KT - 1) / KT;
+        if (x.na >= x.b0) x.na = x.b0 = 0;
+        x.n_tiles = __shfl_sync(0xffffffffu, x.row1 < x.row0 ? 0 : x.na + (x.hi + KT - 1) / KT - x.b0, 0);
+        return true;
+    };
+    Item it;
+    bool more = item_at(0, it);
 
     // Tensor memory is taken after the previous kernel is done with its own and before the next one may start: neither can
     // then hold what the other waits for.
@@ -226,45 +249,50 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
         // ---- loads: lane u takes the u-th page piece of a tile.  The page numbers of 32 pieces are read at once, a lane each and
         // a block of tiles ahead: a table lookup takes longer than a tile.
         const int log_piece = min(a.log_page, 6), log_pc = 6 - log_piece, n_pc = 1 << log_pc, ahead = 32 >> log_pc;
-        const int* const tab = a.table + (size_t)s * a.max_pages;
-        auto pages_from = [&](int j0) {
-            const int j = j0 + (lane >> log_pc);
-            const int key = j < n_tiles ? tile_key(j) + ((lane & (n_pc - 1)) << log_piece) : hi;
-            return key < hi ? tab[key >> a.log_page] : -1;
-        };
-        int issued = 0, block = pages_from(0), next = pages_from(ahead);
-        for (int j = 0; j < n_tiles; j++) {
-            const int st = j % STAGES, in_block = j & (ahead - 1);
-            if (j > 0 && in_block == 0) {
-                block = next;
-                next = pages_from(j + ahead);
+        int issued = 0;
+        for (int i = 0, t0 = 0; more; t0 += it.n_tiles, more = item_at(++i, it)) {
+            const Item& x = it;
+            const int* const tab = a.table + (size_t)x.s * a.max_pages;
+            auto pages_from = [&](int j0) {
+                const int j = j0 + (lane >> log_pc);
+                const int key = j < x.n_tiles ? x.key(j) + ((lane & (n_pc - 1)) << log_piece) : x.hi;
+                return key < x.hi ? tab[key >> a.log_page] : -1;
+            };
+            int block = pages_from(0), next = pages_from(ahead);
+            for (int j = 0; j < x.n_tiles; j++) {
+                const int t = t0 + j, st = t % STAGES, in_block = j & (ahead - 1);
+                if (j > 0 && in_block == 0) {
+                    block = next;
+                    next = pages_from(j + ahead);
+                }
+                const int key0 = x.key(j), key = key0 + (lane << log_piece);
+                int pg = __shfl_sync(0xffffffffu, block, (in_block << log_pc) + (lane & (n_pc - 1)));
+                const int pieces = min(n_pc, (x.hi - key0 + (1 << log_piece) - 1) >> log_piece);
+                const bool mine = lane < pieces;
+                if (mine && (pg < 0 || pg >= a.n_pages)) {
+                    fk_raise(a.err, 97);
+                    pg = 0;
+                }
+                const int y = ((2 * pg) * a.n_kv + x.kvh) * a.page + (key & (a.page - 1));
+                if (t >= STAGES) wait(&sm.kfree[st], (t / STAGES - 1) & 1);
+                if (t >= STAGES) wait(&sm.vfree[st], (t / STAGES - 1) & 1);
+                if (gave_up()) break;
+                if (lane == 0) {
+                    mbar_expect_tx(smem_u32(&sm.kfull[st]), (pieces << log_piece) * HD * 2);
+                    mbar_expect_tx(smem_u32(&sm.vfull[st]), (pieces << log_piece) * HD * 2);
+                }
+                __syncwarp();
+                if (mine) {
+#pragma unroll
+                    for (int h = 0; h < HD / 64; h++)
+                        tma_load_2d(smem_u32(sm.k[st]) + h * (KT * 128) + (lane << log_piece) * 128, &a.map, h * 64, y, smem_u32(&sm.kfull[st]));
+#pragma unroll
+                    for (int h = 0; h < HD / 64; h++)
+                        tma_load_2d(smem_u32(sm.v[st]) + h * (KT * 128) + (lane << log_piece) * 128, &a.map, h * 64, y + a.n_kv * a.page, smem_u32(&sm.vfull[st]));
+                }
+                issued = t + 1;
             }
-            const int key0 = tile_key(j), key = key0 + (lane << log_piece);
-            int pg = __shfl_sync(0xffffffffu, block, (in_block << log_pc) + (lane & (n_pc - 1)));
-            const int pieces = min(n_pc, (hi - key0 + (1 << log_piece) - 1) >> log_piece);
-            const bool mine = lane < pieces;
-            if (mine && (pg < 0 || pg >= a.n_pages)) {
-                fk_raise(a.err, 97);
-                pg = 0;
-            }
-            const int y = ((2 * pg) * a.n_kv + kvh) * a.page + (key & (a.page - 1));
-            if (j >= STAGES) wait(&sm.kfree[st], (j / STAGES - 1) & 1);
-            if (j >= STAGES) wait(&sm.vfree[st], (j / STAGES - 1) & 1);
             if (gave_up()) break;
-            if (lane == 0) {
-                mbar_expect_tx(smem_u32(&sm.kfull[st]), (pieces << log_piece) * HD * 2);
-                mbar_expect_tx(smem_u32(&sm.vfull[st]), (pieces << log_piece) * HD * 2);
-            }
-            __syncwarp();
-            if (mine) {
-#pragma unroll
-                for (int h = 0; h < HD / 64; h++)
-                    tma_load_2d(smem_u32(sm.k[st]) + h * (KT * 128) + (lane << log_piece) * 128, &a.map, h * 64, y, smem_u32(&sm.kfull[st]));
-#pragma unroll
-                for (int h = 0; h < HD / 64; h++)
-                    tma_load_2d(smem_u32(sm.v[st]) + h * (KT * 128) + (lane << log_piece) * 128, &a.map, h * 64, y + a.n_kv * a.page, smem_u32(&sm.vfull[st]));
-            }
-            issued = j + 1;
         }
         // every copy that was started has landed before the CTA ends
         for (int j = max(0, issued - STAGES); j < issued; j++) {
@@ -276,25 +304,28 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
         // ---- S = q K^T
         constexpr uint32_t ID_S = idesc_of(KIND, 128, KT, 0);
         const uint64_t k_desc = umma_desc(smem_u32(sm.k[0]));
-        if (n_tiles > 0) wait(&sm.qfull, 0);
-        for (int j = 0; j < n_tiles && !gave_up(); j++) {
-            const int st = j % STAGES, x = j - NS;
-            // S takes the place of w of tile j - NS: products with different results may pass one another, so that one is waited for
-            if (x >= 0) wait(&sm.vfree[x % STAGES], (x / STAGES) & 1);
-            wait(&sm.kfull[st], (j / STAGES) & 1);
-            tc_fence_after();
-            const uint32_t d = tmem + P::S0 + (j % NS) * P::SREG + P::LEAD;
-            const uint64_t b = k_desc + (uint32_t)(st * (P::TILE >> 4));
-            if (elected()) {
+        for (int i = 0, t0 = 0, done = 0; more && !gave_up(); t0 += it.n_tiles, more = item_at(++i, it)) {
+            if (it.n_tiles == 0) continue;
+            wait(&sm.qfull, done++ & 1);
+            for (int t = t0; t < t0 + it.n_tiles && !gave_up(); t++) {
+                const int st = t % STAGES, x = t - NS;
+                // S takes the place of w of tile t - NS: products with different results may pass one another, so that one is waited for
+                if (x >= 0) wait(&sm.vfree[x % STAGES], (x / STAGES) & 1);
+                wait(&sm.kfull[st], (t / STAGES) & 1);
+                tc_fence_after();
+                const uint32_t d = tmem + P::S0 + (t % NS) * P::SREG + P::LEAD;
+                const uint64_t b = k_desc + (uint32_t)(st * (P::TILE >> 4));
+                if (elected()) {
 #pragma unroll
-                for (int k = QP - 1; k >= 0; k--)                  // the small parts first
+                    for (int k = QP - 1; k >= 0; k--)              // the small parts first
 #pragma unroll
-                    for (int ks = 0; ks < HD / 16; ks++)
-                        mma_ts(d, tmem + P::Q0 + k * HALF + ks * 8, b + (((ks >> 2) * (KT * 128) + (ks & 3) * 32) >> 4), ID_S, k < QP - 1 || ks > 0);
-                tc_commit(smem_u32(&sm.sfull[j % NS]));
-                tc_commit(smem_u32(&sm.kfree[st]));
+                        for (int ks = 0; ks < HD / 16; ks++)
+                            mma_ts(d, tmem + P::Q0 + k * HALF + ks * 8, b + (((ks >> 2) * (KT * 128) + (ks & 3) * 32) >> 4), ID_S, k < QP - 1 || ks > 0);
+                    tc_commit(smem_u32(&sm.sfull[t % NS]));
+                    tc_commit(smem_u32(&sm.kfree[st]));
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
         // tensor memory is given back only when no product is under way
         if (elected()) tc_commit(smem_u32(&sm.done[0]));
@@ -304,35 +335,38 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
         // ---- O = w V
         constexpr uint32_t ID_O = idesc_of(KIND, 128, HD, 1);
         const uint64_t v_desc = umma_desc_of(smem_u32(sm.v[0]), KT * 128, 1024, 2);
-        for (int j = 0; j < n_tiles && !gave_up(); j++) {
-            const int st = j % STAGES, ob = j % NO;
-            wait(&sm.vready[st], (j / STAGES) & 1);
-            if (j >= NO) wait(&sm.ofree[ob], (j / NO - 1) & 1);
-            wait(&sm.pfull[j % NS], (j / NS) & 1);
-            tc_fence_after();
-            const uint32_t w = tmem + P::S0 + (j % NS) * P::SREG, d = tmem + P::O0 + ob * HD;
-            const uint64_t b = v_desc + (uint32_t)(st * (P::TILE >> 4));
-            if (elected()) {
+        for (int i = 0, t0 = 0; more && !gave_up(); t0 += it.n_tiles, more = item_at(++i, it)) {
+            for (int t = t0; t < t0 + it.n_tiles && !gave_up(); t++) {
+                const int st = t % STAGES, ob = t % NO;
+                wait(&sm.vready[st], (t / STAGES) & 1);
+                if (t >= NO) wait(&sm.ofree[ob], (t / NO - 1) & 1);
+                wait(&sm.pfull[t % NS], (t / NS) & 1);
+                tc_fence_after();
+                const uint32_t w = tmem + P::S0 + (t % NS) * P::SREG, d = tmem + P::O0 + ob * HD;
+                const uint64_t b = v_desc + (uint32_t)(st * (P::TILE >> 4));
+                if (elected()) {
 #pragma unroll
-                for (int k = QP - 1; k >= 0; k--)
+                    for (int k = QP - 1; k >= 0; k--)
 #pragma unroll
-                    for (int ks = 0; ks < KT / 16; ks++)
-                        // 16 keys of all dims: 64-dim halves KT * 128 bytes apart, groups of 8 keys 1024 bytes apart
-                        mma_ts(d, w + (ks >> 1) * (QP * 16) + k * 16 + (ks & 1) * 8, b + (ks * 2048 >> 4), ID_O, k < QP - 1 || ks > 0);
-                tc_commit(smem_u32(&sm.ofull[ob]));
-                tc_commit(smem_u32(&sm.vfree[st]));
+                        for (int ks = 0; ks < KT / 16; ks++)
+                            // 16 keys of all dims: 64-dim halves KT * 128 bytes apart, groups of 8 keys 1024 bytes apart
+                            mma_ts(d, w + (ks >> 1) * (QP * 16) + k * 16 + (ks & 1) * 8, b + (ks * 2048 >> 4), ID_O, k < QP - 1 || ks > 0);
+                    tc_commit(smem_u32(&sm.ofull[ob]));
+                    tc_commit(smem_u32(&sm.vfree[st]));
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
         if (elected()) tc_commit(smem_u32(&sm.done[1]));
         __syncwarp();
         for (uint32_t i = 0; i < SPINS && !__all_sync(0xffffffffu, parked(smem_u32(&sm.done[1]), 0)); i++) {}
     } else if (warp == P::LOOKER) {
         // ---- values that not every row sees
-        for (int j = 0; j < n_tiles && !gave_up(); j++) {
-            const int st = j % STAGES, key0 = tile_key(j);
-            wait(&sm.vfull[st], (j / STAGES) & 1);
-            if (edge_tile(key0)) {
+        for (int i = 0, t0 = 0; more && !gave_up(); t0 += it.n_tiles, more = item_at(++i, it))
+        for (int j = 0; j < it.n_tiles && !gave_up(); j++) {
+            const int st = (t0 + j) % STAGES, key0 = it.key(j), p_min = it.p_min(), p_max = it.p_max();
+            wait(&sm.vfull[st], ((t0 + j) / STAGES) & 1);
+            if (it.edge(a, key0)) {
                 // a quarter of the warp per row of 128 bytes, so that neighbouring lanes read neighbouring pieces
                 uint32_t odd[2] = {0, 0};
 #pragma unroll 4
@@ -372,9 +406,14 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
     } else {
         const int w = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;      // half of the tile's keys, or of the dims; row of the 128
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        int odds = 0;
+        bool again = false;
+        for (int item = 0, t0 = 0; more; t0 += it.n_tiles, more = item_at(++item, it)) {
+        if (it.n_tiles == 0) continue;
+        const int n_tiles = it.n_tiles, row0 = it.row0, row1 = it.row1, kvh = it.kvh, s = it.s;
         const int row = row0 + r / a.group, h = kvh * a.group + r % a.group;
         const bool on = r < a.rq * a.group && row <= row1;
-        const int p = on ? base + row : -1;
+        const int p = on ? it.base + row : -1;
         // q's rows through shared memory (where odd weights will lie): read row by row, taken back a row a thread.  Piece c of row i
         // lies at c ^ i, so that neither side meets a bank twice.
         float4* const stage = reinterpret_cast<float4*>(sm.stage);
@@ -391,6 +430,8 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                 if (i < a.rq * a.group && ri <= row1 && 4 * (x % ROW4) < hd)
                     y[u] = *(const float4*)(a.q + ((size_t)s * a.rows + ri) * a.q_ld + (size_t)(kvh * a.group + i - ig * a.group) * hd + 4 * (x % ROW4));
             }
+            if (again) asm volatile("bar.sync 2, 512;" ::: "memory");      // the item before has left shared memory
+            again = true;
 #pragma unroll
             for (int u = 0; u < SHARE; u++) {
                 const int x = u * 512 + tid, i = x / ROW4;
@@ -442,13 +483,12 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
         if (warp < P::OUT) {
             // ---- softmax
             float m = -INFINITY, l = 0.0f;                         // the denominator of this half's keys, relative to m
-            int odds = 0;
             for (int j = 0; j < n_tiles; j++) {
-                const int b = j & 1, key0 = tile_key(j) + 32 * w;
-                wait(&sm.sfull[j % NS], (j / NS) & 1);
+                const int t = t0 + j, b = t & 1, key0 = it.key(j) + 32 * w;
+                wait(&sm.sfull[t % NS], (t / NS) & 1);
                 tc_fence_after();
-                const uint32_t at = tmem + lanes + P::S0 + (j % NS) * P::SREG;
-                const bool edge = edge_tile(tile_key(j));
+                const uint32_t at = tmem + lanes + P::S0 + (t % NS) * P::SREG;
+                const bool edge = it.edge(a, it.key(j));
                 float v[32];
                 tm_ld<32>(at + P::LEAD + w * 32, v);
                 if (edge) {
@@ -463,15 +503,15 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                     for (int k = 0; k < 4; k++) top[k] = fmaxf(fmaxf(top[k], v[i + k]), v[i + 4 + k]);
 #pragma unroll
                 for (int k = 0; k < 4; k++) top[k] = fmaxf(top[k], v[28 + k]);
-                const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * qs;
+                const float tm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * qs;
                 // the row's other half; behind the barrier both halves of S are in registers
-                sm.top[b][w][r] = t;
+                sm.top[b][w][r] = tm;
                 tc_fence_before();
                 asm volatile("bar.sync 3, 256;" ::: "memory");
                 tc_fence_after();
-                const float m_new = fmaxf(fmaxf(m, t), sm.top[b][1 - w][r]), ms = m_new == -INFINITY ? 0.0f : m_new - SHIFT;
+                const float m_new = fmaxf(fmaxf(m, tm), sm.top[b][1 - w][r]), ms = m_new == -INFINITY ? 0.0f : m_new - SHIFT;
                 const float c = m == -INFINITY ? 0.0f : pow2f(m - m_new);
-                if (w == 0) sm.corr[j & 7][r] = c;
+                if (w == 0) sm.corr[t & 7][r] = c;
                 m = m_new;
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -482,8 +522,8 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                 l = fmaf(l, c, (sum[0] + sum[1]) + (sum[2] + sum[3]));
                 unsigned long long odd = 0;
                 if (edge) {
-                    wait(&sm.vready[j % STAGES], (j / STAGES) & 1);
-                    odd = __shfl_sync(0xffffffffu, sm.odd[j % STAGES], 0);
+                    wait(&sm.vready[t % STAGES], (t / STAGES) & 1);
+                    odd = __shfl_sync(0xffffffffu, sm.odd[t % STAGES], 0);
                     if (odd) {                                     // rare
                         if (odds > 0) wait(&sm.oddfree, (odds - 1) & 1);
                         odds++;
@@ -492,7 +532,7 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                             if (odd >> (32 * w + i) & 1) odd_w[(32 * w + i) * 128 + r] = sees(key0 + i) ? v[i] : -1.0f;
                     }
                 }
-                if (tid == 0) sm.odd_of[j & 7] = odd;
+                if (tid == 0) sm.odd_of[t & 7] = odd;
 #pragma unroll
                 for (int k = 0; k < QP; k++) {
                     uint32_t pk[16];
@@ -503,7 +543,7 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sm.pfull[j % NS]));
+                if (lane == 0) mbar_arrive(smem_u32(&sm.pfull[t % NS]));
             }
             sm.fin[w][0][r] = l;
             sm.fin[w][1][r] = m;
@@ -514,11 +554,11 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
 #pragma unroll
             for (int d = 0; d < HALF; d++) o[d] = 0.0f;
             for (int j = 0; j < n_tiles; j++) {
-                const int ob = j % NO;
-                wait(&sm.ofull[ob], (j / NO) & 1);
+                const int t = t0 + j, ob = t % NO;
+                wait(&sm.ofull[ob], (t / NO) & 1);
                 tc_fence_after();
-                const float c = sm.corr[j & 7][r];
-                const unsigned long long odd = __shfl_sync(0xffffffffu, sm.odd_of[j & 7], 0);
+                const float c = sm.corr[t & 7][r];
+                const unsigned long long odd = __shfl_sync(0xffffffffu, sm.odd_of[t & 7], 0);
                 constexpr int N = HD == 64 ? 32 : 16;
 #pragma unroll
                 for (int d0 = 0; d0 < HALF; d0 += N) {
@@ -532,7 +572,7 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                         if (!(odd >> i & 1)) continue;
                         const float wt = odd_w[i * 128 + r];
                         if (wt < 0.0f) continue;
-                        const int k = tile_key(j) + i, pg = min(max(a.table[(size_t)s * a.max_pages + (k >> a.log_page)], 0), a.n_pages - 1);
+                        const int k = it.key(j) + i, pg = min(max(a.table[(size_t)s * a.max_pages + (k >> a.log_page)], 0), a.n_pages - 1);
                         const uint16_t* vr = (const uint16_t*)a.data + ((((size_t)2 * pg + 1) * a.n_kv + kvh) * a.page + (k & (a.page - 1))) * hd + w * HALF;
 #pragma unroll
                         for (int d = 0; d < HALF; d++)
@@ -547,7 +587,7 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
             }
             // the halves' denominators, the sink, the output
             asm volatile("bar.sync 2, 512;" ::: "memory");
-            if (n_tiles > 0) {
+            {
                 const float m = sm.fin[0][1][r];
                 float l = sm.fin[0][0][r] + sm.fin[1][0][r];
                 if (a.sinks && on) l += m == -INFINITY ? 1.0f : pow2f(a.sinks[h] * LOG2E - m + SHIFT);
@@ -565,6 +605,7 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                             stage[i * ROW4 + ((x % ROW4) ^ (i & (ROW4 - 1)))];
                 }
             }
+        }
         }
     }
     tc_fence_before();
@@ -634,8 +675,8 @@ int fk_attn_prompt_launch(fk_ctx* ctx, cudaStream_t st, const fk_pages* p, int l
     a.first = first;
     a.rq = 128 / a.group;
     a.n_rb = (rows + a.rq - 1) / a.rq;
-    const long long grid = (long long)a.n_rb * a.n_seqs * a.n_kv;
-    if (grid > 0x7fffffffLL) return fk_fail(FK_UNSUPPORTED, "attention_paged: %d rows of %d sequences", rows, p->n_seqs);
+    const long long items = (long long)a.n_rb * a.n_seqs * a.n_kv, grid = items < ctx->sm_count ? items : ctx->sm_count;
+    if (items > 0x7fffffffLL) return fk_fail(FK_UNSUPPORTED, "attention_paged: %d rows of %d sequences", rows, p->n_seqs);
     // shorter heads are zeros behind their last dim: the tiled copy fills what lies outside its tensor
     if (p->kind == KIND_F16) return p->head_dim <= 64 ? launch_prompt<KIND_F16, 64>(ctx, st, a, (unsigned)grid) : launch_prompt<KIND_F16, 128>(ctx, st, a, (unsigned)grid);
     return p->head_dim <= 64 ? launch_prompt<FK_BF16, 64>(ctx, st, a, (unsigned)grid) : launch_prompt<FK_BF16, 128>(ctx, st, a, (unsigned)grid);

@@ -677,10 +677,10 @@ def _rows_of(pg, t, width, what):
     return n, ld if n > 1 else max(ld, width)
 
 
-def _out_like(pg, out, n, width, what):
-    """The result's tensor: a new one, or the caller's."""
+def _out_like(pg, out, q, n, width, what):
+    """The result's tensor: a new one beside q, or the caller's."""
     if out is None:
-        return torch.empty((n, width), dtype=torch.float32, device=pg.data.device)
+        return q.new_empty(n, width)
     if out.dtype != torch.float32 or out.get_device() != pg._dev or out.shape != (n, width) or not out.is_contiguous():
         raise _lib.Invalid(f"{what}: out is a contiguous float32 tensor of q's shape")
     return out
@@ -705,7 +705,7 @@ def rope_kv_paged(q, k, v, pg, layer, n_heads, theta, neox=False, n_new=None, q_
     nv, v_ld = _rows_of(pg, v, pg.n_kv * hd, "rope_kv_paged: v")
     if nk != n or nv != n:
         raise _lib.Invalid("rope_kv_paged: q, k and v have the same number of rows")
-    out = _out_like(pg, out, n, n_heads * hd, "rope_kv_paged")
+    out = _out_like(pg, out, q, n, n_heads * hd, "rope_kv_paged")
     if n == 1:
         q_ld, k_ld, v_ld = n_heads * hd, pg.n_kv * hd, pg.n_kv * hd
     check(lib().fk_rope_kv_paged(pg._ctx, _raw_stream(pg._dev), pg._p, layer, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ld, k_ld, v_ld, n // pg.n_seqs,
@@ -721,7 +721,7 @@ def attention_paged(q, pg, layer, n_heads, n_new=None, scale=None, window=0, fir
     (int32 [n_seqs]) on are left as they were in `out`."""
     width = n_heads * pg.head_dim
     n, ld = _rows_of(pg, q, width, "attention_paged: q")
-    out = _out_like(pg, out, n, width, "attention_paged")
+    out = _out_like(pg, out, q, n, width, "attention_paged")
     check(lib().fk_attention_paged(pg._ctx, _raw_stream(pg._dev), pg._p, layer, q.data_ptr(), ld if n > 1 else width, n // pg.n_seqs,
                                    _counts(pg, n_new), n_heads, pg._scale if scale is None else scale, window, first,
                                    _vec(pg, sinks, n_heads, "attention_paged: sinks"), out.data_ptr()))
@@ -746,7 +746,8 @@ def logit_rules(logits, history=None, penalties=None, bias=None, mask=None, out=
     h, hp, pen, bp, b_ld, mp, m_ld = 0, None, None, None, 0, None, 0
     if history is not None:
         hist = history if history.dim() == 2 else history[None]
-        if hist.dtype != torch.int32 or hist.get_device() != dev or hist.dim() != 2 or hist.shape[0] != n or not hist.is_contiguous():
+        at = hist.shape
+        if hist.dtype != torch.int32 or hist.get_device() != dev or len(at) != 2 or at[0] != n or not hist.is_contiguous():
             raise _lib.Invalid("logit_rules: history is a contiguous int32 tensor [n, h] beside the logits")
         if penalties is None:
             raise _lib.Invalid("logit_rules: a history needs penalties (repeat, frequency, presence)")
@@ -755,20 +756,20 @@ def logit_rules(logits, history=None, penalties=None, bias=None, mask=None, out=
         pen = penalties if penalties.is_contiguous() else penalties.contiguous()
         if pen.dtype != torch.float32 or pen.get_device() != dev or pen.shape != (n, 3):
             raise _lib.Invalid("logit_rules: penalties are float32 [n, 3]: repeat, frequency, presence")
-        h = hist.shape[1]
+        h = at[1]
         hp = hist.data_ptr() if h else None
     if bias is not None:
         bp, b_ld = _rule_rows(bias, torch.float32, dev, n, V, "bias is float32 [vocab] or [n, vocab]")
     if mask is not None:
         mp, m_ld = _rule_rows(mask, torch.int32, dev, n, (V + 31) // 32, "mask is int32 words [ceil(vocab / 32)] or [n, ...]")
     if out is None:
-        o = torch.empty((n, V), dtype=torch.float32, device=x.device)
+        o = x.new_empty(n, V)
     else:
         o = out if out.dim() == 2 else out[None]
         if o.shape != (n, V) or o.dtype != torch.float32 or o.get_device() != dev or not o.is_contiguous():
             raise _lib.Invalid("logit_rules: out is a contiguous float32 tensor of the logits' shape")
     if tokens is None:
-        tokens = torch.empty(n, dtype=torch.int32, device=x.device)
+        tokens = x.new_empty(n, dtype=torch.int32)
     elif tokens.shape != (n,) or tokens.dtype != torch.int32 or tokens.get_device() != dev or not tokens.is_contiguous():
         raise _lib.Invalid("logit_rules: tokens is a contiguous int32 tensor [n]")
     ctx = _contexts.get(dev) or context(x.device)
