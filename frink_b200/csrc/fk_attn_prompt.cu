@@ -636,10 +636,11 @@ bool fk_attn_prompt_takes(fk_ctx* ctx, const fk_pages* p, int rows, int n_heads)
     const int group = n_heads / p->n_kv;
     if (p->kind == KIND_F32 || group > 128) return false;
     if ((long long)p->n_pages * 2 * p->n_kv * p->page > 0x7fffffffLL) return false;      // a token's row number is 32 bits
-    // This kernel takes 23 ns an SM for a key of a tile of 128 columns, whatever of the tile is filled, and does not split the
-    // keys; the other takes 14 ns an SM for a key of 16 columns and spreads over all SMs (bf16, heads of 128; f16 heads of 64: 13
-    // and 7.6).  24/8 heads of 128, one sequence after 8000 tokens, us here / there: 64 rows 196 / 82, 128 rows 200 / 157, 256
-    // rows 209 / 299; four sequences: 24 rows 198 / 140, 43 rows 204 / 250.
+    // This kernel takes 19 ns an SM for a key of a tile of 128 columns, whatever of the tile is filled, and does not split the
+    // keys; the other takes 13 ns an SM for a key of 16 columns and spreads over all SMs (bf16, heads of 128; f16 heads of 64: 15
+    // and 7).  24/8 heads of 128, one sequence after 8000 tokens, us here / there: 64 rows 161 / 86, 128 rows 164 / 154, 256
+    // rows 167 / 302; four sequences: 24 rows 161 / 138, 43 rows 164 / 248.  64/8 heads of 64, f16, 64 rows 124 / 112, 128 rows
+    // 127 / 214.
     const long long tiles = (long long)p->n_seqs * p->n_kv * ((rows + 128 / group - 1) / (128 / group));
     const long long blocks = (long long)p->n_seqs * p->n_kv * (((long long)rows * group + 15) / 16);
     return 3 * blocks > 5 * ctx->sm_count * ((tiles + ctx->sm_count - 1) / ctx->sm_count);

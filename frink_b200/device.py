@@ -608,6 +608,7 @@ class Pages:
 
 
 # These calls are a few microseconds of GPU work: the checks read each attribute once, the stream comes as its plain handle.
+_F32, _I32 = torch.float32, torch.int32
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda i: torch.cuda.current_stream(i).cuda_stream
 
 
@@ -665,23 +666,26 @@ def pages_compact(pg):
 
 def _rows_of(pg, t, width, what):
     """t [n_seqs * rows, width], any row stride -> (number of rows, row stride)."""
-    if t.dtype != torch.float32 or t.get_device() != pg._dev or t.dim() != 2:
+    at = t.shape
+    if t.dtype is not _F32 or t.get_device() != pg._dev or len(at) != 2:
         raise _lib.Invalid(f"{what}: float32 rows of {width} on the pages' device")
-    (n, w), (ld, one) = t.shape, t.stride()
+    (n, w), (ld, one) = at, t.stride()
     if w != width or one != 1:
         raise _lib.Invalid(f"{what}: float32 rows of {width}, their values side by side")
     if n == 0 or n % pg.n_seqs:
         raise _lib.Invalid(f"{what}: {n} rows for {pg.n_seqs} sequences")
-    if n > 1 and ld < width:
-        raise _lib.Invalid(f"{what}: rows of {width} floats that lie over one another")
-    return n, ld if n > 1 else max(ld, width)
+    if ld < width:
+        if n > 1:
+            raise _lib.Invalid(f"{what}: rows of {width} floats that lie over one another")
+        ld = width
+    return n, ld
 
 
 def _out_like(pg, out, q, n, width, what):
     """The result's tensor: a new one beside q, or the caller's."""
     if out is None:
         return q.new_empty(n, width)
-    if out.dtype != torch.float32 or out.get_device() != pg._dev or out.shape != (n, width) or not out.is_contiguous():
+    if out.dtype is not _F32 or out.get_device() != pg._dev or out.shape != (n, width) or not out.is_contiguous():
         raise _lib.Invalid(f"{what}: out is a contiguous float32 tensor of q's shape")
     return out
 
@@ -690,7 +694,7 @@ def _vec(pg, t, n, what):
     """An optional contiguous float32 vector of n values on the pages' device -> its address."""
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.get_device() != pg._dev or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not _F32 or t.get_device() != pg._dev or t.numel() != n or not t.is_contiguous():
         raise _lib.Invalid(f"{what}: {n} contiguous float32 values on the pages' device")
     return t.data_ptr()
 
@@ -733,12 +737,12 @@ def logit_rules(logits, history=None, penalties=None, bias=None, mask=None, out=
     """What a sampler does to logits [n, vocab] (or one row) before it picks, and the greedy pick -> (changed logits, tokens
     int32 [n]).  history [n, h] int32: the tokens that came before (entries outside the vocabulary are empty places); a token
     that occurs c > 0 times has its logit divided (if positive, else multiplied) by repeat, less c * frequency, less presence
-    (penalties: float32 [n, 3], or one triple for all rows: numbers of the host, so not while a graph is captured).  bias [vocab] or [n, vocab] is added, then logits whose bit in mask
-    (int32 words [words] or [n, words], bit v % 32 of word v / 32) is clear become -inf.  tokens: the largest, ties to the lower
-    index; -1 where nothing is left."""
+    (penalties: float32 [n, 3], or one triple for all rows: numbers of the host, so not while a graph is captured).  bias [vocab]
+    or [n, vocab] is added, then logits whose bit in mask (int32 words [words] or [n, words], bit v % 32 of word v / 32) is clear
+    become -inf.  tokens: the largest, ties to the lower index; -1 where nothing is left."""
     x = logits if logits.dim() == 2 else logits[None]
     dev = x.get_device()
-    if dev < 0 or x.dtype != torch.float32 or x.dim() != 2:
+    if dev < 0 or x.dtype is not _F32 or x.dim() != 2:
         raise _lib.Invalid("logit_rules: float32 CUDA logits [n, vocab]")
     (n, V), (ld, one) = x.shape, x.stride()
     if one != 1 or n == 0 or V == 0:
@@ -747,14 +751,14 @@ def logit_rules(logits, history=None, penalties=None, bias=None, mask=None, out=
     if history is not None:
         hist = history if history.dim() == 2 else history[None]
         at = hist.shape
-        if hist.dtype != torch.int32 or hist.get_device() != dev or len(at) != 2 or at[0] != n or not hist.is_contiguous():
+        if hist.dtype is not _I32 or hist.get_device() != dev or len(at) != 2 or at[0] != n or not hist.is_contiguous():
             raise _lib.Invalid("logit_rules: history is a contiguous int32 tensor [n, h] beside the logits")
         if penalties is None:
             raise _lib.Invalid("logit_rules: a history needs penalties (repeat, frequency, presence)")
         if not isinstance(penalties, torch.Tensor):
             penalties = torch.tensor([[float(v) for v in penalties]], dtype=torch.float32).to(x.device).expand(n, -1)
         pen = penalties if penalties.is_contiguous() else penalties.contiguous()
-        if pen.dtype != torch.float32 or pen.get_device() != dev or pen.shape != (n, 3):
+        if pen.dtype is not _F32 or pen.get_device() != dev or pen.shape != (n, 3):
             raise _lib.Invalid("logit_rules: penalties are float32 [n, 3]: repeat, frequency, presence")
         h = at[1]
         hp = hist.data_ptr() if h else None
@@ -766,11 +770,11 @@ def logit_rules(logits, history=None, penalties=None, bias=None, mask=None, out=
         o = x.new_empty(n, V)
     else:
         o = out if out.dim() == 2 else out[None]
-        if o.shape != (n, V) or o.dtype != torch.float32 or o.get_device() != dev or not o.is_contiguous():
+        if o.shape != (n, V) or o.dtype is not _F32 or o.get_device() != dev or not o.is_contiguous():
             raise _lib.Invalid("logit_rules: out is a contiguous float32 tensor of the logits' shape")
     if tokens is None:
         tokens = x.new_empty(n, dtype=torch.int32)
-    elif tokens.shape != (n,) or tokens.dtype != torch.int32 or tokens.get_device() != dev or not tokens.is_contiguous():
+    elif tokens.shape != (n,) or tokens.dtype is not _I32 or tokens.get_device() != dev or not tokens.is_contiguous():
         raise _lib.Invalid("logit_rules: tokens is a contiguous int32 tensor [n]")
     ctx = _contexts.get(dev) or context(x.device)
     check(lib().fk_logit_rules(ctx, _raw_stream(dev), x.data_ptr(), ld if n > 1 else max(ld, V), n, V, hp, h,
