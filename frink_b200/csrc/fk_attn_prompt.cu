@@ -3,8 +3,8 @@
 //
 // An item is 128 (row, query head) pairs of one KV head -- 128 / group consecutive rows, so a short prompt still fills the
 // tile -- and the visible keys in tiles of 64.  There is a CTA per SM, which goes through its items with the rings running on:
-// the next item's first tiles and q are on their way while the current one ends (a CTA per item: 430 us where this takes 393,
-// see below).  A tile:
+// the next item's first tiles and q are on their way while the current one ends (the last case below: 393 us, 430 with a CTA per
+// item).  A tile:
 //
 //   S = q K^T          A = q's parts in tensor memory, B = a tile of K in shared memory, S in tensor memory (two or three buffers)
 //   w = 2^(S - m)      a thread per row; its parts go back over S as the next product's A operand
@@ -25,10 +25,11 @@
 // values of tiles that not every row sees: a value that no row sees is zeroed in shared memory (stale memory may hold NaN); one
 // that some rows see and that is not finite is zeroed too and added in plain f32 for the rows that see it.
 //
-// Measured (B200): 512 rows of 24/8 heads of 128, bf16, empty cache 23.9 us; 4200 rows 315 us = 344 TFLOP/s of the formula's
-// operations, three times that of MMA, f16 287 us; 1001, 801, 601 and 401 rows after 2000 to 8000 tokens, window 2048, 64/8
-// heads of 64, f16, 393 us.  What bounds it is a tile's chain from scores to weights (f16 heads of 64: tensor pipe 22 %, issue
-// slots 45 %) and, bf16 heads of 128, the products' own time on top of it; an item alone is bound by its way in and out.
+// Measured (B200): 512 rows of 24/8 heads of 128, bf16, empty cache 23.2 us; 4200 rows 316 us = 343 TFLOP/s of the formula's
+// operations, three times that of MMA, f16 276 us; 1001, 801, 601 and 401 rows after 2000 to 8000 tokens, window 2048, 64/8
+// heads of 64, f16, 386 us.  What bounds it is a tile's chain from scores to weights (tensor pipe 25 %, issue slots 53 %): with
+// one part of each product instead of two or three the last case gains 3 % and the bf16 one 6 %, without the exponentials and
+// the parts' arithmetic 20 and 9 %.  An item alone is bound by its way in and out.
 #include "fk_paged.cuh"
 #include "fk_tc.cuh"
 
@@ -136,19 +137,31 @@ __device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
+// two at a time: the last case 393 -> 386 us, f16 heads of 128 286 -> 276
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(*(uint64_t*)&a), "l"(*(uint64_t*)&b), "l"(*(uint64_t*)&c));
+    return *(float2*)&r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*(uint64_t*)&a), "l"(*(uint64_t*)&b));
+    return *(float2*)&r;
+}
 // (lo, hi) rounded to a pair of the type; lo and hi become what is left
 template <int KIND> __device__ __forceinline__ uint32_t take_part(float& lo, float& hi) {
     uint32_t r;
+    float2 h;
     if (KIND == KIND_F16) {
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-        const __half2 h = *(const __half2*)&r;
-        lo -= __low2float(h);
-        hi -= __high2float(h);
+        h = __half22float2(*(const __half2*)&r);
     } else {
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-        lo -= __uint_as_float(r << 16);
-        hi -= __uint_as_float(r & 0xffff0000u);
+        h = make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
     }
+    const float2 left = fma2(h, make_float2(-1.0f, -1.0f), make_float2(lo, hi));
+    lo = left.x;
+    hi = left.y;
     return r;
 }
 template <int N> __device__ __forceinline__ void tm_ld(uint32_t addr, float* v) {
@@ -513,13 +526,15 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                 const float c = m == -INFINITY ? 0.0f : pow2f(m - m_new);
                 if (w == 0) sm.corr[t & 7][r] = c;
                 m = m_new;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    v[i] = pow2f(fmaf(v[i], qs, -ms));
-                    sum[i & 3] += v[i];
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 x = fma2(make_float2(v[i], v[i + 1]), make_float2(qs, qs), make_float2(-ms, -ms));
+                    v[i] = pow2f(x.x);
+                    v[i + 1] = pow2f(x.y);
+                    sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(v[i], v[i + 1]));
                 }
-                l = fmaf(l, c, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                l = fmaf(l, c, (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
                 unsigned long long odd = 0;
                 if (edge) {
                     wait(&sm.vready[t % STAGES], (t / STAGES) & 1);
@@ -565,7 +580,11 @@ __global__ void __launch_bounds__((Plan<KIND, HD>::THREADS), 1) attn_prompt_kern
                     float x[N];
                     tm_ld<N>(tmem + lanes + P::O0 + ob * HD + w * HALF + d0, x);
 #pragma unroll
-                    for (int d = 0; d < N; d++) o[d0 + d] = fmaf(o[d0 + d], c, x[d]);
+                    for (int d = 0; d < N; d += 2) {
+                        const float2 y = fma2(make_float2(o[d0 + d], o[d0 + d + 1]), make_float2(c, c), make_float2(x[d], x[d + 1]));
+                        o[d0 + d] = y.x;
+                        o[d0 + d + 1] = y.y;
+                    }
                 }
                 if (odd) {                                         // rare: values that are not finite, for the rows that see them
                     for (int i = 0; i < KT; i++) {
