@@ -232,8 +232,8 @@ fork_kernel(int* table, int* lens, int* refs, int n_pages, int page, int max_pag
     }
 }
 
-// Four forks of 1000 tokens in 28 layers are 14 us with the deciding block, all of it latency: two dependent launches, and in the
-// first a chain of table reads, the scan for free pages, the table's and the counts' writes.
+// Four forks of 1000 tokens in 28 layers, with the frees before and the growth behind them, are 14 us, all of it latency: four
+// dependent launches, three of them a chain of table reads, the scan for free pages, the table's and the counts' writes.
 // The last, partly filled pages: `part` tokens of every head, K and V, of every layer.  blockIdx.x: fork, blockIdx.y: layer.
 __global__ void __launch_bounds__(256)
 copy_parts_kernel(char* __restrict__ data, const CopyItem* __restrict__ items, size_t layer_bytes, size_t page_bytes, int heads2, int head_bytes, int row_bytes) {

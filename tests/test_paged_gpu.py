@@ -512,6 +512,15 @@ def test_prompt_values_behind_a_mask_do_not_matter(dtype, x):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,n_kv,hd,window", [(16, 8, 64, 300), (16, 8, 128, 0), (30, 10, 96, 64), (24, 24, 40, 1000)])
+def test_prompt_of_several_items_a_cta(dtype, heads, n_kv, hd, window):
+    """Hundreds of (row block, KV head) items, some of rows that do not exist, bad tokens in several of them."""
+    nan, inf = float("nan"), float("inf")
+    attend_fast([0, 90, 200, 31], [1500, 0, 700, 1], 1500, heads, n_kv, hd, 16, TYPES[dtype], window=window, first=5 if window else 0, sinks=True, seed=hd,
+                bad=[(0, 700, nan), (0, 702, inf), (0, 1400, inf), (2, 300, nan), (2, 850, inf), (2, 899, nan), (3, 31, inf)])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_a_long_prompt_keeps_its_precision_and_repeats(dtype):
     a = attend_fast([20000], [256], 256, 4, 1, 128, 128, TYPES[dtype], seed=6)
     assert torch.equal(a, attend_fast([20000], [256], 256, 4, 1, 128, 128, TYPES[dtype], seed=6))
