@@ -867,7 +867,8 @@ template <int KIND, int HDP, bool EXACT, int NT> int launch_attn(fk_ctx* ctx, cu
     a.n_cb = (int)(((long long)a.rows * a.group + 8 * NT - 1) / (8 * NT));
     const long long entries = (long long)a.n_cb * a.n_seqs;
     if (entries * a.n_kv > 0x7fffffffLL) return fk_fail(FK_UNSUPPORTED, "attention_paged: %d rows of %d sequences", a.rows, a.n_seqs);
-    a.whole = entries > MAX_ENTRIES;
+    // the deal counts slots in 32 bits, full table rows' too
+    a.whole = entries > MAX_ENTRIES || entries * ((long long)a.max_pages * a.page / (16 * WARPS * Ring<KIND, HDP>::SUB) + 2) > 1 << 30;
     const int ctas = per_sm * ctx->sm_count;
     const unsigned grid = a.whole ? (unsigned)(entries * a.n_kv) : (unsigned)(ctas < MAX_CTAS ? ctas : MAX_CTAS);
     FK_CUDA(launch(kern, dim3(grid), dim3(WARPS * 32), smem, st, a), FK_LAUNCH);

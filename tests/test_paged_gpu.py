@@ -586,3 +586,17 @@ def test_more_missing_pages_than_32_bits_count():
 def test_more_columns_than_the_deal_holds():
     """Tens of thousands of (sequence, block of columns) pairs of 32-bit pages."""
     attend([10, 0], [2050, 7], 2050, 130, 1, 8, 64, torch.float32, window=60, first=2, sinks=True, seed=9, ragged=True)
+
+
+def test_table_rows_of_two_million_pages():
+    """Rows so long that the work of full ones would not be counted in 32 bits."""
+    from frink_b200 import device
+    n, lens = 512, torch.arange(512, dtype=torch.int32, device="cuda") % 127
+    data = torch.randn((1, n, 2, 1, 128, 8), generator=torch.Generator().manual_seed(8)).bfloat16().cuda()
+    table = torch.full((n, (1 << 21) + 1), -1, dtype=torch.int32, device="cuda")
+    table[:, 0] = torch.arange(n, device="cuda").flip(0)
+    refs = torch.ones(n, dtype=torch.int32, device="cuda")
+    q = queries(n, 16, 5).cuda()
+    short = device.attention_paged(q, device.Pages(data, table[:, :1].contiguous(), lens, refs), 0, 2)
+    full = device.attention_paged(q, device.Pages(data, table, lens, refs), 0, 2)
+    assert device.device_error() == 0 and rel_l2(full.cpu().numpy(), short.cpu().numpy()) <= 2 * TOL
