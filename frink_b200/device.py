@@ -563,7 +563,9 @@ class _CPages(C.Structure):
 class Pages:
     """A KV cache of pages shared by many sequences: data [n_layers, n_pages, 2, n_kv, page, head_dim] (float32, float16 or
     bfloat16; page 16, 32, 64 or 128), table [n_seqs, max_pages] int32 (-1: no page), lens [n_seqs] int32, refs [n_pages]
-    int32.  The tensors stay the caller's; the workspace is this object's, and calls on it belong on one stream at a time."""
+    int32.  The tensors stay the caller's; the workspace is this object's, and calls on it belong on one stream at a time.
+    A cache of some of the pool's sequences (`seq`, or rows of the table) serves every call but `pages_compact`, which moves
+    pages and so needs the rows of all."""
 
     def __init__(self, data, table, lens, refs, _ws=None):
         if data.dim() != 6 or data.shape[2] != 2 or data.dtype not in _PAGE_KINDS:
@@ -581,12 +583,13 @@ class Pages:
         self.n_layers, self.n_pages, self.page, self.n_kv, self.head_dim = n_layers, n_pages, page, n_kv, hd
         self.n_seqs, self.max_pages = table.shape
         self._ctx = context(data.device)
-        if _ws is None:
+        whole = _ws is None                               # a view goes by its cache's workspace
+        if whole:
             need = lib().fk_pages_workspace(self._ctx, n_pages)
             _ws = torch.empty(need + 256, dtype=torch.uint8, device=data.device)
             _ws[:8192 + 256].zero_()                      # the arrival counters; what lies behind them is scratch
             torch.cuda.current_stream(data.device).synchronize()    # whatever stream the first call comes on
-        self._ws = _ws
+        self._ws, self._whole = _ws, whole
         base = (_ws.data_ptr() + 255) & ~255
         self._c = _CPages(data.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), base, _ws.numel() - (base - _ws.data_ptr()),
                           _PAGE_KINDS[data.dtype], n_layers, n_pages, page, n_kv, hd, self.n_seqs, self.max_pages)
@@ -658,7 +661,10 @@ def pages_free(pg, seqs):
 
 
 def pages_compact(pg):
-    """Moves the pages in use to the front of the pool -> their number (int32 [1] on the device)."""
+    """Moves the pages in use to the front of the pool -> their number (int32 [1] on the device).  pg's table holds every
+    sequence of the pool: one that it leaves out would keep the old numbers of pages that have moved."""
+    if not pg._whole:
+        raise _lib.Invalid("pages_compact: one sequence's view of a cache (the pages of the others would move under them)")
     used = torch.empty(1, dtype=torch.int32, device=pg.data.device)
     check(lib().fk_pages_compact(pg._ctx, _raw_stream(pg._dev), pg._p, used.data_ptr()))
     return used

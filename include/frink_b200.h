@@ -420,7 +420,9 @@ int fk_pages_fork(fk_ctx* ctx, void* stream, const fk_pages* pages, const int* s
 /* The listed sequences (each once, m <= 64) give their pages back and hold nothing. */
 int fk_pages_free(fk_ctx* ctx, void* stream, const fk_pages* pages, const int* seqs_host, int m);
 /* Moves the pages in use to the front: the k-th used page at or behind position U = pages in use goes to the k-th free page
- * before it, in every layer; tables and counts follow.  *used_dev = U. */
+ * before it, in every layer; tables and counts follow.  *used_dev = U.  The table must hold every sequence of the pool: the
+ * other calls also serve some of its rows (table_dev, lens_dev and n_seqs of those), but here a row that is left out would keep
+ * the old numbers of pages that have moved. */
 int fk_pages_compact(fk_ctx* ctx, void* stream, const fk_pages* pages, int* used_dev);
 /* fk_rope_kv into pages: `rows` rows a sequence (q, k, v rows s * rows + i; q_ld, k_ld, v_ld floats apart), row i of
  * sequence s at position lens[s] + i, rows i >= n_new_dev[s] (null: none) skipped.  The rotated q goes to q_out_dev
