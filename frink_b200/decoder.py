@@ -147,7 +147,12 @@ class LogitRules:
     """What a server does to n sequences' logits before it takes the largest: penalties (repeat, frequency, presence; one triple,
     or [n, 3]) for the `last` most recent tokens, a bias [vocab] or [n, vocab], and a grammar's mask of int32 words (bit v % 32
     of word v / 32 set: token v may follow), one row or [n, words].  bias and mask may be rewritten in place between steps, of a
-    captured step too.  A sequence that nothing may follow gets token -1."""
+    captured step too.  A sequence that nothing may follow gets token -1.
+
+    history [n, last] holds the token at position p of row's sequence in place p % last (-1: none), at [n] the position behind
+    the last one.  `Decoder` keeps both with the sequences: a prompt of a sequence that held nothing starts its row anew, rows that
+    a step leaves out stay as they are.  A fork's row is the caller's: `copy` where all tokens were taken over, else `forget`
+    and `see`."""
 
     def __init__(self, n, penalties=(1.0, 0.0, 0.0), last=64, bias=None, mask=None, device="cuda"):
         if last < 1:
@@ -160,14 +165,18 @@ class LogitRules:
         self.history = torch.full((n, last), -1, dtype=torch.int32, device=device)
         self.at = torch.zeros(n, dtype=torch.int64, device=device)
 
-    def see(self, row, ids):
-        """Tokens that row's sequence begins with (a prompt): only the most recent ones stay."""
+    def see(self, row, ids, at=None):
+        """More tokens of row's sequence (a prompt): only the most recent ones stay.  at: the position of the first (an int or a
+        device tensor of one; default: behind those that were seen)."""
+        n = ids.numel()
         ids = ids.reshape(-1)[-self.last:].to(torch.int32)
-        where = (self.at[row] + torch.arange(ids.numel(), device=ids.device)) % self.last
+        end = (self.at[row:row + 1] if at is None else at) + n
+        where = (end - ids.numel() + torch.arange(ids.numel(), device=ids.device)) % self.last
         self.history[row, where] = ids
-        self.at[row] += ids.numel()
+        self.at[row] = end
 
     def forget(self, row):
+        """Row's history is empty again (a sequence that has nothing to do with the one before)."""
         self.history[row] = -1
         self.at[row] = 0
 
@@ -179,16 +188,20 @@ class LogitRules:
     def _row(self, t, row):
         return t if t is None or t.dim() == 1 else t[row:row + 1]
 
-    def pick(self, ops, logits, row=None):
-        """logits [n, vocab] (or row's alone) -> tokens, which join the histories."""
+    def pick(self, ops, logits, row=None, moves=None):
+        """logits [n, vocab] (or row's alone) -> tokens, which join the histories.  moves [n] (0 or 1): the history of a row that
+        does not move stays as it is."""
         if row is None:
             h, at, pen, bias, mask = self.history, self.at, self.penalties, self.bias, self.mask
         else:
             h, at, pen = self.history[row:row + 1], self.at[row:row + 1], self.penalties[row:row + 1]
             bias, mask = self._row(self.bias, row), self._row(self.mask, row)
         _, tok = ops.logit_rules(logits, history=h, penalties=pen, bias=bias, mask=mask)
-        h.scatter_(1, (at % self.last)[:, None], tok[:, None])
-        at.add_(1)
+        slot, new, on = (at % self.last)[:, None], tok[:, None], 1
+        if moves is not None:
+            on, new = moves, torch.where(moves[:, None] > 0, new, h.gather(1, slot))
+        h.scatter_(1, slot, new)
+        at.add_(on)
         return tok
 
 
@@ -531,8 +544,9 @@ class Decoder:
     def _live(self, s, on):
         self.page_live[s:s + 1].fill_(int(on))
 
-    def forward_pages_seq(self, s, ids):
-        """More tokens of sequence s (a prompt, or its next chunk) -> logits of the last one [1, vocab]."""
+    def forward_pages_seq(self, s, ids, rules=None):
+        """More tokens of sequence s (a prompt, or its next chunk) -> logits of the last one [1, vocab].  rules: whose history
+        the tokens join."""
         self._sequences([s])
         n = ids.numel()
         add = [n if i == s else 0 for i in range(len(self._pool.lens))]
@@ -541,18 +555,19 @@ class Decoder:
         self.ops.pages_grow(pg, n)
         paged = (pg, None)
         logits = self._forward_fused(ids, paged=paged) if self._fuses(n) else self._forward_wide(ids, paged=paged)
+        if rules is not None:
+            if not self._pool.lens[s]:
+                rules.forget(s)
+            rules.see(s, ids, at=pg.lens)
         self.ops.pages_advance(pg, n)
         self._pool.advance(add)
         self._live(s, True)
         return logits
 
     def prefill_pages(self, s, prompt_ids, rules=None):
-        """Sequence s's prompt -> its first generated token (device int32 [1])."""
-        logits = self.forward_pages_seq(s, prompt_ids)
-        if rules is None:
-            return self.ops.argmax(logits)
-        rules.see(s, prompt_ids)
-        return rules.pick(self.ops, logits, row=s)
+        """Sequence s's prompt (or the last chunk of it) -> its first generated token (device int32 [1])."""
+        logits = self.forward_pages_seq(s, prompt_ids, rules)
+        return self.ops.argmax(logits) if rules is None else rules.pick(self.ops, logits, row=s)
 
     def forward_pages(self, toks):
         """toks [n_seqs] (device int32), every sequence's newest token -> logits [n_seqs, vocab]; the sequences that hold
@@ -576,7 +591,7 @@ class Decoder:
 
     def _pick(self, logits, rules):
         if rules is not None:
-            return rules.pick(self.ops, logits)
+            return rules.pick(self.ops, logits, moves=self.page_live)
         return torch.cat([self.ops.argmax(logits[i:i + 64]) for i in range(0, logits.shape[0], 64)])
 
     def step_pages(self, toks, rules=None):
@@ -615,7 +630,8 @@ class Decoder:
         self._pool.advance(add)
 
     def fork_pages(self, src, dst, n=None):
-        """Sequence dst[i] (empty) becomes the first n[i] (default: all) tokens of src[i]; whole pages are shared."""
+        """Sequence dst[i] (empty) becomes the first n[i] (default: all) tokens of src[i]; whole pages are shared.  Rules follow by
+        `LogitRules.copy`, or by `forget` and `see` where not all tokens were taken."""
         src, dst = self._sequences(src), self._sequences(dst)
         if len(src) != len(dst) or (n is not None and len(n) != len(src)):
             raise ValueError("lists of one length")
@@ -781,12 +797,17 @@ class Decoder:
 
     def generate(self, prompt_ids, n_new, use_graph=False, rules=None):
         """Greedy: returns the n_new generated token ids (list of int).  rules (`LogitRules` of one sequence): what happens to the
-        logits first; the token is then -1 where nothing may follow, and generation ends there."""
+        logits first; the token is then -1 where nothing may follow, and generation ends there.  Their history starts anew where
+        the caches are empty, and goes on where the prompt does."""
         if rules is not None:
             if use_graph:
                 raise ValueError("rules run eagerly here; a captured step with rules is capture_pages'")
-            rules.see(0, prompt_ids)
-            tok = rules.pick(self.ops, self.forward(prompt_ids))
+            at = self._pos_host
+            logits = self.forward(prompt_ids)
+            if at == 0:
+                rules.forget(0)
+            rules.see(0, prompt_ids, at=at)
+            tok = rules.pick(self.ops, logits)
             outs = [int(tok.item())]
             while len(outs) < n_new and outs[-1] >= 0:
                 tok = rules.pick(self.ops, self.forward(tok))

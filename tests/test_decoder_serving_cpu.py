@@ -1,0 +1,120 @@
+"""`Decoder` over pages as a server drives it, on the CPU stand-ins: slots that are idle, freed and filled again, under rules."""
+import numpy as np
+import pytest
+import torch
+
+from frink_b200.decoder import Decoder, LogitRules
+from oracle import frink_oracle as fo
+from tests import paged_ops
+from tests.helpers import tiny_gpt_oss
+
+PRESENCE = (1.0, 0.0, 100.0)       # a token that occurred before is not picked again
+
+
+def model(**kw):
+    cfg, layers, tok, out_norm, head = tiny_gpt_oss()
+    return Decoder(cfg, layers, tok, fo.BF16, out_norm, output=head, output_kind=fo.BF16, max_seq=64, ops=paged_ops, device="cpu", **kw)
+
+
+def ids(n, seed):
+    return torch.from_numpy(np.random.default_rng(seed).integers(0, 512, n).astype(np.int32))
+
+
+def alone(prompt, n, **kw):
+    """The tokens of a sequence that is the only one, in a cache of its own."""
+    dec, rules = model(), LogitRules(1, device="cpu", **kw)
+    dec.alloc_pages(1, 4, page=16, dtype=torch.float32)
+    cur = dec.prefill_pages(0, prompt, rules)
+    out = [int(cur)]
+    for _ in range(n - 1):
+        cur = dec.step_pages(cur, rules)
+        out.append(int(cur))
+    return out
+
+
+def steps(dec, rules, cur, n, slot):
+    """n more steps of all slots -> slot's tokens."""
+    out = []
+    for _ in range(n):
+        cur.copy_(dec.step_pages(cur, rules))
+        out.append(int(cur[slot]))
+    return out
+
+
+def serving(n_seqs=2, **kw):
+    dec, rules = model(), LogitRules(n_seqs, penalties=PRESENCE, device="cpu", **kw)
+    dec.alloc_pages(n_seqs, 4 * n_seqs, page=16, dtype=torch.float32)
+    return dec, rules, torch.zeros(n_seqs, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("seed", range(3))
+def test_a_slot_that_was_idle_answers_as_a_sequence_alone(seed):
+    dec, rules, cur = serving()
+    cur[0] = dec.prefill_pages(0, ids(9, seed), rules)
+    steps(dec, rules, cur, 12, 0)
+    assert rules.history[1].tolist() == [-1] * 64 and int(rules.at[1]) == 0
+    prompt = ids(7, 50 + seed)
+    cur[1] = dec.prefill_pages(1, prompt, rules)
+    assert [int(cur[1])] + steps(dec, rules, cur, 5, 1) == alone(prompt, 6, penalties=PRESENCE)
+
+
+@pytest.mark.parametrize("forget", [False, True])
+def test_a_slot_that_was_freed_and_idle_answers_as_a_sequence_alone(forget):
+    dec, rules, cur = serving()
+    for s in range(2):
+        cur[s] = dec.prefill_pages(s, ids(8 + s, s), rules)
+    steps(dec, rules, cur, 6, 1)
+    dec.free_pages([1])
+    if forget:
+        rules.forget(1)
+    before = rules.history[1].clone()
+    steps(dec, rules, cur, 5, 0)
+    assert torch.equal(rules.history[1], before)
+    prompt = ids(6, 77)
+    cur[1] = dec.prefill_pages(1, prompt, rules)
+    assert [int(cur[1])] + steps(dec, rules, cur, 5, 1) == alone(prompt, 6, penalties=PRESENCE)
+
+
+@pytest.mark.parametrize("last", [3, 64])
+def test_a_prompt_in_chunks_is_remembered_whole(last):
+    prompt = ids(23, 5)
+    dec, rules, cur = serving(last=last)
+    dec.forward_pages_seq(1, prompt[:9], rules)
+    dec.forward_pages_seq(1, prompt[9:11], rules)
+    cur[1] = dec.prefill_pages(1, prompt[11:], rules)
+    assert [int(cur[1])] + steps(dec, rules, cur, 4, 1) == alone(prompt, 5, penalties=PRESENCE, last=last)
+    assert sorted(rules.history[1].tolist()) == sorted(([-1] * 64 + prompt.tolist() + alone(prompt, 5, penalties=PRESENCE, last=last))[-last:])
+
+
+def test_a_picked_token_that_begins_the_next_chunk_is_counted_once():
+    """A conversation's second turn: its chunk begins with the last token that was picked, which no step has read yet."""
+    prompt, turn = ids(9, 6), ids(4, 7)
+    dec, rules, cur = serving(last=32)
+    cur[0] = dec.prefill_pages(0, prompt, rules)
+    said = [int(cur[0])] + steps(dec, rules, cur, 3, 0)
+    whole = prompt.tolist() + said + turn.tolist()
+    tok = int(dec.prefill_pages(0, torch.tensor(said[-1:] + turn.tolist(), dtype=torch.int32), rules))
+    assert sorted(t for t in rules.history[0].tolist() if t >= 0) == sorted(whole + [tok])
+    assert tok == alone(torch.tensor(whole, dtype=torch.int32), 1, penalties=PRESENCE, last=32)[0]
+
+
+def test_generate_starts_a_history_anew_and_goes_on_with_its_own():
+    prompt = ids(8, 9)
+    dec, rules = model(), LogitRules(1, penalties=PRESENCE, last=32, device="cpu")
+    first = dec.generate(prompt, 5, rules=rules)
+    dec.reset()
+    assert dec.generate(prompt, 5, rules=rules) == first
+    more = ids(3, 10)
+    dec.generate(more, 1, rules=rules)                            # behind prompt and all but the last token
+    held = [t for t in rules.history[0].tolist() if t >= 0]
+    assert len(held) == int(rules.at[0]) == 8 + 4 + 3 + 1
+    assert sorted(held[:-1]) == sorted(prompt.tolist() + first[:4] + more.tolist())
+
+
+def test_a_chunk_that_does_not_fit_leaves_the_history_as_it_was():
+    dec, rules, cur = serving()
+    cur[0] = dec.prefill_pages(0, ids(60, 1), rules)
+    kept = rules.history.clone(), rules.at.clone()
+    with pytest.raises(ValueError):
+        dec.prefill_pages(0, ids(5, 2), rules)
+    assert torch.equal(rules.history, kept[0]) and torch.equal(rules.at, kept[1])
