@@ -147,7 +147,7 @@ class LogitRules:
     """What a server does to n sequences' logits before it takes the largest: penalties (repeat, frequency, presence; one triple,
     or [n, 3]) for the `last` most recent tokens, a bias [vocab] or [n, vocab], and a grammar's mask of int32 words (bit v % 32
     of word v / 32 set: token v may follow), one row or [n, words].  bias and mask may be rewritten in place between steps, of a
-    captured step too.  A sequence that nothing may follow gets token -1.
+    captured step too.  A sequence that nothing may follow gets token -1, which joins no history, and steps leave it out.
 
     history [n, last] holds the token at position p of row's sequence in place p % last (-1: none), at [n] the position behind
     the last one.  `Decoder` keeps both with the sequences: a prompt of a sequence that held nothing starts its row anew, rows that
@@ -189,18 +189,18 @@ class LogitRules:
         return t if t is None or t.dim() == 1 else t[row:row + 1]
 
     def pick(self, ops, logits, row=None, moves=None):
-        """logits [n, vocab] (or row's alone) -> tokens, which join the histories.  moves [n] (0 or 1): the history of a row that
-        does not move stays as it is."""
+        """logits [n, vocab] (or row's alone) -> tokens, which join the histories.  moves [n] (0 or 1): a row that does not move
+        gets token -1."""
         if row is None:
             h, at, pen, bias, mask = self.history, self.at, self.penalties, self.bias, self.mask
         else:
             h, at, pen = self.history[row:row + 1], self.at[row:row + 1], self.penalties[row:row + 1]
             bias, mask = self._row(self.bias, row), self._row(self.mask, row)
         _, tok = ops.logit_rules(logits, history=h, penalties=pen, bias=bias, mask=mask)
-        slot, new, on = (at % self.last)[:, None], tok[:, None], 1
         if moves is not None:
-            on, new = moves, torch.where(moves[:, None] > 0, new, h.gather(1, slot))
-        h.scatter_(1, slot, new)
+            tok = torch.where(moves > 0, tok, -1)
+        on, slot = tok >= 0, (at % self.last)[:, None]
+        h.scatter_(1, slot, torch.where(on[:, None], tok[:, None], h.gather(1, slot)))
         at.add_(on)
         return tok
 
@@ -242,12 +242,22 @@ class _PoolMirror:
     def advance(self, n):
         self.lens = [l + a for l, a in zip(self.lens, n)]
 
+    def settle(self, lens, held):
+        """The device's own account: every sequence's length and number of pages."""
+        for s, h in enumerate(held):
+            self._drop(self.held[s][h:])
+            del self.held[s][h:]
+        self.lens = list(lens)
+
+    def _drop(self, pages):
+        for p in pages:
+            self.refs[p] -= 1
+            if not self.refs[p]:
+                del self.refs[p]
+
     def free(self, seqs):
         for s in seqs:
-            for p in self.held[s]:
-                self.refs[p] -= 1
-                if not self.refs[p]:
-                    del self.refs[p]
+            self._drop(self.held[s])
             self.held[s], self.lens[s] = [], 0
 
     def fork(self, src, dst, n):
@@ -533,6 +543,7 @@ class Decoder:
         self.page_live = torch.zeros(n_seqs, dtype=torch.int32, device=self.dev)       # which sequences a decode step moves
         self._page_out = torch.zeros((n_seqs, self.h_loc * cfg.head_dim), dtype=torch.float32, device=self.dev)     # a step's attention
         self._graph_pages = None
+        self._ahead = False         # whether the host's account may count a token that a step has left out
 
     def _sequences(self, seqs):
         seqs = list(seqs)
@@ -544,13 +555,37 @@ class Decoder:
     def _live(self, s, on):
         self.page_live[s:s + 1].fill_(int(on))
 
+    def _settle(self):
+        """Puts the host's account right where it has run ahead (waits for the device)."""
+        if self._ahead:
+            pg = self.pages
+            self._pool.settle(*torch.stack([pg.lens, (pg.table >= 0).sum(1, dtype=torch.int32)]).tolist())
+            self._ahead = False
+
+    def _account(self, toks):
+        """The host's account of a step: a token more for every sequence that holds something.  Which tokens are negative only the
+        device knows, so the account runs ahead of the sequences that have none, and is put right where a step would not fit."""
+        add = [int(l > 0) for l in self._pool.lens]
+        try:
+            self._pool.grow(add)
+            self._ahead = True
+        except ValueError:
+            self._settle()
+            add = [int(l > 0 and t >= 0) for l, t in zip(self._pool.lens, toks.reshape(-1).tolist())]
+            self._pool.grow(add)
+        return add
+
     def forward_pages_seq(self, s, ids, rules=None):
         """More tokens of sequence s (a prompt, or its next chunk) -> logits of the last one [1, vocab].  rules: whose history
         the tokens join."""
         self._sequences([s])
         n = ids.numel()
         add = [n if i == s else 0 for i in range(len(self._pool.lens))]
-        self._pool.grow(add)
+        try:
+            self._pool.grow(add)
+        except ValueError:
+            self._settle()
+            self._pool.grow(add)
         pg = self._page_seq[s]
         self.ops.pages_grow(pg, n)
         paged = (pg, None)
@@ -571,37 +606,43 @@ class Decoder:
 
     def forward_pages(self, toks):
         """toks [n_seqs] (device int32), every sequence's newest token -> logits [n_seqs, vocab]; the sequences that hold
-        something move on by one, the other rows mean nothing."""
+        something move on by one.  One whose token is negative (nothing may follow it) is left out and stays as it is.  The other
+        rows mean nothing."""
+        return self._step_pages(toks)[0]
+
+    def _step_pages(self, toks):
         n = toks.numel()
         if n != len(self._pool.lens):
             raise ValueError(f"{n} tokens for {len(self._pool.lens)} sequences")
-        add = [int(l > 0) for l in self._pool.lens]
-        self._pool.grow(add)
-        logits = self._forward_pages_device(toks)
+        add = self._account(toks)
+        out = self._forward_pages_device(toks)
         self._pool.advance(add)
-        return logits
+        return out
 
     def _forward_pages_device(self, toks):
-        ops, paged = self.ops, (self.pages, self.page_live)
-        ops.pages_grow(self.pages, self.page_live)
-        n = toks.numel()
-        logits = self._forward_fused(toks, paged=paged, all_rows=True) if self._fuses(n) else self._forward_wide(toks, paged=paged, all_rows=True)
-        ops.pages_advance(self.pages, self.page_live)
-        return logits
+        """-> logits, and which sequences moved (int32)."""
+        ops, toks = self.ops, toks.reshape(-1)
+        moves = self.page_live * (toks >= 0)
+        paged, ids = (self.pages, moves), toks.clamp(min=0)
+        ops.pages_grow(self.pages, moves)
+        logits = self._forward_fused(ids, paged=paged, all_rows=True) if self._fuses(ids.numel()) else self._forward_wide(ids, paged=paged, all_rows=True)
+        ops.pages_advance(self.pages, moves)
+        return logits, moves
 
-    def _pick(self, logits, rules):
+    def _pick(self, logits, moves, rules):
         if rules is not None:
-            return rules.pick(self.ops, logits, moves=self.page_live)
-        return torch.cat([self.ops.argmax(logits[i:i + 64]) for i in range(0, logits.shape[0], 64)])
+            return rules.pick(self.ops, logits, moves=moves)
+        return torch.where(moves > 0, torch.cat([self.ops.argmax(logits[i:i + 64]) for i in range(0, logits.shape[0], 64)]), -1)
 
     def step_pages(self, toks, rules=None):
-        """`forward_pages` and the next tokens [n_seqs]: the largest logits, after the rules if there are any."""
-        return self._pick(self.forward_pages(toks), rules)
+        """`forward_pages` and the next tokens [n_seqs]: the largest logits, after the rules if there are any; -1 for a sequence that
+        nothing may follow, and from then on, as for one that holds nothing."""
+        return self._pick(*self._step_pages(toks), rules)
 
     def capture_pages(self, toks, rules=None):
         """`step_pages` captured in a CUDA graph (reads `toks`; returns the graph and the next tokens).  The graph grows the
         sequences by itself and leaves out those that have been freed since: replay it with `replay_pages`."""
-        pg, saved = self.pages, self._pool.save()
+        pg, saved, ahead = self.pages, self._pool.save(), self._ahead
         kept = [t.clone() for t in (pg.table, pg.lens, pg.refs)] + ([rules.history.clone(), rules.at.clone()] if rules is not None else [])
         state = [pg.table, pg.lens, pg.refs] + ([rules.history, rules.at] if rules is not None else [])
 
@@ -609,6 +650,7 @@ class Decoder:
             for t, k in zip(state, kept):
                 t.copy_(k)
             self._pool.restore(saved)
+            self._ahead = ahead
 
         try:
             for _ in range(2):                  # warm up outside the capture, then put everything back
@@ -618,14 +660,13 @@ class Decoder:
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            out = self._pick(self._forward_pages_device(toks), rules)
-        self._graph_pages = g
+            out = self._pick(*self._forward_pages_device(toks), rules)
+        self._graph_pages, self._graph_toks = g, toks
         return g, out
 
     def replay_pages(self):
         """One more step of the captured graph; the host's account moves with it."""
-        add = [int(l > 0) for l in self._pool.lens]
-        self._pool.grow(add)
+        add = self._account(self._graph_toks)
         self._graph_pages.replay()
         self._pool.advance(add)
 
@@ -633,6 +674,7 @@ class Decoder:
         """Sequence dst[i] (empty) becomes the first n[i] (default: all) tokens of src[i]; whole pages are shared.  Rules follow by
         `LogitRules.copy`, or by `forget` and `see` where not all tokens were taken."""
         src, dst = self._sequences(src), self._sequences(dst)
+        self._settle()
         if len(src) != len(dst) or (n is not None and len(n) != len(src)):
             raise ValueError("lists of one length")
         n = [self._pool.lens[a] if n is None or n[i] is None else n[i] for i, a in enumerate(src)]

@@ -118,3 +118,93 @@ def test_a_chunk_that_does_not_fit_leaves_the_history_as_it_was():
     with pytest.raises(ValueError):
         dec.prefill_pages(0, ids(5, 2), rules)
     assert torch.equal(rules.history, kept[0]) and torch.equal(rules.at, kept[1])
+
+
+def grammar(dec, n_seqs):
+    """Rules under which every token may follow, a row of words for each sequence (clear it: nothing may)."""
+    words = torch.full((n_seqs, dec.cfg.vocab // 32), -1, dtype=torch.int32)
+    return words, LogitRules(n_seqs, penalties=PRESENCE, mask=words, device="cpu")
+
+
+def test_a_sequence_that_nothing_may_follow_stays_as_it_is():
+    dec, _, cur = serving()
+    words, rules = grammar(dec, 2)
+    for s in range(2):
+        cur[s] = dec.prefill_pages(s, ids(8 + s, s), rules)
+    before = steps(dec, rules, cur, 2, 0)
+    words[1] = 0
+    assert steps(dec, rules, cur, 1, 1) == [-1]                  # this step still read the token before
+    kept = dec.pages.lens[1].item(), dec.pages.table[1].clone(), rules.history[1].clone(), rules.at[1].item()
+    assert kept[0] == kept[3] == 9 + 3
+    after, data = steps(dec, rules, cur, 1, 0), dec.pages.data[:, dec.pages.table[1, 0]].clone()
+    after += steps(dec, rules, cur, 6, 0)
+    assert cur[1] == -1 and kept[0] == dec.pages.lens[1] and torch.equal(kept[1], dec.pages.table[1])
+    assert torch.equal(kept[2], rules.history[1]) and kept[3] == rules.at[1] and torch.equal(data, dec.pages.data[:, dec.pages.table[1, 0]])
+    first = alone(ids(8, 0), 11, penalties=PRESENCE)
+    assert first[1:3] == before and first[4:] == after
+    words[1] = -1                                                # the grammar lets it go on, with a token of the caller's
+    cur[1] = 7
+    cur.copy_(dec.step_pages(cur, rules))
+    assert cur[1] >= 0 and dec.pages.lens.tolist() == [8 + 3 + 8, kept[0] + 1]
+
+
+def test_a_prompt_that_nothing_may_follow():
+    dec, _, cur = serving()
+    words, rules = grammar(dec, 2)
+    words[0] = 0
+    cur[0] = dec.prefill_pages(0, ids(8, 1), rules)
+    assert cur[0] == -1 and rules.at[0] == 8
+    cur[1] = dec.prefill_pages(1, ids(6, 2), rules)
+    assert steps(dec, rules, cur, 4, 1) == alone(ids(6, 2), 5, penalties=PRESENCE)[1:] and cur[0] == -1
+    assert dec.pages.lens.tolist() == [8, 10]
+
+
+def test_the_account_follows_sequences_that_have_ended():
+    """Pages that an ended sequence would have taken are there for the others; forks take what it holds."""
+    dec = model()
+    dec.alloc_pages(3, 4, page=16, dtype=torch.float32, max_tokens=48)
+    words, rules = grammar(dec, 3)
+    cur = torch.zeros(3, dtype=torch.int32)
+    words[0] = 0
+    cur[0] = dec.prefill_pages(0, ids(16, 1), rules)              # one page, full
+    cur[1] = dec.prefill_pages(1, ids(30, 2), rules)              # two pages
+    steps(dec, rules, cur, 18, 1)                                 # a third one: the pool is full, and so is sequence 1 with 48 tokens
+    assert dec.pages.lens.tolist() == dec._pool.lens == [16, 48, 0] and len(dec._pool.refs) == 4
+    with pytest.raises(ValueError):
+        dec.step_pages(cur, rules)                                # sequence 1 has a token that does not fit
+    words[1] = 0
+    cur[1] = -1
+    assert dec.step_pages(cur, rules).tolist() == [-1, -1, -1]    # ... and without one the step leaves all of them out
+    dec.fork_pages([0], [2])
+    assert dec.pages.lens.tolist() == dec._pool.lens == [16, 48, 16]
+    dec.free_pages([1, 0])
+    assert dec._pool.lens == [0, 0, 16] and len(dec._pool.refs) == 1 and dec.pages.refs.sum() == 1
+
+
+def test_a_fork_of_an_ended_sequence_takes_what_it_holds():
+    dec, _, cur = serving(3)
+    words, rules = grammar(dec, 3)
+    words[0] = 0
+    cur[0] = dec.prefill_pages(0, ids(15, 1), rules)
+    cur[1] = dec.prefill_pages(1, ids(15, 2), rules)
+    steps(dec, rules, cur, 5, 1)
+    with pytest.raises(ValueError, match="holds 15"):
+        dec.fork_pages([0], [2], [16])
+    dec.fork_pages([0], [2])
+    assert dec.pages.lens.tolist() == dec._pool.lens == [15, 20, 15]
+    assert len(dec._pool.refs) == int((dec.pages.refs > 0).sum()) == 4
+    dec.forward_pages_seq(0, ids(3, 4), rules)                    # it goes on with tokens of the caller's
+    assert dec.pages.lens.tolist() == dec._pool.lens and rules.at[0] == 18
+
+
+def test_negative_tokens_without_rules():
+    dec = model()
+    dec.alloc_pages(2, 6, page=16, dtype=torch.float32)
+    cur = torch.cat([dec.prefill_pages(s, ids(5 + s, s)) for s in range(2)])
+    want = dec.step_pages(cur.clone())
+    two = model()
+    two.alloc_pages(2, 6, page=16, dtype=torch.float32)
+    cur = torch.cat([two.prefill_pages(s, ids(5 + s, s)) for s in range(2)])
+    cur[0] = -1
+    got = two.step_pages(cur)
+    assert got.tolist() == [-1, int(want[1])] and two.pages.lens.tolist() == [5, 7]

@@ -81,3 +81,53 @@ def test_chunks_and_generate_keep_the_whole_history():
     want = dec.generate(p, 6, rules=rules)
     dec.reset()
     assert dec.generate(p, 6, rules=rules) == want and device.device_error() == 0
+
+
+@pytest.mark.parametrize("n_seqs", [3, 10])
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_sequence_that_nothing_may_follow_is_left_out(n_seqs, captured):
+    """The grammar of sequence 1 closes, the others go on as if alone; a fork takes what it holds; it opens again."""
+    from frink_b200 import device
+    words = torch.full((n_seqs, model()[0].vocab // 32), -1, dtype=torch.int32, device="cuda")
+    one = Server(n_seqs, captured, penalties=PRESENCE, mask=words)
+    dec, rules = one.dec, one.rules
+    first, second = ids(one.cfg, 9, 9), ids(one.cfg, 15, 15)
+    got = [one.prompt(0, first)]
+    one.prompt(1, second)
+    got += one.steps(3, 0)
+    words[1] = 0
+    got += one.steps(1, 0)
+    assert one.cur[1] == -1
+    kept = dec.pages.lens[1].item(), dec.pages.table[1].clone(), rules.history[1].clone(), rules.at[1].item()
+    assert kept[0] == kept[3] == 15 + 4
+    data = dec.pages.data[:, dec.pages.table[1, 1]].clone()
+    got += one.steps(20, 0)
+    assert one.cur[1] == -1 and dec.pages.lens[:2].tolist() == [9 + 24, kept[0]] and rules.at[1] == kept[3]
+    assert torch.equal(kept[1], dec.pages.table[1]) and torch.equal(kept[2], rules.history[1]) and torch.equal(data, dec.pages.data[:, dec.pages.table[1, 1]])
+    dec.fork_pages([1], [2])
+    assert dec._pool.lens[:3] == dec.pages.lens[:3].tolist() == [33, 19, 19] and len(dec._pool.refs) == int((dec.pages.refs > 0).sum())
+    words[1] = -1
+    one.cur[1] = 7
+    one.steps(2, 1)
+    assert one.cur[1] >= 0 and dec.pages.lens[:3].tolist() == [35, 21, 19]
+    solo = Server(n_seqs, False, penalties=PRESENCE)
+    assert got == [solo.prompt(0, first)] + solo.steps(24, 0) and device.device_error() == 0
+
+
+def test_a_full_sequence_that_has_ended_does_not_stop_the_others():
+    from frink_b200 import device
+    cfg, dec = model()
+    dec.alloc_pages(2, 5, page=16, max_tokens=48)
+    words = torch.full((2, cfg.vocab // 32), -1, dtype=torch.int32, device="cuda")
+    rules, cur = LogitRules(2, mask=words), torch.zeros(2, dtype=torch.int32, device="cuda")
+    cur[1:] = dec.prefill_pages(1, ids(cfg, 48, 1), rules)        # its table row is full
+    cur[:1] = dec.prefill_pages(0, ids(cfg, 20, 2), rules)
+    g, out = dec.capture_pages(torch.full_like(cur, -1), rules)   # leaves all of them out
+    dec.replay_pages()
+    assert out.tolist() == [-1, -1] and dec.pages.lens.tolist() == [20, 48]
+    with pytest.raises(ValueError):
+        dec.step_pages(cur, rules)                                # a token that does not fit
+    cur[1] = -1
+    for _ in range(12):
+        cur.copy_(dec.step_pages(cur, rules))
+    assert dec.pages.lens.tolist() == dec._pool.lens == [32, 48] and cur[1] == -1 and device.device_error() == 0
