@@ -610,10 +610,12 @@ class Decoder:
         rows mean nothing."""
         return self._step_pages(toks)[0]
 
+    def _one_each(self, toks):
+        if toks.numel() != len(self._pool.lens):
+            raise ValueError(f"{toks.numel()} tokens for {len(self._pool.lens)} sequences")
+
     def _step_pages(self, toks):
-        n = toks.numel()
-        if n != len(self._pool.lens):
-            raise ValueError(f"{n} tokens for {len(self._pool.lens)} sequences")
+        self._one_each(toks)
         add = self._account(toks)
         out = self._forward_pages_device(toks)
         self._pool.advance(add)
@@ -640,23 +642,12 @@ class Decoder:
         return self._pick(*self._step_pages(toks), rules)
 
     def capture_pages(self, toks, rules=None):
-        """`step_pages` captured in a CUDA graph (reads `toks`; returns the graph and the next tokens).  The graph grows the
-        sequences by itself and leaves out those that have been freed since: replay it with `replay_pages`."""
-        pg, saved, ahead = self.pages, self._pool.save(), self._ahead
-        kept = [t.clone() for t in (pg.table, pg.lens, pg.refs)] + ([rules.history.clone(), rules.at.clone()] if rules is not None else [])
-        state = [pg.table, pg.lens, pg.refs] + ([rules.history, rules.at] if rules is not None else [])
-
-        def back():
-            for t, k in zip(state, kept):
-                t.copy_(k)
-            self._pool.restore(saved)
-            self._ahead = ahead
-
-        try:
-            for _ in range(2):                  # warm up outside the capture, then put everything back
-                self.step_pages(toks, rules)
-        finally:
-            back()
+        """`step_pages` captured in a CUDA graph (reads `toks`; returns the graph and the next tokens).  Capturing moves no
+        sequence and needs no room.  The graph grows the sequences by itself and leaves out those that have been freed since:
+        replay it with `replay_pages`."""
+        self._one_each(toks)
+        for _ in range(2):                      # warm up outside the capture, with no sequence moving
+            self._pick(*self._forward_pages_device(torch.full_like(toks, -1)), rules)
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):

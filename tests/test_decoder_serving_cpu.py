@@ -208,3 +208,46 @@ def test_negative_tokens_without_rules():
     cur[0] = -1
     got = two.step_pages(cur)
     assert got.tolist() == [-1, int(want[1])] and two.pages.lens.tolist() == [5, 7]
+
+
+class _NoGraph:
+    """Stands in for a CUDA graph and its capture."""
+    inside = False
+
+    def __init__(self, *a):
+        pass
+
+    def __enter__(self):
+        _NoGraph.inside = True
+
+    def __exit__(self, *a):
+        _NoGraph.inside = False
+
+
+@pytest.mark.parametrize("n", [31, 32])
+@pytest.mark.parametrize("n_pages,max_tokens", [(4, 64), (8, 32)])
+def test_a_step_is_captured_where_little_or_nothing_fits(monkeypatch, n, n_pages, max_tokens):
+    """The pool, or the sequences' table rows, have room for one more token each, or for none (a replay is then refused)."""
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", _NoGraph)
+    monkeypatch.setattr(torch.cuda, "graph", _NoGraph)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: None)
+    dec, rules = model(), LogitRules(2, penalties=PRESENCE, device="cpu")
+    dec.alloc_pages(2, n_pages, page=16, dtype=torch.float32, max_tokens=max_tokens)
+    cur = torch.cat([dec.prefill_pages(s, ids(n, s), rules) for s in range(2)])
+    state = lambda: [t.clone() for t in (dec.pages.table, dec.pages.lens, dec.pages.refs, dec.pages.data, rules.history, rules.at)]
+    before, seen, run = state(), [], dec._forward_pages_device
+
+    def forward(toks):
+        seen.append((toks.tolist(), state()))
+        return run(torch.full_like(toks, -1) if _NoGraph.inside else toks)      # a capture runs nothing
+
+    monkeypatch.setattr(dec, "_forward_pages_device", forward)
+    dec.capture_pages(cur, rules)
+    assert seen[-1][0] == cur.tolist() and dec._pool.lens == dec.pages.lens.tolist() == [n, n]
+    for st in [s for _, s in seen] + [state()]:
+        assert all(torch.equal(a, b) for a, b in zip(before, st))
+    with pytest.raises(ValueError):
+        dec.capture_pages(cur[:1], rules)
+    if n == 32:
+        with pytest.raises(ValueError):
+            dec.replay_pages()

@@ -131,3 +131,25 @@ def test_a_full_sequence_that_has_ended_does_not_stop_the_others():
     for _ in range(12):
         cur.copy_(dec.step_pages(cur, rules))
     assert dec.pages.lens.tolist() == dec._pool.lens == [32, 48] and cur[1] == -1 and device.device_error() == 0
+
+
+@pytest.mark.parametrize("n", [31, 32])
+def test_a_step_is_captured_where_little_or_nothing_fits(n):
+    """Room for one more token of each sequence, or for none: the capture moves nothing, a replay is refused where it does not fit."""
+    from frink_b200 import device
+    cfg, dec = model()
+    dec.alloc_pages(2, 4, page=16)
+    rules = LogitRules(2, penalties=PRESENCE)
+    cur = torch.cat([dec.prefill_pages(s, ids(cfg, n, s), rules) for s in range(2)])
+    state = lambda: [t.clone() for t in (dec.pages.table, dec.pages.lens, dec.pages.refs, dec.pages.data, rules.history, rules.at)]
+    before = state()
+    g, out = dec.capture_pages(cur, rules)
+    assert all(torch.equal(a, b) for a, b in zip(before, state())) and dec._pool.lens == [n, n]
+    for _ in range(32 - n):
+        dec.replay_pages()
+        assert dec.pages.lens.tolist() == dec._pool.lens == [32, 32] and min(out.tolist()) >= 0
+    with pytest.raises(ValueError):
+        dec.replay_pages()
+    dec.free_pages([0])
+    dec.replay_pages()
+    assert dec.pages.lens.tolist() == dec._pool.lens == [0, 33] and device.device_error() == 0
