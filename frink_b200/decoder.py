@@ -542,7 +542,7 @@ class Decoder:
         self._pool = _PoolMirror(n_seqs, n_pages, page, max_pages)
         self.page_live = torch.zeros(n_seqs, dtype=torch.int32, device=self.dev)       # which sequences a decode step moves
         self._page_out = torch.zeros((n_seqs, self.h_loc * cfg.head_dim), dtype=torch.float32, device=self.dev)     # a step's attention
-        self._graph_pages = None
+        self._graph_pages = self._graph_uses = None
         self._ahead = False         # whether the host's account may count a token that a step has left out
 
     def _sequences(self, seqs):
@@ -652,12 +652,14 @@ class Decoder:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             out = self._pick(*self._forward_pages_device(toks), rules)
-        self._graph_pages, self._graph_toks = g, toks
+        self._graph_pages = g
+        # the graph knows addresses only: what it reads and writes stays, whatever the caller's names come to mean
+        self._graph_uses = [toks] + ([] if rules is None else [rules.history, rules.at, rules.penalties, rules.bias, rules.mask])
         return g, out
 
     def replay_pages(self):
         """One more step of the captured graph; the host's account moves with it."""
-        add = self._account(self._graph_toks)
+        add = self._account(self._graph_uses[0])
         self._graph_pages.replay()
         self._pool.advance(add)
 

@@ -1,4 +1,7 @@
 """`Decoder` over pages as a server drives it, on the CPU stand-ins: slots that are idle, freed and filled again, under rules."""
+import gc
+import weakref
+
 import numpy as np
 import pytest
 import torch
@@ -251,3 +254,22 @@ def test_a_step_is_captured_where_little_or_nothing_fits(monkeypatch, n, n_pages
     if n == 32:
         with pytest.raises(ValueError):
             dec.replay_pages()
+
+
+def test_a_captured_step_keeps_what_it_reads_and_writes(monkeypatch):
+    """The graph holds addresses: the tokens and the rules' tensors live as long as it, whatever becomes of the caller's names."""
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", _NoGraph)
+    monkeypatch.setattr(torch.cuda, "graph", _NoGraph)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: None)
+    dec, rules, cur = serving()
+    words, rules = grammar(dec, 2)
+    rules.bias = torch.zeros(dec.cfg.vocab)
+    dec.capture_pages(cur, rules)
+    held = [weakref.ref(t) for t in (cur, words, rules.bias, rules.history, rules.at, rules.penalties)]
+    rules.bias = rules.mask = None
+    del cur, words, rules
+    gc.collect()
+    assert all(r() is not None for r in held)
+    dec.alloc_pages(2, 8)                                         # the graph is gone, and so are they
+    gc.collect()
+    assert all(r() is None for r in held)
