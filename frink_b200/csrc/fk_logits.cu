@@ -174,6 +174,7 @@ FK_EXPORT int fk_logit_rules(fk_ctx* ctx, void* stream, const float* logits_dev,
     if (history_dev && !penalties_dev) return fk_fail(FK_INVALID, "logit_rules: a history without penalties");
     if (bias_dev && bias_ld != 0 && bias_ld < (size_t)vocab) return fk_fail(FK_INVALID, "logit_rules: bias rows %zu apart", bias_ld);
     if (mask_dev && mask_ld != 0 && mask_ld < (size_t)(vocab + 31) / 32) return fk_fail(FK_INVALID, "logit_rules: mask rows of %zu words", mask_ld);
+    if (n_rows == 1) ld = vocab;                             // no next row: how far it would be says nothing
     if (out_dev == logits_dev && ld != (size_t)vocab) return fk_fail(FK_INVALID, "logit_rules: logits are changed in place only where their rows are packed");
     if (history > LR_HISTORY) return fk_fail(FK_UNSUPPORTED, "logit_rules: a history of %d (at most %d)", history, LR_HISTORY);
     FkDeviceGuard g(ctx->device);

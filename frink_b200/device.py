@@ -783,7 +783,7 @@ def logit_rules(logits, history=None, penalties=None, bias=None, mask=None, out=
     elif tokens.shape != (n,) or tokens.dtype is not _I32 or tokens.get_device() != dev or not tokens.is_contiguous():
         raise _lib.Invalid("logit_rules: tokens is a contiguous int32 tensor [n]")
     ctx = _contexts.get(dev) or context(x.device)
-    check(lib().fk_logit_rules(ctx, _raw_stream(dev), x.data_ptr(), ld if n > 1 else max(ld, V), n, V, hp, h,
+    check(lib().fk_logit_rules(ctx, _raw_stream(dev), x.data_ptr(), ld if n > 1 else V, n, V, hp, h,
                                pen.data_ptr() if pen is not None else None, bp, b_ld, mp, m_ld, o.data_ptr(), tokens.data_ptr()))
     return (o if logits.dim() == 2 else o[0]), tokens
 

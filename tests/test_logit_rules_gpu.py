@@ -132,3 +132,18 @@ def test_zeros_of_both_signs_are_ties():
     out, tok = device.logit_rules(x.cuda())
     assert tok.tolist() == [3, 3, 4, 100]
     assert torch.equal(torch.signbit(out.cpu()), torch.signbit(x))
+
+
+def test_one_row_of_a_wide_tensor_is_changed_in_place():
+    """A single row is packed, whatever its tensor says about the distance to a next one."""
+    from frink_b200 import device
+    wide = torch.randn((4, 900), generator=torch.Generator().manual_seed(11)).cuda()
+    hist, pen = torch.tensor([[5, 5, 9]], dtype=torch.int32).cuda(), torch.tensor([[1.2, 0.25, 0.5]]).cuda()
+    for at in (100, 101):                                         # on and off a 16-byte boundary
+        was = wide.clone()
+        row = wide[1:2, at:at + 700]
+        want, tok = device.logit_rules(row.clone(), history=hist, penalties=pen)
+        got, tok2 = device.logit_rules(row, history=hist, penalties=pen, out=row)
+        assert got.data_ptr() == row.data_ptr() and torch.equal(row, want) and torch.equal(tok, tok2)
+        was[1, at:at + 700] = want[0]
+        assert torch.equal(wide, was)
