@@ -185,6 +185,14 @@ class LogitRules:
         self.history[dst] = self.history[src]
         self.at[dst] = self.at[src]
 
+    def fits(self, vocab, n=None, row=None):
+        """Refuses rules that are not for logits of this vocabulary and these n sequences (or this row's)."""
+        if row is not None and row >= self.n or n is not None and n != self.n:
+            raise ValueError(f"rules of {self.n} sequences for " + (f"sequence {row}" if n is None else f"{n}"))
+        for name, t, dtype, width in (("bias", self.bias, torch.float32, vocab), ("mask", self.mask, torch.int32, (vocab + 31) // 32)):
+            if t is not None and (t.dtype != dtype or t.dim() not in (1, 2) or t.shape[-1] < width or (t.dim() == 2 and t.shape[0] != self.n)):
+                raise ValueError(f"{name}: {dtype} rows of at least {width}, one or {self.n}, not {t.dtype} {tuple(t.shape)}")
+
     def _row(self, t, row):
         return t if t is None or t.dim() == 1 else t[row:row + 1]
 
@@ -579,6 +587,8 @@ class Decoder:
         """More tokens of sequence s (a prompt, or its next chunk) -> logits of the last one [1, vocab].  rules: whose history
         the tokens join."""
         self._sequences([s])
+        if rules is not None:
+            rules.fits(self.cfg.vocab, row=s)
         n = ids.numel()
         add = [n if i == s else 0 for i in range(len(self._pool.lens))]
         try:
@@ -639,6 +649,8 @@ class Decoder:
     def step_pages(self, toks, rules=None):
         """`forward_pages` and the next tokens [n_seqs]: the largest logits, after the rules if there are any; -1 for a sequence that
         nothing may follow, and from then on, as for one that holds nothing."""
+        if rules is not None:
+            rules.fits(self.cfg.vocab, toks.numel())
         return self._pick(*self._step_pages(toks), rules)
 
     def capture_pages(self, toks, rules=None):
@@ -646,6 +658,8 @@ class Decoder:
         sequence and needs no room.  The graph grows the sequences by itself and leaves out those that have been freed since:
         replay it with `replay_pages`."""
         self._one_each(toks)
+        if rules is not None:
+            rules.fits(self.cfg.vocab, toks.numel())
         for _ in range(2):                      # warm up outside the capture, with no sequence moving
             self._pick(*self._forward_pages_device(torch.full_like(toks, -1)), rules)
         torch.cuda.synchronize()
@@ -659,6 +673,8 @@ class Decoder:
 
     def replay_pages(self):
         """One more step of the captured graph; the host's account moves with it."""
+        if self._graph_pages is None:
+            raise ValueError("no step was captured for these pages (capture_pages)")
         add = self._account(self._graph_uses[0])
         self._graph_pages.replay()
         self._pool.advance(add)
@@ -837,6 +853,7 @@ class Decoder:
         if rules is not None:
             if use_graph:
                 raise ValueError("rules run eagerly here; a captured step with rules is capture_pages'")
+            rules.fits(self.cfg.vocab, 1)
             at = self._pos_host
             logits = self.forward(prompt_ids)
             if at == 0:

@@ -273,3 +273,29 @@ def test_a_captured_step_keeps_what_it_reads_and_writes(monkeypatch):
     dec.alloc_pages(2, 8)                                         # the graph is gone, and so are they
     gc.collect()
     assert all(r() is None for r in held)
+
+
+def test_rules_that_do_not_fit_are_refused_before_a_step():
+    dec, rules, cur = serving()
+    cur[0] = dec.prefill_pages(0, ids(8, 1), rules)
+    mask = lambda *shape: torch.full(shape, -1, dtype=torch.int32)
+    wrong = [dict(mask=mask(15)), dict(mask=mask(3, 16)), dict(mask=torch.ones(512, dtype=torch.bool)), dict(bias=torch.zeros(511)), dict(bias=torch.zeros(3, 512)),
+             dict(bias=torch.zeros(512, dtype=torch.float64))]
+    two, one = [LogitRules(2, device="cpu", **kw) for kw in wrong], [LogitRules(1, device="cpu", **kw) for kw in wrong]
+    state = lambda: [t.clone() for t in (dec.pages.table, dec.pages.lens, dec.pages.refs, dec.page_live)]
+    before, pool = state(), dec._pool.save()
+    for r in two + [LogitRules(3, device="cpu"), LogitRules(1, device="cpu")]:
+        for call in (dec.step_pages, dec.capture_pages):
+            with pytest.raises(ValueError):
+                call(cur, r)
+    for r in two + [LogitRules(1, device="cpu")]:
+        with pytest.raises(ValueError):
+            dec.prefill_pages(1, ids(4, 2), r)
+    for r in one + [LogitRules(2, device="cpu")]:
+        with pytest.raises(ValueError):
+            dec.generate(ids(4, 2), 2, rules=r)
+    assert all(torch.equal(a, b) for a, b in zip(before, state())) and dec._pool.save() == pool and dec._pos_host == 0
+    assert all(int(r.at.sum()) == 0 for r in one + two)
+    with pytest.raises(ValueError, match="captured"):
+        dec.replay_pages()
+    LogitRules(2, bias=torch.zeros(2, 600), mask=mask(20), device="cpu").fits(512, 2)      # longer rows are fine
