@@ -28,8 +28,8 @@ def context(device=None):
         return _contexts[idx]
 
 
-def _stream(device=None):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _stream():
+    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
 def _ptr(t):
