@@ -149,14 +149,14 @@ class LogitRules:
     of word v / 32 set: token v may follow), one row or [n, words].  bias and mask may be rewritten in place between steps, of a
     captured step too.  A sequence that nothing may follow gets token -1, which joins no history, and steps leave it out.
 
-    history [n, last] holds the token at position p of row's sequence in place p % last (-1: none), at [n] the position behind
-    the last one.  `Decoder` keeps both with the sequences: a prompt of a sequence that held nothing starts its row anew, rows that
-    a step leaves out stay as they are.  A fork's row is the caller's: `copy` where all tokens were taken over, else `forget`
-    and `see`."""
+    history [n, last] holds the tokens that were seen and picked, the one at position p of row's sequence in place p % last (-1:
+    none); at [n] is the position behind the last one.  `Decoder` keeps both with the sequences: the prompt of a sequence that
+    held nothing starts its row anew, rows that a step leaves out stay as they are.  A fork's row is the caller's: `copy` where all
+    tokens were taken over, else `forget` and `see`."""
 
     def __init__(self, n, penalties=(1.0, 0.0, 0.0), last=64, bias=None, mask=None, device="cuda"):
-        if last < 1:
-            raise ValueError("the history holds at least one token")
+        if not 1 <= last <= 65535:
+            raise ValueError(f"a history of {last} tokens (1 to 65535)")
         pen = torch.as_tensor(penalties, dtype=torch.float32)
         if pen.shape not in ((3,), (n, 3)):
             raise ValueError(f"penalties are (repeat, frequency, presence) or [{n}, 3]")

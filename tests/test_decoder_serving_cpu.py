@@ -299,3 +299,6 @@ def test_rules_that_do_not_fit_are_refused_before_a_step():
     with pytest.raises(ValueError, match="captured"):
         dec.replay_pages()
     LogitRules(2, bias=torch.zeros(2, 600), mask=mask(20), device="cpu").fits(512, 2)      # longer rows are fine
+    for last in (0, 65536):                                       # what the rules' kernel counts in
+        with pytest.raises(ValueError, match="65535"):
+            LogitRules(2, last=last, device="cpu")
