@@ -27,14 +27,16 @@
 // units, one after another, are dealt out in equal runs to the CTAs of one grid, so that ragged lengths keep every SM busy and
 // the grid does not depend on lengths that only the device knows.  An item's way in (pages' numbers, q) and out (sums of the
 // warps) takes about a unit's time and is dealt out like one: 500 sequences of 1 to 600 tokens, 8 KV heads, 155 us without, 125
-// with.  A run's first and last item may be shared with other CTAs: their partial sums go to a record of the CTA; the CTA that
+// with (one row's own kernel: 113).  A run's first and last item may be shared with other CTAs: their partial sums go to a record of the CTA; the CTA that
 // arrives last joins up to eight of them in one trip to memory, more in groups of about the square root of their number (131071
 // tokens, 55 records an item: one CTA for all 57.2 us, groups 51.3).
 //
 // Bound by HBM where sequences are long, by its way in and out (some 10 us: launch, entries, page numbers, first copies, join)
 // where they are short.  B200: 64 sequences of 250 to 16000 tokens, window 4096, 32/4 heads of 128 in bf16, 84 us = 5.7 TB/s;
-// 131071 tokens, 64/8 heads of 64 in f16, 51.3 us = 5.2 TB/s; 8 x 4000 as above 29.7 us = 4.4 TB/s; 8 x 64000 6.4 TB/s; 17
-// tokens in f32 6.5 us.  (A plain copy moves 6.55 TB/s.)
+// 131071 tokens, 64/8 heads of 64 in f16, 50.7 us = 5.3 TB/s, in f32 91 us = 5.9 TB/s; 8 x 4000 as above 28.6 us = 4.6 TB/s, in
+// f32 51.4 us = 5.1 TB/s; 8 x 64000 6.4 TB/s; 17 tokens in f32 5.7 us.  (A plain copy moves 6.55 TB/s.)  Registers: three CTAs an
+// SM leave 168 a thread (two, with 16 columns: 255), where one row's variants spill 44 bytes for heads of 128 in f16 and f32, 56
+// with 16 columns in bf16, the others (almost) none; several rows' up to 76.
 #include "fk_paged.cuh"
 
 #include <type_traits>
@@ -46,8 +48,8 @@ namespace {
 constexpr int WARPS = 4;
 // (sequence, block of columns) pairs that are dealt out in runs; where there are more, each (pair, KV head) has a CTA.  The deal
 // costs a scan of the pairs by every CTA and keeps one long sequence from outlasting the others; 512 pairs dealt / 513 with CTAs
-// of their own, us: 100 tokens and 8 KV heads 75 / 63, 1000 and 8 329 / 305, 1000 and 1 56 / 60, 4000 and 1 172 / 204; 500
-// sequences of very different lengths (mean 8000) and 2 KV heads 639 / 1005.
+// of their own, us: 100 tokens and 8 KV heads 66 / 57, 1000 and 8 330 / 306, 1000 and 1 52 / 60, 4000 and 1 175 / 206; 500
+// sequences of very different lengths (mean 8000) and 2 KV heads 631 / 1078.
 constexpr int MAX_ENTRIES = 512;
 constexpr int MAX_CTAS = 640;              // of a grid that shares items: three counters each
 static_assert(3 * MAX_CTAS * sizeof(unsigned) <= WS_COUNTERS, "");
@@ -876,7 +878,8 @@ template <int KIND, int HDP, bool EXACT, int NT, bool ONE> int launch_attn(fk_ct
 
 template <int KIND, bool ONE> int launch_kind(fk_ctx* ctx, cudaStream_t st, const AttnArgs& a) {
     // 16 columns a CTA read the keys once for twice the columns, with registers for two CTAs an SM instead of three.  Us with 16 /
-    // with 8: 16 columns 64 x 4000 tokens 117 / 170, 8 x 16000 69 / 91, 1 x 64000 51 / 49; 12 columns 64 x 4000 45 / 40.
+    // with 8: 16 columns, 4 KV heads, 64 x 4000 tokens 114 / 171, 8 x 16000 67 / 87, 1 x 64000 49 / 42; 12 columns, 3 KV heads,
+    // 64 x 4000 90 / 130.
     const bool wide = (long long)a.rows * a.group > 8;
     if (a.head_dim == 64) return wide ? launch_attn<KIND, 64, true, 2, ONE>(ctx, st, a) : launch_attn<KIND, 64, true, 1, ONE>(ctx, st, a);
     if (a.head_dim == 128) return wide ? launch_attn<KIND, 128, true, 2, ONE>(ctx, st, a) : launch_attn<KIND, 128, true, 1, ONE>(ctx, st, a);

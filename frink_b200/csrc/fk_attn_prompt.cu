@@ -25,9 +25,9 @@
 // values of tiles that not every row sees: a value that no row sees is zeroed in shared memory (stale memory may hold NaN); one
 // that some rows see and that is not finite is zeroed too and added in plain f32 for the rows that see it.
 //
-// Measured (B200): 512 rows of 24/8 heads of 128, bf16, empty cache 23.2 us; 4200 rows 316 us = 343 TFLOP/s of the formula's
-// operations, three times that of MMA, f16 276 us; 1001, 801, 601 and 401 rows after 2000 to 8000 tokens, window 2048, 64/8
-// heads of 64, f16, 386 us.  What bounds it is a tile's chain from scores to weights (tensor pipe 25 %, issue slots 53 %): with
+// Measured (B200): 512 rows of 24/8 heads of 128, bf16, empty cache 23.5 us; 4200 rows 309 us = 351 TFLOP/s of the formula's
+// operations, three times that of MMA, f16 267 us; 1001, 801, 601 and 401 rows after 2000 to 8000 tokens, window 2048, 64/8
+// heads of 64, f16, 385 us.  What bounds it is a tile's chain from scores to weights (tensor pipe 25 %, issue slots 49 %): with
 // one part of each product instead of two or three the last case gains 3 % and the bf16 one 6 %, without the exponentials and
 // the parts' arithmetic 20 and 9 %.  An item alone is bound by its way in and out.
 #include "fk_paged.cuh"
@@ -657,9 +657,10 @@ bool fk_attn_prompt_takes(fk_ctx* ctx, const fk_pages* p, int rows, int n_heads)
     if ((long long)p->n_pages * 2 * p->n_kv * p->page > 0x7fffffffLL) return false;      // a token's row number is 32 bits
     // This kernel takes 19 ns an SM for a key of a tile of 128 columns, whatever of the tile is filled, and does not split the
     // keys; the other takes 13 ns an SM for a key of 16 columns and spreads over all SMs (bf16, heads of 128; f16 heads of 64: 15
-    // and 7).  24/8 heads of 128, one sequence after 8000 tokens, us here / there: 64 rows 161 / 86, 128 rows 164 / 154, 256
-    // rows 167 / 302; four sequences: 24 rows 161 / 138, 43 rows 164 / 248.  64/8 heads of 64, f16, 64 rows 124 / 112, 128 rows
-    // 127 / 214.
+    // and 7).  24/8 heads of 128, one sequence after 8000 tokens, us here / there: 64 rows 167 / 84, 128 rows 170 / 152, 256
+    // rows 172 / 293; four sequences: 24 rows 167 / 133, 43 rows 169 / 224.  64/8 heads of 64, f16, 64 rows 119 / 107, 128 rows
+    // 121 / 206.  f32 pages stay there, as 128 columns of three-part products have no kernel here: 512 rows of 24/8 heads of 128
+    // into an empty cache 69 us, four of 900 rows after 8000 tokens 7.5 ms (bf16 here: 1.05).
     const long long tiles = (long long)p->n_seqs * p->n_kv * ((rows + 128 / group - 1) / (128 / group));
     const long long blocks = (long long)p->n_seqs * p->n_kv * (((long long)rows * group + 15) / 16);
     return 3 * blocks > 5 * ctx->sm_count * ((tiles + ctx->sm_count - 1) / ctx->sm_count);

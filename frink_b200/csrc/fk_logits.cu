@@ -7,7 +7,8 @@
 // before a step is worked on.  Every logit is read, changed and written once, and the largest is kept as an order-preserving key
 // that the block which arrives last for the row joins.
 // 64 x 201088 with bias, mask and a history of 1000, B200: blocks of 4096 logits that each read the history 52.8 us, with the
-// loads ahead of it 36.5 us; this form 27.5 us = 3.8 TB/s, what is left is the latency of 40 KB in flight an SM (registers).
+// loads ahead of it 36.5 us; this form 26.6 us = 4.0 TB/s, what is left is the latency of 40 KB in flight an SM: loads go to
+// registers, since the counts (16 bits a token, 45 KB a block) hold the shared memory that a ring of copies would need.
 #include "fk_paged.cuh"
 
 namespace {
