@@ -745,7 +745,8 @@ def logit_rules(logits, history=None, penalties=None, bias=None, mask=None, out=
     that occurs c > 0 times has its logit divided (if positive, else multiplied) by repeat, less c * frequency, less presence
     (penalties: float32 [n, 3], or one triple for all rows: numbers of the host, so not while a graph is captured).  bias [vocab]
     or [n, vocab] is added, then logits whose bit in mask (int32 words [words] or [n, words], bit v % 32 of word v / 32) is clear
-    become -inf.  tokens: the largest, ties to the lower index; -1 where nothing is left."""
+    become -inf.  tokens: the largest, ties to the lower index; -1 where nothing is left.  One call of this or of `argmax` at a time
+    on a device: they share its context's workspace, captured steps too."""
     x = logits if logits.dim() == 2 else logits[None]
     dev = x.get_device()
     if dev < 0 or x.dtype is not _F32 or x.dim() != 2:
