@@ -662,6 +662,15 @@ extern "C" {
         n_new_dev: *const c_int,
         n_new: c_int,
     ) -> c_int;
+    pub fn fk_pages_moves(
+        ctx: *mut FkCtx,
+        stream: *mut c_void,
+        tokens_dev: *const c_int,
+        live_dev: *const c_int,
+        n: c_int,
+        ids_dev: *mut c_int,
+        moves_dev: *mut c_int,
+    ) -> c_int;
     pub fn fk_pages_fork(
         ctx: *mut FkCtx,
         stream: *mut c_void,
@@ -737,6 +746,16 @@ extern "C" {
         mask_ld: usize,
         out_dev: *mut f32,
         tokens_dev: *mut c_int,
+    ) -> c_int;
+    pub fn fk_tokens_join(
+        ctx: *mut FkCtx,
+        stream: *mut c_void,
+        tokens_dev: *mut c_int,
+        moves_dev: *const c_int,
+        n: c_int,
+        history_dev: *mut c_int,
+        history: c_int,
+        at_dev: *mut i64,
     ) -> c_int;
     pub fn fk_comm_create(
         ctx: *mut FkCtx,

@@ -7,7 +7,7 @@ import os
 import re
 
 ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
-TYPES = {"int": "c_int", "float": "f32", "size_t": "usize", "uint64_t": "u64", "int32_t": "i32", "uint8_t": "u8", "char": "c_char", "void": "c_void",
+TYPES = {"int": "c_int", "float": "f32", "size_t": "usize", "uint64_t": "u64", "int32_t": "i32", "int64_t": "i64", "uint8_t": "u8", "char": "c_char", "void": "c_void",
          "fk_ctx": "FkCtx", "fk_comm": "FkComm", "fk_matvec_launch": "FkMatvecLaunch", "fk_pages": "FkPages"}
 
 HEAD = '''//! Raw declarations of `libfrink_b200.so`'s C ABI, one per entry point of `include/frink_b200.h`, in the

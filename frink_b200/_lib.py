@@ -77,11 +77,13 @@ SYMBOLS = {
     "fk_pages_grow": (_I, [_P, _P, _P, _P, _I]),
     "fk_pages_advance": (_I, [_P, _P, _P, _P, _I]),
     "fk_pages_fork": (_I, [_P, _P, _P, _P, _P, _P, _I]),
+    "fk_pages_moves": (_I, [_P, _P, _P, _P, _I, _P, _P]),
     "fk_pages_free": (_I, [_P, _P, _P, _P, _I]),
     "fk_pages_compact": (_I, [_P, _P, _P, _P]),
     "fk_rope_kv_paged": (_I, [_P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _I, C.c_float, _I, _P, _P, C.c_float, _P]),
     "fk_attention_paged": (_I, [_P, _P, _P, _I, _P, _I, _I, _P, _I, C.c_float, _I, _I, _P, _P]),
     "fk_logit_rules": (_I, [_P, _P, _P, _SZ, _I, _I, _P, _I, _P, _P, _SZ, _P, _SZ, _P, _P]),
+    "fk_tokens_join": (_I, [_P, _P, _P, _P, _I, _P, _I, _P]),
     "fk_comm_create": (_I, [_P, _SZ, _I, _I, _P, C.POINTER(_P)]),
     "fk_comm_connect": (_I, [_P, _P]),
     "fk_comm_connect_local": (_I, [_P, C.POINTER(_P)]),

@@ -163,7 +163,31 @@ template <bool VEC> __global__ void __launch_bounds__(LR_THREADS, LR_PER_SM) rul
     }
 }
 
+// The picked tokens into their histories, a thread a sequence: a launch's latency.
+__global__ void join_kernel(int* __restrict__ tokens, const int* __restrict__ moves, int n, int* __restrict__ history, int n_hist, int64_t* __restrict__ at) {
+    fk_paged::pdl_sync();
+    const int s = blockIdx.x * blockDim.x + threadIdx.x;
+    if (s >= n) return;
+    int t = tokens[s];
+    if (moves && moves[s] == 0) tokens[s] = t = -1;
+    if (!history || t < 0) return;
+    const int64_t a = at[s];
+    history[(size_t)s * n_hist + (size_t)((uint64_t)a % (unsigned)n_hist)] = t;
+    at[s] = a + 1;
+}
+
 }  // namespace
+
+FK_EXPORT int fk_tokens_join(fk_ctx* ctx, void* stream, int* tokens_dev, const int* moves_dev, int n, int* history_dev, int history, int64_t* at_dev) {
+    if (!ctx || !tokens_dev) return fk_fail(FK_INVALID, "tokens_join: null argument");
+    if (n < 1) return fk_fail(FK_INVALID, "tokens_join: %d tokens", n);
+    if (history_dev && (!at_dev || history < 1)) return fk_fail(FK_INVALID, "tokens_join: a history of %d tokens without their number", history);
+    FkDeviceGuard g(ctx->device);
+    FK_CUDA(fk_paged::launch(join_kernel, dim3((n + 255) / 256), dim3(256), 0, (cudaStream_t)stream, tokens_dev, moves_dev, n, history_dev, history, at_dev), FK_LAUNCH);
+    FK_CUDA(cudaGetLastError(), FK_LAUNCH);
+    ctx->launches++;
+    return FK_OK;
+}
 
 FK_EXPORT int fk_logit_rules(fk_ctx* ctx, void* stream, const float* logits_dev, size_t ld, int n_rows, int vocab, const int* history_dev, int history,
                              const float* penalties_dev, const float* bias_dev, size_t bias_ld, const int* mask_dev, size_t mask_ld, float* out_dev,

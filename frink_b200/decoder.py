@@ -143,6 +143,19 @@ class _Merged:
         return outs
 
 
+def _join(ops, tok, moves, history=None, at=None):
+    """A step's tokens: -1 where moves is 0 (None: all move); those that are not negative join their histories."""
+    if hasattr(ops, "tokens_join"):
+        return ops.tokens_join(tok, moves, history, at)
+    if moves is not None:
+        tok = torch.where(moves > 0, tok, -1)
+    if history is not None:
+        on, slot = tok >= 0, (at % history.shape[1])[:, None]
+        history.scatter_(1, slot, torch.where(on[:, None], tok[:, None], history.gather(1, slot)))
+        at.add_(on)
+    return tok
+
+
 class LogitRules:
     """What a server does to n sequences' logits before it takes the largest: penalties (repeat, frequency, presence; one triple,
     or [n, 3]) for the `last` most recent tokens, a bias [vocab] or [n, vocab], and a grammar's mask of int32 words (bit v % 32
@@ -205,12 +218,7 @@ class LogitRules:
             h, at, pen = self.history[row:row + 1], self.at[row:row + 1], self.penalties[row:row + 1]
             bias, mask = self._row(self.bias, row), self._row(self.mask, row)
         _, tok = ops.logit_rules(logits, history=h, penalties=pen, bias=bias, mask=mask)
-        if moves is not None:
-            tok = torch.where(moves > 0, tok, -1)
-        on, slot = tok >= 0, (at % self.last)[:, None]
-        h.scatter_(1, slot, torch.where(on[:, None], tok[:, None], h.gather(1, slot)))
-        at.add_(on)
-        return tok
+        return _join(ops, tok, moves, h, at)
 
 
 class _PoolMirror:
@@ -634,8 +642,11 @@ class Decoder:
     def _forward_pages_device(self, toks):
         """-> logits, and which sequences moved (int32)."""
         ops, toks = self.ops, toks.reshape(-1)
-        moves = self.page_live * (toks >= 0)
-        paged, ids = (self.pages, moves), toks.clamp(min=0)
+        if hasattr(ops, "pages_moves"):
+            ids, moves = ops.pages_moves(toks, self.page_live)
+        else:
+            ids, moves = toks.clamp(min=0), self.page_live * (toks >= 0)
+        paged = (self.pages, moves)
         ops.pages_grow(self.pages, moves)
         logits = self._forward_fused(ids, paged=paged, all_rows=True) if self._fuses(ids.numel()) else self._forward_wide(ids, paged=paged, all_rows=True)
         ops.pages_advance(self.pages, moves)
@@ -644,7 +655,8 @@ class Decoder:
     def _pick(self, logits, moves, rules):
         if rules is not None:
             return rules.pick(self.ops, logits, moves=moves)
-        return torch.where(moves > 0, torch.cat([self.ops.argmax(logits[i:i + 64]) for i in range(0, logits.shape[0], 64)]), -1)
+        n, ops = logits.shape[0], self.ops
+        return _join(ops, ops.argmax(logits) if n <= 64 else torch.cat([ops.argmax(logits[i:i + 64]) for i in range(0, n, 64)]), moves)
 
     def step_pages(self, toks, rules=None):
         """`forward_pages` and the next tokens [n_seqs]: the largest logits, after the rules if there are any; -1 for a sequence that

@@ -631,6 +631,26 @@ def _counts(pg, n_new):
     return None if n_new is None else _n_new(pg, n_new)[0]
 
 
+def _ints(dev, what, **ts):
+    """Contiguous int32 tensors of one length on a device -> that length."""
+    n = {t.numel() for t in ts.values()}
+    for name, t in ts.items():
+        if t.dtype is not _I32 or t.get_device() != dev or dev < 0 or not t.is_contiguous() or len(n) != 1:
+            raise _lib.Invalid(f"{what}: {name} is a contiguous int32 CUDA tensor as long as the others")
+    return n.pop()
+
+
+def pages_moves(tokens, live):
+    """What a decode step over sequences moves -> (ids, moves), int32: moves (counts for the calls on pages) is 1 where live is not
+    0 and the token is not negative; ids are the tokens, 0 in the place of a negative one."""
+    dev = tokens.get_device()
+    n = _ints(dev, "pages_moves", tokens=tokens, live=live)
+    both = tokens.new_empty(2, n)
+    check(lib().fk_pages_moves(_contexts.get(dev) or context(tokens.device), _raw_stream(dev), tokens.data_ptr(), live.data_ptr(), n, both.data_ptr(),
+                               both.data_ptr() + 4 * n))
+    return both[0], both[1]
+
+
 def _list(ids):
     return (C.c_int * len(ids))(*ids)
 
@@ -787,6 +807,23 @@ def logit_rules(logits, history=None, penalties=None, bias=None, mask=None, out=
     check(lib().fk_logit_rules(ctx, _raw_stream(dev), x.data_ptr(), ld if n > 1 else V, n, V, hp, h,
                                pen.data_ptr() if pen is not None else None, bp, b_ld, mp, m_ld, o.data_ptr(), tokens.data_ptr()))
     return (o if logits.dim() == 2 else o[0]), tokens
+
+
+def tokens_join(tokens, moves=None, history=None, at=None):
+    """A step's tokens int32 [n], in place: -1 where moves [n] (None: all move) is 0.  With a history int32 [n, h] and at int64 [n]
+    the others that are not negative join their rows, history[s, at[s] % h] = token, and at counts on.  -> tokens"""
+    dev = tokens.get_device()
+    n = _ints(dev, "tokens_join", tokens=tokens) if moves is None else _ints(dev, "tokens_join", tokens=tokens, moves=moves)
+    h = 0
+    if history is not None:
+        h = history.shape[-1]
+        if history.dtype is not _I32 or history.get_device() != dev or history.shape != (n, h) or h < 1 or not history.is_contiguous():
+            raise _lib.Invalid("tokens_join: history is a contiguous int32 tensor [n, h] beside the tokens")
+        if at is None or at.dtype is not torch.int64 or at.get_device() != dev or at.shape != (n,) or not at.is_contiguous():
+            raise _lib.Invalid("tokens_join: at is a contiguous int64 tensor [n] beside the tokens")
+    check(lib().fk_tokens_join(_contexts.get(dev) or context(tokens.device), _raw_stream(dev), tokens.data_ptr(), None if moves is None else moves.data_ptr(), n,
+                               None if history is None else history.data_ptr(), h, None if at is None else at.data_ptr()))
+    return tokens
 
 
 def _rule_rows(t, dtype, dev, n, width, what):

@@ -414,6 +414,9 @@ size_t fk_pages_workspace(fk_ctx* ctx, int n_pages);
 int fk_pages_grow(fk_ctx* ctx, void* stream, const fk_pages* pages, const int* n_new_dev, int n_new);
 /* lens[s] += n_new_dev[s] (null: n_new): the step's tokens are in. */
 int fk_pages_advance(fk_ctx* ctx, void* stream, const fk_pages* pages, const int* n_new_dev, int n_new);
+/* What a decode step over n sequences moves: moves_dev[s] (the counts of the calls above and below) is 1 where live_dev[s] is not 0
+ * and the token is not negative, else 0; ids_dev[s] is the token, 0 in the place of a negative one.  Any n. */
+int fk_pages_moves(fk_ctx* ctx, void* stream, const int* tokens_dev, const int* live_dev, int n, int* ids_dev, int* moves_dev);
 /* Sequence dst[i] becomes the first n[i] tokens of src[i] (n null or n[i] < 0: all of them): whole pages are shared, the
  * last part of one is copied in every layer.  Host lists of m <= 64; a dst occurs once, is no src and holds nothing. */
 int fk_pages_fork(fk_ctx* ctx, void* stream, const fk_pages* pages, const int* src_host, const int* dst_host, const int* n_host, int m);
@@ -451,6 +454,10 @@ int fk_attention_paged(fk_ctx* ctx, void* stream, const fk_pages* pages, int lay
 int fk_logit_rules(fk_ctx* ctx, void* stream, const float* logits_dev, size_t ld, int n_rows, int vocab, const int* history_dev, int history,
                    const float* penalties_dev, const float* bias_dev, size_t bias_ld, const int* mask_dev, size_t mask_ld, float* out_dev,
                    int* tokens_dev);
+
+/* A step's tokens [n] in place: -1 where moves_dev[s] (null: none) is 0.  With a history (null: none) the others that are not
+ * negative join their rows: history_dev[s][at_dev[s] % history] = token, at_dev[s] += 1. */
+int fk_tokens_join(fk_ctx* ctx, void* stream, int* tokens_dev, const int* moves_dev, int n, int* history_dev, int history, int64_t* at_dev);
 
 /* ---- multi-GPU: peer-memory all-reduce ---------------------------------------
  * The reference is single-device (crates/frink-cuda/src/gpu.rs:219); these have no counterpart
