@@ -155,8 +155,8 @@ __global__ void advance_kernel(int* __restrict__ lens, int n_seqs, const int* __
     if (s < n_seqs) lens[s] += n_new_dev ? n_new_dev[s] : n_new;
 }
 
-// What a step moves: a launch's latency.  With the tokens' join (fk_logits.cu) in place of eight elementwise launches: the captured
-// step of a decoder of two layers, four sequences under rules, 112 -> 93 us (without rules 102 -> 91).
+// What a step moves: a launch's latency.  With the tokens' join (fk_logits.cu) in place of eleven elementwise launches: the captured
+// step of a decoder of two layers, four sequences under rules, 112 -> 93 us (without rules six, 102 -> 91).
 __global__ void moves_kernel(const int* __restrict__ tokens, const int* __restrict__ live, int n, int* __restrict__ ids, int* __restrict__ moves) {
     pdl_sync();
     const int s = blockIdx.x * blockDim.x + threadIdx.x;
